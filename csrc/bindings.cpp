@@ -3,6 +3,10 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <cmath>
+#include <string>
+#include <vector>
+
 #include "launchers.h"
 
 namespace {
@@ -708,6 +712,231 @@ void rope_append(Tensor qkv, Tensor pos, int64_t Hq, int64_t Hkv, Tensor cos_t, 
                   stream());
 }
 
+// ------------------------------------------------------------------------------------------------ block-wise KV cache
+// Numbers in messages go in as text: formatting them in a stream crashes where the extension carries a C++ library of its
+// own (linked statically) next to torch's.
+std::string num(int64_t n) { return std::to_string(n); }
+
+// Rows [T, heads, D] whose 16-byte pieces are aligned, or an aligned copy of them (a size-1 dimension's stride is free).
+Tensor aligned_rows(const Tensor& x, const char* what) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 3, what, " must be a CUDA tensor [tokens, heads, head_dim]");
+  CHECK_DTYPE(x, torch::kBFloat16);
+  bool ok = x.stride(2) == 1 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+  for (int i = 0; i < 2; ++i) ok = ok && (x.size(i) <= 1 || x.stride(i) % 8 == 0);
+  return ok ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+
+int kv_format(const Tensor& cache) {
+  if (cache.scalar_type() == torch::kFloat8_e4m3fn) return 0;
+  TORCH_CHECK(cache.scalar_type() == torch::kInt8, "the cache must be float8_e4m3fn or int8");
+  return 1;
+}
+
+qw::KvPages kv_pages(const Tensor& cache, const Tensor& scale, const char* what) {
+  TORCH_CHECK(cache.is_cuda() && cache.dim() == 4, what, " must be a CUDA tensor [blocks, kv_heads, block, head_dim]");
+  const int64_t D = cache.size(3);
+  TORCH_CHECK(D == 32 || D == 64 || D == 128, what, ": head_dim must be 32, 64 or 128, got ", num(D));
+  TORCH_CHECK(cache.size(2) % 16 == 0 && cache.size(2) > 0, what, ": a block holds a multiple of 16 tokens");
+  TORCH_CHECK(cache.size(0) * cache.size(2) < (int64_t{1} << 31), what, ": slots must fit 32 bits");
+  TORCH_CHECK(cache.size(1) < 32768, what, ": too many heads");
+  TORCH_CHECK(cache.stride(3) == 1 && cache.stride(2) >= D, what, ": a token's numbers must be consecutive");
+  bool ok = reinterpret_cast<uintptr_t>(cache.data_ptr()) % 16 == 0;
+  for (int i = 0; i < 3; ++i) ok = ok && (cache.size(i) <= 1 || cache.stride(i) % 16 == 0);
+  TORCH_CHECK(ok, what, ": storage and strides must be multiples of 16 bytes");
+  TORCH_CHECK(scale.is_cuda() && scale.scalar_type() == torch::kFloat32 && scale.dim() == 2 && scale.size(0) == cache.size(0) &&
+                  scale.size(1) == cache.size(1) && (scale.size(1) <= 1 || scale.stride(1) == 1),
+              what, ": scales must be float32 [blocks, kv_heads] with unit inner stride");
+  TORCH_CHECK(scale.device() == cache.device(), what, ": scales on another device");
+  return {cache.data_ptr(), cache.stride(0), cache.stride(1), cache.stride(2), scale.data_ptr<float>(), scale.stride(0)};
+}
+
+void check_caches(const Tensor& kc, const Tensor& vc) {
+  TORCH_CHECK(kc.sizes() == vc.sizes() && kc.scalar_type() == vc.scalar_type() && kc.device() == vc.device(),
+              "k_cache and v_cache must have one shape, dtype and device");
+}
+
+void check_ints(const Tensor& t, int64_t n, const at::Device& device, const char* what) {
+  TORCH_CHECK(t.device() == device && t.scalar_type() == torch::kInt32 && t.is_contiguous() && t.dim() == 1 && t.size(0) == n,
+              what, " must be a contiguous int32 tensor of ", num(n), " elements on ", device.str());
+}
+
+void check_table(const Tensor& t, int64_t B, const at::Device& device) {
+  TORCH_CHECK(t.device() == device && t.scalar_type() == torch::kInt32 && t.dim() == 2 && t.size(0) == B && t.size(1) >= 1 &&
+                  (t.size(1) == 1 || t.stride(1) == 1),
+              "block_table must be int32 [", num(B), ", width >= 1] with unit inner stride on ", device.str());
+}
+
+std::vector<Tensor> plan_blocks(Tensor cached_lens, Tensor new_lens, Tensor state, Tensor table, Tensor free_blocks,
+                                int64_t block, int64_t tokens) {
+  CHECK_CUDA(cached_lens);
+  const auto dev = cached_lens.device();
+  const int64_t B = cached_lens.numel();
+  check_ints(cached_lens, B, dev, "cached_lens");
+  check_ints(new_lens, B, dev, "new_lens");
+  check_ints(state, B + 1, dev, "state");
+  check_ints(free_blocks, free_blocks.numel(), dev, "free_blocks");
+  check_table(table, B, dev);
+  TORCH_CHECK(B <= qw::plan_max_requests(), "plan_blocks: at most ", num(qw::plan_max_requests()), " requests, got ", num(B));
+  TORCH_CHECK(block > 0 && block % 16 == 0 && block < (int64_t{1} << 31), "plan_blocks: a block holds a multiple of 16 tokens");
+  TORCH_CHECK(tokens >= 0 && tokens < (int64_t{1} << 30), "plan_blocks: bad token count ", num(tokens));
+  TORCH_CHECK(free_blocks.numel() * block < (int64_t{1} << 31), "plan_blocks: slots must fit 32 bits");
+  c10::cuda::CUDAGuard g(dev);
+  const auto opt = cached_lens.options();
+  auto query_start = torch::empty({B + 1}, opt), context = torch::empty({B}, opt), positions = torch::empty({tokens}, opt),
+       slots = torch::empty({tokens}, opt), state_out = torch::empty({B + 1}, opt), missing = torch::empty({1}, opt);
+  qw::plan_blocks(cached_lens.data_ptr<int>(), new_lens.data_ptr<int>(), state.data_ptr<int>(), table.data_ptr<int>(),
+                  table.stride(0), free_blocks.data_ptr<int>(), static_cast<int>(free_blocks.numel()), static_cast<int>(B),
+                  static_cast<int>(table.size(1)), static_cast<int>(block), static_cast<int>(tokens),
+                  query_start.data_ptr<int>(), context.data_ptr<int>(), positions.data_ptr<int>(), slots.data_ptr<int>(),
+                  state_out.data_ptr<int>(), missing.data_ptr<int>(), stream());
+  return {query_start, context, positions, slots, state_out, missing};
+}
+
+void release_blocks(Tensor keep_lens, Tensor state, Tensor table, Tensor free_blocks, int64_t block) {
+  CHECK_CUDA(keep_lens);
+  const auto dev = keep_lens.device();
+  const int64_t B = keep_lens.numel();
+  check_ints(keep_lens, B, dev, "keep_lens");
+  check_ints(state, B + 1, dev, "state");
+  check_ints(free_blocks, free_blocks.numel(), dev, "free_blocks");
+  check_table(table, B, dev);
+  TORCH_CHECK(block > 0 && block % 16 == 0 && block < (int64_t{1} << 31), "release_blocks: a block holds a multiple of 16 tokens");
+  c10::cuda::CUDAGuard g(dev);
+  qw::release_blocks(keep_lens.data_ptr<int>(), state.data_ptr<int>(), table.data_ptr<int>(), table.stride(0),
+                     free_blocks.data_ptr<int>(), static_cast<int>(free_blocks.numel()), static_cast<int>(B),
+                     static_cast<int>(table.size(1)), static_cast<int>(block), stream());
+}
+
+void append_kv(Tensor k, Tensor v, Tensor slots, Tensor kc, Tensor vc, Tensor ks, Tensor vs) {
+  check_caches(kc, vc);
+  const int fmt = kv_format(kc);
+  const auto pk = kv_pages(kc, ks, "k_cache"), pv = kv_pages(vc, vs, "v_cache");
+  c10::cuda::CUDAGuard g(kc.device());
+  k = aligned_rows(k, "k");
+  v = aligned_rows(v, "v");
+  const int64_t T = k.size(0), Hkv = kc.size(1), D = kc.size(3);
+  TORCH_CHECK(k.size(1) == Hkv && k.size(2) == D && v.sizes() == k.sizes(), "append_kv: k and v must be [tokens, ", num(Hkv), ", ", num(D), "]");
+  TORCH_CHECK(k.device() == kc.device() && v.device() == kc.device(), "append_kv: k and v must be on the cache's device");
+  TORCH_CHECK(T < (int64_t{1} << 30), "append_kv: too many tokens");
+  check_ints(slots, T, kc.device(), "slot_map");
+  qw::append_kv({bptr(k), k.stride(0), k.stride(1)}, {bptr(v), v.stride(0), v.stride(1)}, slots.data_ptr<int>(), pk, pv,
+                static_cast<int>(T), static_cast<int>(Hkv), static_cast<int>(D), static_cast<int>(kc.size(2)),
+                static_cast<int>(kc.size(0)), fmt, stream());
+}
+
+Tensor cached_attention(Tensor q, Tensor kc, Tensor vc, Tensor ks, Tensor vs, Tensor table, Tensor context,
+                        Tensor query_start, int64_t max_query, int64_t max_context, double scale, OptT out_) {
+  check_caches(kc, vc);
+  const int fmt = kv_format(kc);
+  const auto pk = kv_pages(kc, ks, "k_cache"), pv = kv_pages(vc, vs, "v_cache");
+  c10::cuda::CUDAGuard g(kc.device());
+  q = aligned_rows(q, "q");
+  const int64_t T = q.size(0), Hq = q.size(1), Hkv = kc.size(1), D = kc.size(3), B = context.numel();
+  TORCH_CHECK(q.device() == kc.device() && q.size(2) == D, "cached_attention: q must be [tokens, heads, ", num(D), "] on the cache's device");
+  TORCH_CHECK(Hkv > 0 && Hq % Hkv == 0 && Hq < 65536, "cached_attention: the query heads (", num(Hq), ") must be a multiple of the kv heads (", num(Hkv), ")");
+  TORCH_CHECK(T < (int64_t{1} << 30) && T * Hq < (int64_t{1} << 33), "cached_attention: too many tokens");
+  TORCH_CHECK(max_query >= 1 && max_context >= 1 && max_query < (int64_t{1} << 31) && max_context < (int64_t{1} << 31),
+              "cached_attention: max_query and max_context must be positive");
+  TORCH_CHECK(scale > 0 && std::isfinite(scale), "cached_attention: the scale must be positive");
+  check_ints(context, B, kc.device(), "context_lens");
+  check_ints(query_start, B + 1, kc.device(), "query_start");
+  check_table(table, B, kc.device());
+  Tensor out = out_ && out_->defined() ? *out_ : torch::empty({T, Hq, D}, q.options());
+  TORCH_CHECK(out.device() == kc.device() && out.scalar_type() == torch::kBFloat16 && out.sizes() == q.sizes() &&
+                  (D <= 1 || out.stride(2) == 1) && reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0 &&
+                  (out.size(0) <= 1 || out.stride(0) % 8 == 0) && (out.size(1) <= 1 || out.stride(1) % 8 == 0),
+              "cached_attention: out must be bfloat16 like q, its rows consecutive and aligned to 16 bytes");
+  if (T == 0) return out;
+  auto ws = torch::empty({qw::cached_attention_workspace(T, B, Hq, Hkv, D, max_query, max_context)},
+                         q.options().dtype(torch::kUInt8));
+  qw::cached_attention(bptr(q), q.stride(0), q.stride(1), bptr_mut(out), out.stride(0), out.stride(1), pk, pv,
+                       table.data_ptr<int>(), table.stride(0), context.data_ptr<int>(), query_start.data_ptr<int>(),
+                       static_cast<int>(T), static_cast<int>(B), static_cast<int>(Hq), static_cast<int>(Hkv),
+                       static_cast<int>(D), static_cast<int>(kc.size(2)), static_cast<int>(kc.size(0)),
+                       static_cast<int>(table.size(1)), static_cast<int>(max_query), static_cast<int>(max_context),
+                       static_cast<float>(scale), fmt, ws.data_ptr(), stream());
+  return out;
+}
+
+// ------------------------------------------------------------------------------------------------ logits
+const int* opt_ints(const OptT& t, int64_t n, const at::Device& device, const char* what) {
+  if (!t || !t->defined()) return nullptr;
+  check_ints(*t, n, device, what);
+  return t->data_ptr<int>();
+}
+const float* opt_floats(const OptT& t, int64_t n, const at::Device& device, const char* what) {
+  if (!t || !t->defined()) return nullptr;
+  TORCH_CHECK(t->device() == device && t->scalar_type() == torch::kFloat32 && t->is_contiguous() && t->dim() == 1 && t->size(0) == n,
+              what, " must be a contiguous float32 tensor of ", num(n), " elements on ", device.str());
+  return t->data_ptr<float>();
+}
+
+Tensor process_logits(Tensor logits, OptT history, OptT history_lens, OptT prompt_lens, OptT repetition, OptT frequency,
+                      OptT presence, OptT bias, OptT bias_rows, OptT mask, OptT mask_rows, OptT out_) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.size(1) <= 1 || logits.stride(1) == 1),
+              "process_logits: logits must be a CUDA tensor [rows, vocab] with unit inner stride");
+  const auto dev = logits.device();
+  const int64_t rows = logits.size(0), vocab = logits.size(1);
+  TORCH_CHECK(rows <= 65535 && vocab < (int64_t{1} << 30), "process_logits: at most 65535 rows");
+  qw::LogitsArgs a{};
+  const auto dt = logits.scalar_type();
+  TORCH_CHECK(dt == torch::kFloat32 || dt == torch::kBFloat16 || dt == torch::kFloat16,
+              "process_logits: logits must be float32, bfloat16 or float16");
+  a.dtype = dt == torch::kFloat32 ? 0 : dt == torch::kBFloat16 ? 1 : 2;
+  c10::cuda::CUDAGuard g(dev);
+  Tensor out = out_ && out_->defined() ? *out_ : torch::empty({rows, vocab}, logits.options());
+  TORCH_CHECK(out.device() == dev && out.scalar_type() == dt && out.sizes() == logits.sizes() &&
+                  (vocab <= 1 || out.stride(1) == 1) && (rows <= 1 || out.stride(0) >= vocab),
+              "process_logits: out must be like logits");
+  if (rows == 0 || vocab == 0) return out;
+  if (history && history->defined()) {
+    TORCH_CHECK(history->device() == dev && history->scalar_type() == torch::kInt32 && history->dim() == 2 &&
+                    history->size(0) == rows && (history->size(1) <= 1 || history->stride(1) == 1) && history->size(1) < (int64_t{1} << 31),
+                "process_logits: history must be int32 [rows, length] with unit inner stride");
+    TORCH_CHECK(history_lens && history_lens->defined(), "process_logits: history needs history_lens");
+    a.history = history->data_ptr<int>();
+    a.history_stride = history->stride(0);
+    a.history_width = static_cast<int>(history->size(1));
+    a.history_lens = opt_ints(history_lens, rows, dev, "history_lens");
+    a.prompt_lens = opt_ints(prompt_lens, rows, dev, "prompt_lens");
+    a.repetition = opt_floats(repetition, rows, dev, "repetition");
+    a.frequency = opt_floats(frequency, rows, dev, "frequency");
+    a.presence = opt_floats(presence, rows, dev, "presence");
+    if (!a.repetition && !a.frequency && !a.presence) a.history = nullptr;
+  } else {
+    TORCH_CHECK(!(repetition && repetition->defined()) && !(frequency && frequency->defined()) && !(presence && presence->defined()),
+                "process_logits: penalties need the history");
+  }
+  if (bias && bias->defined()) {
+    TORCH_CHECK(bias->device() == dev && bias->scalar_type() == torch::kFloat32 && bias->dim() == 2 && bias->size(1) == vocab &&
+                    (vocab <= 1 || bias->stride(1) == 1),
+                "process_logits: bias must be float32 [biases, vocab] with unit inner stride");
+    a.bias = bias->data_ptr<float>();
+    a.bias_stride = bias->stride(0);
+    a.biases = static_cast<int>(bias->size(0));
+    a.bias_rows = opt_ints(bias_rows, rows, dev, "bias_rows");
+    TORCH_CHECK(a.bias_rows || bias->size(0) == rows, "process_logits: bias without bias_rows needs one row per logits row");
+  }
+  if (mask && mask->defined()) {
+    TORCH_CHECK(mask->device() == dev && mask->scalar_type() == torch::kInt32 && mask->dim() == 2 &&
+                    mask->size(1) == (vocab + 31) / 32 && (mask->size(1) <= 1 || mask->stride(1) == 1),
+                "process_logits: mask must be int32 [masks, ceil(vocab / 32)] with unit inner stride");
+    a.mask = reinterpret_cast<const uint32_t*>(mask->data_ptr<int>());
+    a.mask_stride = mask->stride(0);
+    a.masks = static_cast<int>(mask->size(0));
+    a.mask_rows = opt_ints(mask_rows, rows, dev, "mask_rows");
+    TORCH_CHECK(a.mask_rows || mask->size(0) == rows, "process_logits: mask without mask_rows needs one row per logits row");
+  }
+  a.logits = logits.data_ptr();
+  a.ld = logits.stride(0);
+  a.out = out.data_ptr();
+  a.ldo = out.stride(0);
+  a.rows = static_cast<int>(rows);
+  a.vocab = static_cast<int>(vocab);
+  qw::process_logits(a, stream());
+  return out;
+}
+
 // ------------------------------------------------------------------------------------------------ status
 int64_t read_status(bool clear) {
   int s = qw::gemm_status(clear);
@@ -723,6 +952,7 @@ int64_t read_status(bool clear) {
   if ((t = qw::p2p_status(clear)) && !s) s = t;
   if ((t = qw::tp_status(clear)) && !s) s = t;
   if ((t = qw::decode_status(clear)) && !s) s = t;
+  if ((t = qw::cached_attention_status(clear)) && !s) s = t;
   return s;
 }
 
@@ -781,6 +1011,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("decode_attention", &decode_attention);
   m.def("rope_append", &rope_append);
   m.def("decode_attention_rope", &decode_attention_rope);
+  m.def("plan_blocks", &plan_blocks);
+  m.def("release_blocks", &release_blocks);
+  m.def("append_kv", &append_kv);
+  m.def("cached_attention", &cached_attention);
+  m.def("process_logits", &process_logits);
   m.def("ep_dispatch", &ep_dispatch);
   m.def("zero_rs_blocks", &zero_rs_blocks);
   m.def("zero_reduce_scatter", &zero_reduce_scatter);

@@ -16,26 +16,11 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "launch.cuh"
 #include "launchers.h"
 
 namespace qw {
 namespace {
-
-template <typename... KArgs, typename... Args>
-void launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const char* what,
-                Args&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  check_cuda(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...), what);
-}
 
 __device__ __forceinline__ void bf16x8_to_float(const uint4& raw, float* v) {
   const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);

@@ -1,0 +1,429 @@
+// The block-wise KV cache's bookkeeping and its quantising write.
+//
+//  * plan_blocks: block tables, slot maps, positions and query offsets of a step from the requests' lengths. The block
+//    pool lives on the device (a stack of free block ids and its height), so a captured step allocates its own blocks.
+//  * release_blocks: blocks of finished (or cut) requests back onto the stack.
+//  * append_kv: new keys and values into their slots in 8 bits (kv_format.cuh), one scale per block and head.
+#include <algorithm>
+
+#include "common.cuh"
+#include "kv_format.cuh"
+#include "launch.cuh"
+#include "launchers.h"
+
+namespace qw {
+namespace {
+
+constexpr int kPlanThreads = 256;
+constexpr int kPlanTokens = 1024;  // tokens of a block of threads
+
+// Exclusive sum over the block's threads; `total` gets the sum. Two barriers inside, one after.
+__device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    int s = lane < kPlanThreads / 32 ? warp_sums[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < kPlanThreads / 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += y;
+    }
+    if (lane < kPlanThreads / 32) warp_sums[lane] = s;
+  }
+  __syncthreads();
+  total = warp_sums[kPlanThreads / 32 - 1];
+  const int before = warp > 0 ? warp_sums[warp - 1] : 0;
+  __syncthreads();
+  return before + x - v;
+}
+
+struct PlanArgs {
+  const int* cached;
+  const int* fresh;
+  const int* state;  // [1 + B]: free blocks, then the blocks that each request holds
+  int* table;
+  int64_t table_stride;
+  const int* free_blocks;
+  int capacity;  // of free_blocks
+  int B, width, block, tokens;
+  int* query_start;
+  int* context;
+  int* positions;
+  int* slots;
+  int* state_out;
+  int* missing;
+};
+
+__device__ __forceinline__ int clamp_len(int64_t v) {
+  return static_cast<int>(v < 0 ? 0 : (v > 0x7fffffff ? 0x7fffffff : v));
+}
+
+struct Need {
+  int held, fits, wanted;
+};
+
+__device__ __forceinline__ Need need_of(const PlanArgs& a, int b) {
+  const int64_t total = static_cast<int64_t>(max(a.cached[b], 0)) + max(a.fresh[b], 0);
+  Need n;
+  n.wanted = static_cast<int>((total + a.block - 1) / a.block);
+  n.fits = min(n.wanted, a.width);
+  n.held = min(max(a.state[1 + b], 0), a.width);
+  return n;
+}
+
+// Two prefix sums over the requests (tokens, and blocks to take), which every block of threads does for itself: at a
+// few hundred requests they cost less than a second launch. Then the work is spread over the blocks: the tokens' slots
+// and positions by ranges, the tables' new entries by requests. A token's slot in a new block comes from the free list
+// itself, not from the table, so that no block reads an entry that another one writes.
+// Bound by the latency of the dependent reads (lengths, then tables, then slots), not by its few bytes.
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(PlanArgs a) {
+  extern __shared__ int plan_smem[];
+  int* start = plan_smem;           // [B + 1]
+  int* rank = plan_smem + a.B + 1;  // [B]
+  __shared__ int sums[kPlanThreads / 32];
+  __shared__ int s_short[kPlanThreads / 32];
+  griddep_wait();
+  griddep_launch();
+  const int per = (a.B + kPlanThreads - 1) / kPlanThreads;
+  const int b0 = min(static_cast<int>(threadIdx.x) * per, a.B), b1 = min(b0 + per, a.B);
+  int tokens = 0, blocks = 0, narrow = 0;
+  for (int b = b0; b < b1; ++b) {
+    const Need n = need_of(a, b);
+    tokens += max(a.fresh[b], 0);
+    blocks += max(n.fits - n.held, 0);
+    narrow += n.wanted - n.fits;
+  }
+  int all_tokens, all_blocks;
+  int t = block_scan(tokens, sums, all_tokens);
+  int r = block_scan(blocks, sums, all_blocks);
+  for (int b = b0; b < b1; ++b) {
+    const Need n = need_of(a, b);
+    start[b] = t;
+    rank[b] = r;
+    t += max(a.fresh[b], 0);
+    r += max(n.fits - n.held, 0);
+  }
+  if (threadIdx.x == 0) start[a.B] = all_tokens;
+  const int free = min(max(a.state[0], 0), a.capacity);
+  __syncthreads();
+
+  if (blockIdx.x == 0) {
+    for (int b = b0; b < b1; ++b) {
+      const Need n = need_of(a, b);
+      a.query_start[b] = start[b];
+      a.context[b] = clamp_len(static_cast<int64_t>(max(a.cached[b], 0)) + max(a.fresh[b], 0));
+      a.state_out[1 + b] = n.held + min(max(n.fits - n.held, 0), max(free - rank[b], 0));
+    }
+    int sum = narrow;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (threadIdx.x % 32 == 0) s_short[threadIdx.x / 32] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      int m = all_blocks - min(all_blocks, free);
+      for (int w = 0; w < kPlanThreads / 32; ++w) m += s_short[w];
+      a.query_start[a.B] = all_tokens;
+      a.state_out[0] = free - min(all_blocks, free);
+      a.missing[0] = m;
+    }
+  }
+  // new table entries: a warp per request
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  for (int b = blockIdx.x * (kPlanThreads / 32) + warp; b < a.B; b += gridDim.x * (kPlanThreads / 32)) {
+    const Need n = need_of(a, b);
+    for (int e = n.held + lane; e < n.fits; e += 32) {
+      const int k = rank[b] + e - n.held;
+      a.table[b * a.table_stride + e] = k < free ? a.free_blocks[free - 1 - k] : -1;
+    }
+  }
+  // slots and positions: kPlanTokens consecutive tokens per turn, neighbouring threads on neighbouring tokens
+  for (int base = blockIdx.x * kPlanTokens; base < a.tokens; base += gridDim.x * kPlanTokens) {
+    for (int i = threadIdx.x; i < kPlanTokens && base + i < a.tokens; i += kPlanThreads) {
+      const int tok = base + i;
+      int slot = -1, pos = 0;
+      if (tok < all_tokens) {
+        int lo = 0, hi = a.B;  // the last request whose start is <= tok
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (start[mid] <= tok) lo = mid;
+          else hi = mid;
+        }
+        const int b = lo;
+        const Need n = need_of(a, b);
+        pos = clamp_len(static_cast<int64_t>(tok - start[b]) + max(a.cached[b], 0));
+        const int e = pos / a.block;
+        int id = -1;
+        if (e < n.held) {
+          id = a.table[b * a.table_stride + e];
+        } else if (e < n.fits) {
+          const int k = rank[b] + e - n.held;
+          if (k < free) id = a.free_blocks[free - 1 - k];
+        }
+        if (id >= 0) slot = id * a.block + pos % a.block;
+      }
+      a.positions[tok] = pos;
+      a.slots[tok] = slot;
+    }
+  }
+}
+
+// One block of threads: a request's entries past its kept tokens go onto the stack, requests in order.
+__global__ void __launch_bounds__(kPlanThreads) release_kernel(const int* keep, int* state, int* table,
+                                                               int64_t table_stride, int* free_blocks, int capacity,
+                                                               int B, int width, int block) {
+  __shared__ int sums[kPlanThreads / 32];
+  griddep_wait();
+  griddep_launch();
+  const int per = (B + kPlanThreads - 1) / kPlanThreads;
+  const int b0 = min(static_cast<int>(threadIdx.x) * per, B), b1 = min(b0 + per, B);
+  auto kept = [&](int b, int held) {
+    return keep[b] < 0 ? held : min(held, static_cast<int>((static_cast<int64_t>(keep[b]) + block - 1) / block));
+  };
+  int n = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int held = min(max(state[1 + b], 0), width);
+    n += held - kept(b, held);
+  }
+  int total;
+  int at = block_scan(n, sums, total) + min(max(state[0], 0), capacity);
+  for (int b = b0; b < b1; ++b) {
+    const int held = min(max(state[1 + b], 0), width), k = kept(b, held);
+    for (int e = k; e < held; ++e, ++at) {
+      if (at < capacity) free_blocks[at] = table[b * table_stride + e];
+      table[b * table_stride + e] = -1;
+    }
+    state[1 + b] = k;
+  }
+  __syncthreads();  // every thread has read state[0]
+  if (threadIdx.x == 0) state[0] = min(min(max(state[0], 0), capacity) + total, capacity);
+}
+
+// ------------------------------------------------------------------------------------------------ append
+struct AppendArgs {
+  const bf16* x[2];  // keys, values: [T, Hkv, D]
+  int64_t token_stride[2], head_stride[2];
+  const int* slots;
+  uint8_t* cache[2];  // [blocks, Hkv, block, D]
+  int64_t c_block[2], c_head[2], c_token[2];
+  float* scale[2];  // [blocks, Hkv]
+  int64_t s_block[2];
+  int T, Hkv, block, blocks, rows;  // rows: tokens of a block of threads
+};
+
+constexpr int kAppendThreads = 128;
+constexpr int kKeep = 8;  // 16-byte pieces of a run that a thread keeps between its two passes
+
+__device__ __forceinline__ float finite_abs(float v) {
+  const float a = fabsf(v);
+  return a <= 3.4028234e38f ? a : 0.f;  // infinities saturate and NaN is no size: neither sets a block's scale
+}
+
+__device__ __forceinline__ float amax8(const uint4& w) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __bfloat1622float2(h[i]);
+    m = fmaxf(m, fmaxf(finite_abs(f.x), finite_abs(f.y)));
+  }
+  return m;
+}
+
+template <int FMT>
+__device__ __forceinline__ uint2 encode8(const uint4& w, float inv) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
+  const float2 a = __bfloat1622float2(h[0]), b = __bfloat1622float2(h[1]), c = __bfloat1622float2(h[2]),
+               d = __bfloat1622float2(h[3]);
+  return make_uint2(Kv<FMT>::encode4(a.x * inv, a.y * inv, b.x * inv, b.y * inv),
+                    Kv<FMT>::encode4(c.x * inv, c.y * inv, d.x * inv, d.y * inv));
+}
+
+// The tokens [t0, t0 + n) of one (block, head), written by NT threads (a warp or the whole block of threads).
+template <int FMT, int D, int NT>
+__device__ __forceinline__ void append_run(const AppendArgs& a, int kv, int h, int t0, int n, int me, float* red) {
+  constexpr int PPR = D / 8;  // 16-byte pieces of a token's row
+  const int slot0 = a.slots[t0];
+  const int64_t id = slot0 / a.block;
+  const int first = slot0 - static_cast<int>(id) * a.block;
+  const bf16* x = (kv ? a.x[1] : a.x[0]) + h * (kv ? a.head_stride[1] : a.head_stride[0]);
+  const int64_t ts = kv ? a.token_stride[1] : a.token_stride[0];
+  const int64_t ct = kv ? a.c_token[1] : a.c_token[0];
+  uint8_t* rows = (kv ? a.cache[1] : a.cache[0]) + id * (kv ? a.c_block[1] : a.c_block[0]) + h * (kv ? a.c_head[1] : a.c_head[0]);
+  float* sp = (kv ? a.scale[1] : a.scale[0]) + id * (kv ? a.s_block[1] : a.s_block[0]) + h;
+  const float old = first > 0 ? *sp : 0.f;
+  const int pieces = n * PPR;
+  auto source = [&](int i) {
+    return reinterpret_cast<const uint4*>(x + static_cast<int64_t>(t0 + i / PPR) * ts + (i % PPR) * 8);
+  };
+  uint4 keep[kKeep];
+  float m = 0.f;
+#pragma unroll
+  for (int k = 0; k < kKeep; ++k)
+    if (me + k * NT < pieces) keep[k] = __ldg(source(me + k * NT));
+#pragma unroll
+  for (int k = 0; k < kKeep; ++k)
+    if (me + k * NT < pieces) m = fmaxf(m, amax8(keep[k]));
+  for (int i = me + kKeep * NT; i < pieces; i += NT) m = fmaxf(m, amax8(__ldg(source(i))));
+  m = warp_max(m);
+  if constexpr (NT > 32) {
+    if (me % 32 == 0) red[me / 32] = m;
+    __syncthreads();
+    m = red[0];
+#pragma unroll
+    for (int w = 1; w < NT / 32; ++w) m = fmaxf(m, red[w]);
+  }
+  int e = scale_exponent<FMT>(m);
+  if (old > 0.f && old <= 3.4028234e38f) {  // a held scale stays unless the new tokens need a larger one (a scale that is no power of two: the next)
+    int xo;
+    const float mo = frexpf(old, &xo);
+    e = max(e, mo == 0.5f ? xo - 1 : xo);
+  }
+  e = min(e, 126);
+  const float scale = exp2i(e), inv = exp2i(-e);
+  if (first > 0 && old != scale) {  // the tokens that the block holds, onto the new scale
+    const float ratio = old * inv;
+    for (int i = me; i < first * (D / 4); i += NT) {
+      uint32_t* p = reinterpret_cast<uint32_t*>(rows + (i / (D / 4)) * ct + (i % (D / 4)) * 4);
+      uint32_t lo, hi;
+      Kv<FMT>::decode4(*p, lo, hi);
+      const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+      *p = Kv<FMT>::encode4(u.x * ratio, u.y * ratio, v.x * ratio, v.y * ratio);
+    }
+  }
+  auto put = [&](int i, const uint4& w) {
+    const int s = a.slots[t0 + i / PPR] - static_cast<int>(id) * a.block;
+    *reinterpret_cast<uint2*>(rows + s * ct + (i % PPR) * 8) = encode8<FMT>(w, inv);
+  };
+#pragma unroll
+  for (int k = 0; k < kKeep; ++k)
+    if (me + k * NT < pieces) put(me + k * NT, keep[k]);
+  for (int i = me + kKeep * NT; i < pieces; i += NT) put(i, __ldg(source(i)));
+  if constexpr (NT > 32) __syncthreads();  // `red` and the old scale have been read
+  else __syncwarp();
+  if (me == 0) *sp = scale;
+}
+
+// A block of threads owns the runs (neighbouring tokens of one cache block) that begin in its `rows` tokens, for one
+// head of the keys or the values: one owner per (cache block, head), so the scale needs no atomics. With few runs all
+// threads share one, with many (decode: every token is a run) each warp takes its own. A run is read once: its pieces
+// stay in registers between the search for the largest magnitude and the rounding (up to 64 tokens of 128 numbers; the
+// rest of a longer one is read again, from L1 or L2).
+// Bound by HBM for prompts (2 bytes read, 1 written per number), by the latency of two dependent reads for decode.
+template <int FMT, int D>
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(AppendArgs a) {
+  __shared__ int s_first[kAppendThreads];
+  __shared__ int s_n;
+  __shared__ float s_red[kAppendThreads / 32];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  griddep_wait();
+  griddep_launch();
+  const int kv = blockIdx.y & 1, h = blockIdx.y >> 1;
+  const int r0 = blockIdx.x * a.rows, r1 = min(r0 + a.rows, a.T);
+  if (threadIdx.x == 0) s_n = 0;
+  __syncthreads();
+  // the cache block of a token; -1: none (padding, or a slot that the cache does not have)
+  auto block_of = [&](int t) {
+    const int s = a.slots[t];
+    if (s < 0) return -1;
+    const int id = s / a.block;
+    return id < a.blocks ? id : -1;
+  };
+  for (int t = r0 + threadIdx.x; t < r1; t += kAppendThreads) {
+    const int id = block_of(t);
+    if (id < 0 || (t > 0 && block_of(t - 1) == id)) continue;
+    s_first[atomicAdd(&s_n, 1)] = t;  // the order of the runs does not matter: each is a block of its own
+  }
+  __syncthreads();
+  const int runs = s_n;
+  auto length = [&](int t) {  // tokens of the run that begins at t; whole warps call it
+    const int id = block_of(t);
+    int n = 1;
+    while (true) {
+      const int u = t + n + lane;
+      const unsigned same = __ballot_sync(0xffffffffu, u < a.T && n + lane < a.block && block_of(u) == id);
+      n += __ffs(~same) ? __ffs(~same) - 1 : 32;
+      if (same != 0xffffffffu) return n;
+    }
+  };
+  if (runs >= kAppendThreads / 32) {
+    for (int i = warp; i < runs; i += kAppendThreads / 32)
+      append_run<FMT, D, 32>(a, kv, h, s_first[i], length(s_first[i]), lane, nullptr);
+  } else {
+    for (int i = 0; i < runs; ++i) {
+      const int n = length(s_first[i]);
+      if (n * (D / 8) <= 32) {  // a short one: a warp is enough
+        if (warp == i) append_run<FMT, D, 32>(a, kv, h, s_first[i], n, lane, nullptr);
+      } else {
+        append_run<FMT, D, kAppendThreads>(a, kv, h, s_first[i], n, threadIdx.x, s_red);
+      }
+    }
+  }
+}
+
+template <int FMT>
+void append_launch(const AppendArgs& a, int D, dim3 grid, cudaStream_t stream) {
+  if (D == 32) launch_pdl(append_kernel<FMT, 32>, grid, dim3(kAppendThreads), 0, stream, "append_kv", a);
+  else if (D == 64) launch_pdl(append_kernel<FMT, 64>, grid, dim3(kAppendThreads), 0, stream, "append_kv", a);
+  else launch_pdl(append_kernel<FMT, 128>, grid, dim3(kAppendThreads), 0, stream, "append_kv", a);
+}
+
+}  // namespace
+
+int plan_max_requests() { return 4096; }
+
+void plan_blocks(const int* cached, const int* fresh, const int* state, int* table, int64_t table_stride,
+                 const int* free_blocks, int capacity, int B, int width, int block, int tokens, int* query_start,
+                 int* context, int* positions, int* slots, int* state_out, int* missing, cudaStream_t stream) {
+  PlanArgs a{cached, fresh, state, table, table_stride, free_blocks, capacity, B, width, block, tokens,
+             query_start, context, positions, slots, state_out, missing};
+  const int grid = std::min(148, std::max((tokens + kPlanTokens - 1) / kPlanTokens, (B + 63) / 64));
+  launch_pdl(plan_kernel, dim3(std::max(grid, 1)), dim3(kPlanThreads), static_cast<size_t>(2 * B + 1) * sizeof(int), stream,
+             "plan_blocks", a);
+}
+
+void release_blocks(const int* keep, int* state, int* table, int64_t table_stride, int* free_blocks, int capacity, int B,
+                    int width, int block, cudaStream_t stream) {
+  if (B == 0) return;
+  launch_pdl(release_kernel, dim3(1), dim3(kPlanThreads), 0, stream, "release_blocks", keep, state, table, table_stride,
+             free_blocks, capacity, B, width, block);
+}
+
+void append_kv(const KvSource& k, const KvSource& v, const int* slots, const KvPages& kc, const KvPages& vc, int T, int Hkv,
+               int D, int block, int blocks, int fmt, cudaStream_t stream) {
+  if (T == 0) return;
+  AppendArgs a{};
+  const KvSource* src[2] = {&k, &v};
+  const KvPages* dst[2] = {&kc, &vc};
+  for (int i = 0; i < 2; ++i) {
+    a.x[i] = src[i]->x;
+    a.token_stride[i] = src[i]->token_stride;
+    a.head_stride[i] = src[i]->head_stride;
+    a.cache[i] = static_cast<uint8_t*>(const_cast<void*>(dst[i]->codes));
+    a.c_block[i] = dst[i]->block_stride;
+    a.c_head[i] = dst[i]->head_stride;
+    a.c_token[i] = dst[i]->token_stride;
+    a.scale[i] = const_cast<float*>(dst[i]->scale);
+    a.s_block[i] = dst[i]->scale_stride;
+  }
+  a.slots = slots;
+  a.T = T;
+  a.Hkv = Hkv;
+  a.block = block;
+  a.blocks = blocks;
+  // few tokens: one per block of threads, for latency; many: up to a cache block of them, so that a prompt's runs are
+  // found by one owner each without a block of threads per token
+  a.rows = std::max(1, std::min(std::min(block, kAppendThreads), static_cast<int>(static_cast<int64_t>(T) * Hkv * 2 / (148 * 8))));
+  const dim3 grid((T + a.rows - 1) / a.rows, Hkv * 2);
+  if (fmt == kKvFp8) append_launch<kKvFp8>(a, D, grid, stream);
+  else append_launch<kKvInt8>(a, D, grid, stream);
+}
+
+}  // namespace qw

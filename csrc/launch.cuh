@@ -1,0 +1,29 @@
+// Launch with programmatic dependent launch: the kernel may be scheduled while its predecessor in the stream drains and
+// waits for it with griddep_wait() (common.cuh).
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <utility>
+
+#include "launchers.h"
+
+namespace qw {
+
+template <typename... KArgs, typename... Args>
+void launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const char* what,
+                Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  check_cuda(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...), what);
+}
+
+}  // namespace qw

@@ -219,6 +219,60 @@ int decode_status(bool clear);
 // bf16 copy of int4 (fmt 2, grouped fp16 scales) / int8 (fmt 1, per-row fp16 scale) weight rows
 void dequant_rows(const void* q, const void* scales, int64_t rows, int K, int group, int fmt, bf16* out,
                   cudaStream_t stream);
+// ---- kv_cache.cu (block-wise 8-bit KV cache: plan, release, quantising write) ----
+struct KvSource {  // new keys or values [T, Hkv, D]; strides in elements
+  const bf16* x;
+  int64_t token_stride, head_stride;
+};
+struct KvPages {  // [blocks, Hkv, block, D] codes and [blocks, Hkv] scales; strides in elements
+  const void* codes;
+  int64_t block_stride, head_stride, token_stride;
+  const float* scale;
+  int64_t scale_stride;
+};
+int plan_max_requests();
+void plan_blocks(const int* cached, const int* fresh, const int* state, int* table, int64_t table_stride,
+                 const int* free_blocks, int capacity, int B, int width, int block, int tokens, int* query_start,
+                 int* context, int* positions, int* slots, int* state_out, int* missing, cudaStream_t stream);
+void release_blocks(const int* keep, int* state, int* table, int64_t table_stride, int* free_blocks, int capacity, int B,
+                    int width, int block, cudaStream_t stream);
+void append_kv(const KvSource& k, const KvSource& v, const int* slots, const KvPages& kc, const KvPages& vc, int T, int Hkv,
+               int D, int block, int blocks, int fmt, cudaStream_t stream);
+// ---- cached_attention.cu ----
+// attention of q [T, Hq, D] over the cache; the query heads of a kv head are consecutive
+void cached_attention(const bf16* q, int64_t q_token, int64_t q_head, bf16* out, int64_t o_token, int64_t o_head,
+                      const KvPages& k, const KvPages& v, const int* table, int64_t table_stride, const int* context,
+                      const int* query_start, int T, int B, int Hq, int Hkv, int D, int block, int blocks, int width,
+                      int max_query, int max_context, float scale, int fmt, void* workspace, cudaStream_t stream);
+// bytes of the workspace for these sizes
+int64_t cached_attention_workspace(int T, int B, int Hq, int Hkv, int D, int max_query, int max_context);
+int cached_attention_status(bool clear);
+// ---- logits.cu ----
+struct LogitsArgs {
+  const void* logits;
+  int64_t ld;
+  void* out;
+  int64_t ldo;
+  int dtype;  // 0 fp32, 1 bf16, 2 fp16
+  int rows, vocab;
+  const int* history;  // [rows, width], or null
+  int64_t history_stride;
+  int history_width;
+  const int* history_lens;
+  const int* prompt_lens;
+  const float* repetition;
+  const float* frequency;
+  const float* presence;
+  const float* bias;  // [biases, vocab], or null
+  int64_t bias_stride;
+  int biases;
+  const int* bias_rows;  // [rows]; null: row r has bias row r
+  const uint32_t* mask;  // [masks, ceil(vocab / 32)], or null
+  int64_t mask_stride;
+  int masks;
+  const int* mask_rows;
+};
+void process_logits(const LogitsArgs& a, cudaStream_t stream);
 // expert-parallel decode exchange (ep_decode.cu)
 void ep_decode_tick(int* step, cudaStream_t stream);
 void ep_decode_push(const bf16* y, const int* slot, const float* top_w, int k, int T, int H, int tstride,
