@@ -953,6 +953,7 @@ int64_t read_status(bool clear) {
   if ((t = qw::tp_status(clear)) && !s) s = t;
   if ((t = qw::decode_status(clear)) && !s) s = t;
   if ((t = qw::cached_attention_status(clear)) && !s) s = t;
+  if ((t = qw::cached_attention_tc_status(clear)) && !s) s = t;
   return s;
 }
 

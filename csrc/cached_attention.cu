@@ -81,7 +81,7 @@ struct Shape {
   int units, tiles;
 };
 __device__ __forceinline__ Shape shape_of(const CachedAttn& p, int b, int rows_per_tile) {
-  const int n = p.query_start[b + 1] - p.query_start[b];
+  const int n = new_rows(p, b).n;
   const int ctx = min(p.context[b], p.max_table_tokens);
   Shape s;
   s.tiles = n > 0 ? (n * p.group + rows_per_tile - 1) / rows_per_tile : 0;
@@ -115,8 +115,7 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) cached_attn_kernel(
   constexpr int NT = D / 8;       // 8-wide output tiles
   extern __shared__ float attn_smem[];
   float* s_o = attn_smem;                     // [kWarps][R][D]
-  __shared__ float s_ml[kWarps][R][2];
-  __shared__ float s_vref[kWarps];
+  __shared__ float s_mlv[kWarps][R][3];      // maximum, sum, largest value scale
   __shared__ int s_poison[D];                 // the first key whose value is NaN in this dim, among masked steps
   __shared__ int64_t s_find[3];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -176,7 +175,8 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) cached_attn_kernel(
     const int n_units = static_cast<int>(min(static_cast<int64_t>(shape.units - u0), end - u));
     u += n_units;
     const int h = item % p.Hkv, tile = item / p.Hkv;
-    const int q0 = p.query_start[b], n = p.query_start[b + 1] - q0;
+    const NewRows fresh = new_rows(p, b);
+    const int q0 = fresh.first, n = fresh.n;
     const int ctx = min(p.context[b], p.max_table_tokens);
     const int row0 = tile * R, rows = min(R, n * p.group - row0);
     // keys that a row sees: [0, lim)
@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) cached_attn_kernel(
 
     float o[MT][NT][4];
     float m_run[MT][2], l_run[MT][2];
-    float v_ref = 0.f, v_up = 0.f;  // the largest value scale so far, and kWeightUp over it
+    float v_ref[MT][2], v_up[MT][2];  // the largest value scale that the row has seen, and kWeightUp over it
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
@@ -264,6 +264,7 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) cached_attn_kernel(
         for (int e = 0; e < 4; ++e) o[mt][i][e] = 0.f;
       m_run[mt][0] = m_run[mt][1] = -INFINITY;
       l_run[mt][0] = l_run[mt][1] = 0.f;
+      v_ref[mt][0] = v_ref[mt][1] = v_up[mt][0] = v_up[mt][1] = 0.f;
     }
 
     for (int j = step0; j < key_end; j += kUnit) {
@@ -312,8 +313,8 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) cached_attn_kernel(
               for (int mt = 0; mt < MT; ++mt) mma_f16(s[mt][x], q[mt][c * (VB / 4) + i], b0, b1);
             }
         // ---- probabilities
-        bool moved = cur.vs > v_ref;
-        float top[MT][2];
+        bool moved = false;
+        float top[MT][2], v_top[MT][2];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -330,15 +331,16 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) cached_attn_kernel(
                 mx = fmaxf(mx, y);
               }
             top[mt][half] = mx;
-            moved = moved || mx > m_run[mt][half] + kLazy || (m_run[mt][half] == -INFINITY && mx > -INFINITY);
+            v_top[mt][half] = lim > 0 ? cur.vs : 0.f;
+            moved = moved || mx > m_run[mt][half] + kLazy || v_top[mt][half] > v_ref[mt][half];
           }
         if (__any_sync(0xffffffffu, moved)) {
-          const float v_new = fmaxf(v_ref, cur.vs);
-          const float vf = v_ref > 0.f ? v_ref / v_new : 0.f;
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
+              const float v_new = fmaxf(v_ref[mt][half], v_top[mt][half]);
+              const float vf = v_ref[mt][half] > 0.f ? v_ref[mt][half] / v_new : 0.f;
               const float m_new = fmaxf(m_run[mt][half], quad_max(top[mt][half]));
               const float f = m_run[mt][half] == -INFINITY ? 0.f : exp2f_approx(m_run[mt][half] - m_new);
               m_run[mt][half] = m_new;
@@ -348,17 +350,17 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) cached_attn_kernel(
                 o[mt][i][half * 2] *= f * vf;
                 o[mt][i][half * 2 + 1] *= f * vf;
               }
+              v_ref[mt][half] = v_new;
+              v_up[mt][half] = v_new > 0.f ? kWeightUp / v_new : 0.f;
             }
-          v_ref = v_new;
-          v_up = v_ref > 0.f ? kWeightUp / v_ref : 0.f;
         }
-        const float up = v_up * cur.vs;
         uint32_t w[MT][4];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const float m = m_run[mt][half] == -INFINITY ? 0.f : m_run[mt][half];
+            const float up = v_up[mt][half] * cur.vs;
             float pr[2][2];
 #pragma unroll
             for (int x = 0; x < 2; ++x)
@@ -394,8 +396,9 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) cached_attn_kernel(
         const int row = mt * 16 + half * 8 + g;
         const float l = quad_sum(l_run[mt][half]);
         if (t == 0) {
-          s_ml[warp][row][0] = m_run[mt][half];
-          s_ml[warp][row][1] = l;
+          s_mlv[warp][row][0] = m_run[mt][half];
+          s_mlv[warp][row][1] = l;
+          s_mlv[warp][row][2] = v_ref[mt][half];
         }
         if (row < rows) {
           float* dst = s_o + (warp * R + row) * D;
@@ -406,7 +409,6 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) cached_attn_kernel(
           }
         }
       }
-    if (lane == 0) s_vref[warp] = v_ref;
     __syncthreads();
     const bool whole = n_units == shape.units;
     const int64_t slot = u0 > 0 ? 2 * static_cast<int64_t>(blockIdx.x) : 2 * static_cast<int64_t>(blockIdx.x) + 1;
@@ -414,15 +416,15 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) cached_attn_kernel(
       const int row = i / (D / 4), d = (i % (D / 4)) * 4;
       float m = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_ml[w][row][0]);
+      for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_mlv[w][row][0]);
       float l = 0.f;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float mw = s_ml[w][row][0];
+        const float mw = s_mlv[w][row][0];
         const float f = mw == -INFINITY ? 0.f : exp2f_approx(mw - m);
-        const float fv = f * s_vref[w] * (1.f / kWeightUp);
-        l += s_ml[w][row][1] * f;
+        const float fv = f * s_mlv[w][row][2] * (1.f / kWeightUp);
+        l += s_mlv[w][row][1] * f;
         const float4 x = *reinterpret_cast<const float4*>(s_o + (w * R + row) * D + d);
         acc.x += x.x * fv; acc.y += x.y * fv; acc.z += x.z * fv; acc.w += x.w * fv;
       }
@@ -471,11 +473,12 @@ __global__ void __launch_bounds__(128) cached_attn_join_kernel(CachedAttn p, int
   }
   const int b = lo;
   float l = 0.f;
-  if (p.B > 0 && tok >= p.query_start[b] && tok < p.query_start[b + 1]) {
+  const NewRows fresh = p.B > 0 ? new_rows(p, b) : NewRows{0, 0};
+  if (tok >= fresh.first && tok < fresh.first + fresh.n) {
     const int64_t total = p.prefix[p.B];
     const Shape s = shape_of(p, b, R);
     if (s.units > 0) {
-      const int row_all = (tok - p.query_start[b]) * p.group + hq % p.group;
+      const int row_all = (tok - fresh.first) * p.group + hq % p.group;
       const int h = hq / p.group, tile = row_all / R, row = row_all % R;
       const int64_t u0 = p.prefix[b] + (static_cast<int64_t>(tile) * p.Hkv + h) * s.units;
       const int workers = static_cast<int>(min(static_cast<int64_t>(workers_max), total));
@@ -503,6 +506,9 @@ __global__ void __launch_bounds__(128) cached_attn_join_kernel(CachedAttn p, int
 #pragma unroll
   for (int e = 0; e < PER; ++e) dst[e] = __float2bfloat16(acc[e] * inv);
 }
+
+// Resident blocks of threads on 148 SMs: two per SM with one row tile (the registers), one with two.
+int cached_attn_workers(int mt) { return 148 * (mt == 1 ? 2 : 1); }
 
 template <int FMT, int D, int MT>
 void launch(const CachedAttn& p, cudaStream_t stream) {
@@ -533,40 +539,47 @@ void dispatch(const CachedAttn& p, int D, int mt, cudaStream_t stream) {
   }
 }
 
-}  // namespace
-
-// Resident blocks of threads on 148 SMs: two per SM with one row tile (the registers), one with two.
-int cached_attn_workers(int mt) { return 148 * (mt == 1 ? 2 : 1); }
-
 void cached_attention_rows(const CachedAttn& p, int D, int fmt, int mt, cudaStream_t stream) {
   if (fmt == kKvFp8) dispatch<kKvFp8>(p, D, mt, stream);
   else dispatch<kKvInt8>(p, D, mt, stream);
 }
 
-namespace {
-
-int row_tiles(int Hq, int Hkv, int max_query) { return static_cast<int64_t>(max_query) * (Hq / Hkv) <= 16 ? 1 : 2; }
-
 int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 
-struct Workspace {
-  int64_t part_o, part_ml, total;  // the prefix sums are at its beginning
+// Which kernel, and how its work is split.
+struct Way {
+  bool prompt;
+  int mt;                   // few rows: 16-row tiles per block of threads
+  int tiles_max, splits;    // prompts
+  int64_t part_o, part_ml, bytes;  // of the workspace; the prefix sums are at its beginning
 };
-Workspace workspace_of(int B, int D, int mt) {
-  const int64_t slots = 2 * static_cast<int64_t>(cached_attn_workers(mt)) * 16 * mt;
-  Workspace w;
+
+Way way_of(int T, int B, int Hq, int Hkv, int D, int max_query, int max_context) {
+  Way w{};
+  const int group = Hq / Hkv;
+  const int64_t rows = static_cast<int64_t>(std::min(max_query, T)) * group;
+  w.prompt = D != 32 && rows > 32;
+  w.mt = rows <= 16 ? 1 : 2;
+  int64_t slots;
+  if (w.prompt) {
+    w.tiles_max = static_cast<int>(static_cast<int64_t>(T) * group / kPromptRows + B);
+    // too few row tiles for the SMs: split the keys, two tiles of 128 at least for each part
+    const int64_t blocks = static_cast<int64_t>(w.tiles_max) * Hkv;
+    w.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(148 / std::max<int64_t>(blocks, 1), max_context / 256)));
+    slots = w.splits > 1 ? blocks * w.splits * kPromptRows : 0;
+  } else {
+    slots = 2 * static_cast<int64_t>(cached_attn_workers(w.mt)) * 16 * w.mt;
+  }
   w.part_o = align256((static_cast<int64_t>(B) + 1) * sizeof(int64_t));
   w.part_ml = w.part_o + align256(slots * D * sizeof(float));
-  w.total = w.part_ml + align256(slots * 2 * sizeof(float));
+  w.bytes = w.part_ml + align256(slots * 2 * sizeof(float));
   return w;
 }
 
 }  // namespace
 
 int64_t cached_attention_workspace(int T, int B, int Hq, int Hkv, int D, int max_query, int max_context) {
-  (void)T;
-  (void)max_context;
-  return workspace_of(B, D, row_tiles(Hq, Hkv, max_query)).total;
+  return way_of(T, B, Hq, Hkv, D, max_query, max_context).bytes;
 }
 
 void cached_attention(const bf16* q, int64_t q_token, int64_t q_head, bf16* out, int64_t o_token, int64_t o_head,
@@ -574,9 +587,7 @@ void cached_attention(const bf16* q, int64_t q_token, int64_t q_head, bf16* out,
                       const int* query_start, int T, int B, int Hq, int Hkv, int D, int block, int blocks, int width,
                       int max_query, int max_context, float scale, int fmt, void* workspace, cudaStream_t stream) {
   if (T == 0) return;
-  (void)max_context;
-  const int mt = row_tiles(Hq, Hkv, max_query);
-  const Workspace ws = workspace_of(B, D, mt);
+  const Way w = way_of(T, B, Hq, Hkv, D, max_query, max_context);
   uint8_t* base = static_cast<uint8_t*>(workspace);
   CachedAttn p{};
   p.q = q;
@@ -600,9 +611,10 @@ void cached_attention(const bf16* q, int64_t q_token, int64_t q_head, bf16* out,
   p.max_table_tokens = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(width) * block, 0x7fffffff));
   p.scale = scale;
   p.prefix = reinterpret_cast<int64_t*>(base);
-  p.part_o = reinterpret_cast<float*>(base + ws.part_o);
-  p.part_ml = reinterpret_cast<float*>(base + ws.part_ml);
-  cached_attention_rows(p, D, fmt, mt, stream);
+  p.part_o = reinterpret_cast<float*>(base + w.part_o);
+  p.part_ml = reinterpret_cast<float*>(base + w.part_ml);
+  if (w.prompt) cached_attention_prompt(p, D, fmt, w.tiles_max, w.splits, stream);
+  else cached_attention_rows(p, D, fmt, w.mt, stream);
 }
 
 int cached_attention_status(bool clear) { return read_status_word(clear); }

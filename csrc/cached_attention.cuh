@@ -30,7 +30,17 @@ struct CachedAttn {
   int64_t* prefix;  // [B + 1]
 };
 
-int cached_attn_workers(int mt);
-void cached_attention_rows(const CachedAttn& p, int D, int fmt, int mt, cudaStream_t stream);
+// The rows of q that belong to request b; offsets outside [0, T] are cut, so that no row outside q is touched.
+struct NewRows {
+  int first, n;
+};
+__device__ __forceinline__ NewRows new_rows(const CachedAttn& p, int b) {
+  const int first = min(max(p.query_start[b], 0), p.T);
+  return {first, min(p.query_start[b + 1], p.T) - first};
+}
+
+// tcgen05 kernel for prompts (head_dim 64 and 128): 256 rows per block of threads, `splits` parts of the keys
+constexpr int kPromptRows = 256;
+void cached_attention_prompt(const CachedAttn& p, int D, int fmt, int tiles_max, int splits, cudaStream_t stream);
 
 }  // namespace qw

@@ -1,0 +1,657 @@
+// Attention over the block-wise 8-bit KV cache for prompts: tcgen05.mma with TMEM accumulators (head_dim 64 and 128).
+//
+//   S_g  = Q_g K_j^T        TMEM, 128 rows x 128 keys per group; Q and K (f16) from shared memory
+//   P_g  = exp2(S_g * scale * k_scale - m_g) * v_scale / v_ref     softmax warps, f16, TMEM
+//   O_g += P_g V_j          TMEM, 128 x D; P_g from TMEM, V_j from shared memory
+//
+// A block of threads owns 256 query rows (new tokens x the query heads of one kv head) of one request as two groups of
+// 128, so that the tensor core works on one group's tiles while the other's scores become probabilities, and walks the
+// request's cache in tiles of 128 keys. No TMA: the operands are not in memory as the tensor core wants them. Four warps
+// fetch the codes of each tile by the block table, widen them to f16 (every code is one) and store them in the
+// 128-byte-swizzled layout; the scales of the tile's 16-key groups go beside it and are applied in 32 bits, as in the
+// kernel for few rows (cached_attention.cu), whose rules for masks, row factors and value scales hold here too. The
+// widening is shared by 256 rows: about 2 instructions per code against 256 x 4 flops.
+//
+// Probabilities come from 32-bit exponentials: f16x2 ones would halve the special-function work, but the rounding of
+// their argument costs 2^-8 relative at arguments of 8.
+//
+// TMEM (512 columns): S_0, S_1 at 0 and 128, O_0, O_1 at 256 (D columns each). head_dim 64 has room for P_0, P_1 at 384 and
+// 448; head_dim 128 has none, so P_g takes the first 64 columns of S_g, and the next S_g is issued only once P_g V has
+// completed. A softmax thread reads its row twice (maximum, then exponentials, 32 columns at a time), so that it needs no
+// 128 registers for it: 13 warps with 152 registers each fit the SM.
+//
+// Warps: 0-3 widen, 4-7 softmax of group 0, 8-11 of group 1, 12 issues the MMAs. Every wait is bounded (common.cuh); on a
+// timeout all roles stop, MMAs in flight are waited for, TMEM is freed and the status word records the cause.
+#include <algorithm>
+
+#include "cached_attention.cuh"
+#include "common.cuh"
+#include "kv_format.cuh"
+#include "launch.cuh"
+#include "launchers.h"
+
+namespace qw {
+namespace {
+
+constexpr int KT = 128;        // keys of a tile
+constexpr int kGroupRows = 128;
+constexpr int kRows = kPromptRows;  // rows of a block of threads
+constexpr int kThreads = 13 * 32;
+constexpr int kTmemCols = 512;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLazy = 6.f;
+constexpr float kWeightUp = 256.f;
+
+template <int D>
+struct Layout {
+  static constexpr bool kAlias = D == 128;                  // P_g in S_g's columns
+  static constexpr int kStages = D == 64 ? 4 : 2;
+  static constexpr int kBoxes = D / 64;                      // 64-wide (128-byte) column boxes
+  static constexpr int kQBytes = kBoxes * kGroupRows * 128;  // one group's rows
+  static constexpr int kTileBytes = kBoxes * KT * 128;       // one K or V tile
+  static constexpr int kKV = 2 * kQBytes;                    // stages of [K | V]
+  static constexpr int kScale = kKV + kStages * 2 * kTileBytes;  // stages of k_scale[8], v_scale[8]
+  static constexpr int kPoison = kScale + kStages * 64;
+  static constexpr int kBar = kPoison + D * 4;
+  static constexpr int kTotal = kBar + 512 + 1024;           // barriers, and slack to align the base to 1 KB
+  static constexpr int kTmemO = 256;
+  static constexpr int tmem_p(int g) { return kAlias ? g * 128 : 384 + g * 64; }
+  static_assert(kTotal <= 227 * 1024, "shared memory per block");
+};
+
+// Instruction descriptor, kind::f16 with f16 operands and fp32 accumulators.
+constexpr uint32_t idesc_f16(int n, bool b_mn_major) {
+  return (1u << 4) | (static_cast<uint32_t>(b_mn_major) << 16) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// 32 lanes x 32 bit, 16 consecutive columns per thread, raw words.
+__device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+
+struct TcArgs {
+  CachedAttn p;
+  int splits;
+};
+
+template <int FMT, int D>
+__global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __grid_constant__ TcArgs args) {
+  using L = Layout<D>;
+  constexpr int kStages = L::kStages;
+  const CachedAttn& p = args.p;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* s_scale = reinterpret_cast<float*>(smem + L::kScale);  // [stage][2][8]
+  int* s_poison = reinterpret_cast<int*>(smem + L::kPoison);
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + L::kBar);
+  uint64_t* k_full = q_full + 1;
+  uint64_t* v_full = k_full + kStages;
+  uint64_t* kv_empty = v_full + kStages;
+  uint64_t* s_full = kv_empty + kStages;  // [2] S_g of the next tile is in TMEM
+  uint64_t* s_free = s_full + 2;          // [2] S_g has been read (head_dim 64)
+  uint64_t* p_full = s_free + 2;          // [2] P_g is written, O_g rescaled if it had to be
+  uint64_t* o_full = p_full + 2;          // [2] O_g += P_g V has completed
+  uint64_t* teardown = o_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(teardown + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* s_item = reinterpret_cast<int*>(tmem_slot + 2);  // request, row tile, number of tiles
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  griddep_wait();
+
+  // ---- which request and row tile: the last tiles, which see the most keys, come first
+  if (warp == 0) {
+    int total = 0;
+    auto tiles_of = [&](int b) {
+      const int n = new_rows(p, b).n;
+      return n > 0 ? static_cast<int>((static_cast<int64_t>(n) * p.group + kRows - 1) / kRows) : 0;
+    };
+    for (int b = lane; b < p.B; b += 32) total += tiles_of(b);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const int want = total - 1 - static_cast<int>(blockIdx.x) / p.Hkv;
+    const bool publish = args.splits > 1 && blockIdx.x == 0 && blockIdx.y == 0;  // for the join kernel
+    if (lane == 0) {
+      s_item[0] = -1;
+      s_item[2] = total;
+    }
+    __syncwarp();
+    int before = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+      const int b = b0 + lane;
+      const int w = b < p.B ? tiles_of(b) : 0;
+      int x = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      const int at = before + x - w;
+      if (want >= at && want < at + w) {
+        s_item[0] = b;
+        s_item[1] = want - at;
+      }
+      if (publish && b < p.B) p.prefix[b] = at;
+      before += __shfl_sync(0xffffffffu, x, 31);
+    }
+  }
+  for (int i = threadIdx.x; i < D; i += kThreads) s_poison[i] = 0x7fffffff;
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 8);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&k_full[s], 4);
+      mbar_init(&v_full[s], 4);
+      mbar_init(&kv_empty[s], 1);
+    }
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(&s_full[g], 1);
+      mbar_init(&s_free[g], 4);
+      mbar_init(&p_full[g], 4);
+      mbar_init(&o_full[g], 1);
+    }
+    mbar_init(teardown, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+  const int b = s_item[0], row_tile = s_item[1];
+  const int h = static_cast<int>(blockIdx.x) % p.Hkv;
+
+  // rows that belong to no request are zero
+  if (blockIdx.x < static_cast<unsigned>(p.Hkv) && blockIdx.y == 0) {
+    const int first = p.B > 0 ? min(max(p.query_start[0], 0), p.T) : p.T, last = p.B > 0 ? min(p.query_start[p.B], p.T) : p.T;
+    const int rows = first + max(p.T - max(last, first), 0);
+    for (int64_t i = threadIdx.x; i < static_cast<int64_t>(rows) * p.group * (D / 8); i += kThreads) {
+      const int r = static_cast<int>(i / (p.group * (D / 8))), c = static_cast<int>(i % (p.group * (D / 8)));
+      const int64_t tok = r < first ? r : last + (r - first);
+      *reinterpret_cast<uint4*>(p.out + tok * p.o_token + (h * p.group + c / (D / 8)) * p.o_head + (c % (D / 8)) * 8) =
+          make_uint4(0, 0, 0, 0);
+    }
+  }
+  if (b < 0) {  // the grid is an upper bound
+    griddep_launch();
+    return;
+  }
+
+  const NewRows fresh = new_rows(p, b);
+  const int q0 = fresh.first, n = fresh.n;
+  const int ctx = min(p.context[b], p.max_table_tokens);
+  const int row0 = row_tile * kRows;
+  const int rows = static_cast<int>(min(static_cast<int64_t>(kRows), static_cast<int64_t>(n) * p.group - row0));
+  // keys that a row of the tile sees: [0, lim)
+  auto lim_of = [&](int row) { return min(ctx, p.context[b] - n + (row0 + min(row, rows - 1)) / p.group + 1); };
+  const int lim_all = lim_of(0), lim_any = lim_of(rows - 1);
+  const int tiles = lim_any > 0 ? (lim_any + KT - 1) / KT : 0;
+  const int per = (tiles + args.splits - 1) / args.splits;
+  const int t0 = min(tiles, static_cast<int>(blockIdx.y) * per), t1 = min(tiles, t0 + per);
+  auto tiles_of_group = [&](int g) {
+    if (rows <= g * kGroupRows) return 0;
+    const int lim = lim_of(min(rows, (g + 1) * kGroupRows) - 1);
+    return max(0, min(t1, lim > 0 ? (lim + KT - 1) / KT : 0) - t0);
+  };
+  const int n0 = tiles_of_group(0), n1 = tiles_of_group(1);
+  const int nk = max(n0, n1);
+
+  if (warp == 12) tmem_alloc(tmem_slot, kTmemCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp < 4) {
+    // ------------------------------------------------------------------ codes -> f16 tiles in shared memory
+    constexpr int CPK = D / 16;          // 16-byte pieces of a key
+    constexpr int KPP = 128 / CPK;       // keys that the 128 threads cover at a time
+    constexpr int NP = 64 / KPP;         // pieces per thread of a half tile (64 keys)
+    const int piece = threadIdx.x % CPK, key_in = threadIdx.x / CPK;
+    const int* table = p.table + static_cast<int64_t>(b) * p.table_stride;
+    const uint8_t* base[2] = {p.k.codes + h * p.k.head_stride + piece * 16, p.v.codes + h * p.v.head_stride + piece * 16};
+    const int64_t block_stride[2] = {p.k.block_stride, p.v.block_stride};
+    const int64_t token_stride[2] = {p.k.token_stride, p.v.token_stride};
+    // half tiles in the order K lower, K upper, V lower, V upper of each tile; two in flight
+    uint4 raw[2][NP];
+    float scale[2];
+    auto fetch = [&](auto which, int slot, int j, int half) {
+      constexpr int kv = decltype(which)::value;
+      const int k0 = (t0 + j) * KT + half * 64;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int key = k0 + key_in + i * KPP;
+        raw[slot][i] = make_uint4(0, 0, 0, 0);
+        if (key < lim_any) {
+          const int id = __ldg(table + key / p.block);
+          if (static_cast<unsigned>(id) < static_cast<unsigned>(p.blocks))
+            raw[slot][i] = __ldg(reinterpret_cast<const uint4*>(base[kv] + static_cast<int64_t>(id) * block_stride[kv] +
+                                                                static_cast<int64_t>(key % p.block) * token_stride[kv]));
+        }
+      }
+      // scales of the four 16-key groups; a group without a block counts as masked
+      scale[slot] = -1.f;
+      if (threadIdx.x < 4) {
+        const int key = k0 + threadIdx.x * 16;
+        const int id = key < lim_any ? __ldg(table + key / p.block) : -1;
+        if (static_cast<unsigned>(id) < static_cast<unsigned>(p.blocks))
+          scale[slot] = kv == 0 ? __ldg(p.k.scale + static_cast<int64_t>(id) * p.k.scale_stride + h)
+                                : __ldg(p.v.scale + static_cast<int64_t>(id) * p.v.scale_stride + h);
+      }
+    };
+    auto store = [&](auto which, int slot, int j, int half) {
+      constexpr int kv = decltype(which)::value;
+      const int st = j % kStages;
+      uint8_t* dst = smem + L::kKV + st * 2 * L::kTileBytes + kv * L::kTileBytes + (piece / 4) * (KT * 128);
+      const bool edge = kv == 1 && (t0 + j + 1) * KT > lim_all;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int in = half * 64 + key_in + i * KPP;  // key in the tile
+        uint32_t w[4] = {raw[slot][i].x, raw[slot][i].y, raw[slot][i].z, raw[slot][i].w};
+        if (edge && (t0 + j) * KT + in >= lim_all) {  // seen by some rows only: a NaN must not reach the others
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t bad = Kv<FMT>::nan_bytes(w[c]);
+            if (bad)
+              for (int e = 0; e < 4; ++e)
+                if ((bad >> (8 * e + 7)) & 1) {
+                  atomicMin(&s_poison[piece * 16 + c * 4 + e], (t0 + j) * KT + in);
+                  w[c] &= ~(0xffu << (8 * e));
+                }
+          }
+        }
+        uint4 lo, hi;
+        Kv<FMT>::decode4(w[0], lo.x, lo.y);
+        Kv<FMT>::decode4(w[1], lo.z, lo.w);
+        Kv<FMT>::decode4(w[2], hi.x, hi.y);
+        Kv<FMT>::decode4(w[3], hi.z, hi.w);
+        uint8_t* row = dst + in * 128;
+        const int c = (piece % 4) * 2, sw = in & 7;
+        // the pieces of the second column box store their halves in the other order: no bank is hit twice
+        const bool swap = piece >= 4;
+        *reinterpret_cast<uint4*>(row + ((c + (swap ? 1 : 0)) ^ sw) * 16) = swap ? hi : lo;
+        *reinterpret_cast<uint4*>(row + ((c + (swap ? 0 : 1)) ^ sw) * 16) = swap ? lo : hi;
+      }
+      if (threadIdx.x < 4) s_scale[st * 16 + kv * 8 + half * 4 + threadIdx.x] = scale[slot];
+    };
+    auto arrive = [&](uint64_t* bar) {
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    using K_ = std::integral_constant<int, 0>;
+    using V_ = std::integral_constant<int, 1>;
+    if (nk > 0) {
+      fetch(K_{}, 0, 0, 0);
+      fetch(K_{}, 1, 0, 1);
+    }
+    for (int j = 0; j < nk; ++j) {
+      const int st = j % kStages;
+      const bool ok = mbar_sleep_wait(&kv_empty[st], ((j / kStages) & 1) ^ 1, kTimeoutEmpty);
+      if (!__all_sync(0xffffffffu, ok && *abort_flag == 0)) {
+        *abort_flag = 1;
+        break;
+      }
+      store(K_{}, 0, j, 0);
+      fetch(V_{}, 0, j, 0);
+      store(K_{}, 1, j, 1);
+      arrive(&k_full[st]);
+      fetch(V_{}, 1, j, 1);
+      store(V_{}, 0, j, 0);
+      if (j + 1 < nk) fetch(K_{}, 0, j + 1, 0);
+      store(V_{}, 1, j, 1);
+      arrive(&v_full[st]);
+      if (j + 1 < nk) fetch(K_{}, 1, j + 1, 1);
+    }
+  } else if (warp == 12) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t id_s = idesc_f16(KT, false);
+      constexpr uint32_t id_o = idesc_f16(D, true);
+      int ns[2] = {0, 0};  // next S to issue, per group
+      int no[2] = {0, 0};  // next P V to issue
+      int released = 0;
+      const uint64_t dq0 = smem_desc_sw128(smem_u32(smem), 16, 1024);
+      const uint64_t dk0 = smem_desc_sw128(smem_u32(smem + L::kKV), 16, 1024);
+      const uint64_t dv0 = smem_desc_sw128(smem_u32(smem + L::kKV + L::kTileBytes), KT * 128, 1024);
+      auto issue_s = [&](int g, int j) {
+        const uint64_t dq = dq0 + static_cast<uint32_t>(g * (L::kQBytes >> 4));
+        const uint64_t dk = dk0 + static_cast<uint32_t>((j % kStages) * ((2 * L::kTileBytes) >> 4));
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          umma_bf16(tmem + g * KT, dq + (((k / 4) * (kGroupRows * 128) + (k % 4) * 32) >> 4),
+                    dk + (((k / 4) * (KT * 128) + (k % 4) * 32) >> 4), id_s, k > 0 ? 1u : 0u);
+        umma_commit(&s_full[g]);
+      };
+      auto issue_o = [&](int g, int j) {
+        const uint64_t dv = dv0 + static_cast<uint32_t>((j % kStages) * ((2 * L::kTileBytes) >> 4));
+        const uint32_t a0 = tmem + L::tmem_p(g);
+        const uint32_t d = tmem + L::kTmemO + g * D;
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < KT / 16; ++k)
+          umma_bf16_ts(d, a0 + k * 8, dv + ((k * 2048) >> 4), id_o, k > 0 || j > 0 ? 1u : 0u);
+        umma_commit(&o_full[g]);
+      };
+      bool ok = mbar_sleep_wait(q_full, 0, kTimeoutFull);
+      int idle = 0;
+      uint64_t idle_start = 0;
+      auto step = [&](int g, int n_g) -> bool {
+        bool moved = false;
+        if (no[g] < ns[g] && mbar_test(&p_full[g], no[g] & 1) && mbar_test(&v_full[no[g] % kStages], (no[g] / kStages) & 1)) {
+          issue_o(g, no[g]++);
+          moved = true;
+        }
+        if (ns[g] < n_g && mbar_test(&k_full[ns[g] % kStages], (ns[g] / kStages) & 1)) {
+          bool free = ns[g] == 0;
+          if (!free) free = L::kAlias ? no[g] == ns[g] && mbar_test(&o_full[g], (ns[g] - 1) & 1)
+                                      : mbar_test(&s_free[g], (ns[g] - 1) & 1);
+          if (free) {
+            issue_s(g, ns[g]++);
+            moved = true;
+          }
+        }
+        return moved;
+      };
+      while (ok && (no[0] < n0 || no[1] < n1)) {
+        bool progress = step(0, n0);
+        progress = step(1, n1) || progress;
+        while (released < nk && (released >= n0 || no[0] > released) && (released >= n1 || no[1] > released)) {
+          umma_commit(&kv_empty[released % kStages]);
+          ++released;
+          progress = true;
+        }
+        if (progress) {
+          idle = 0;
+          continue;
+        }
+        if ((++idle & 1023) == 0) {
+          if (*abort_flag) { ok = false; break; }
+          const uint64_t now = globaltimer();
+          if (idle == 1024) idle_start = now;
+          else if (now - idle_start > QW_WAIT_TIMEOUT_NS) { set_status(kTimeoutAccum); ok = false; break; }
+        }
+      }
+      if (!ok) *abort_flag = 1;
+      umma_commit(teardown);  // fires once every MMA issued above has completed
+      mbar_sleep_wait(teardown, 0, kTimeoutAccum);
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax
+    const int g = (warp - 4) / 4;
+    const int row = (warp % 4) * 32 + lane;     // of the group = TMEM lane
+    const int r = g * kGroupRows + row;         // of the tile
+    const int n_g = g == 0 ? n0 : n1;
+    const bool real = r < rows;
+    const int tok = q0 + (row0 + r) / p.group, head = h * p.group + (row0 + r) % p.group;
+    const uint32_t lane_off = static_cast<uint32_t>((warp % 4) * 32) << 16;
+    const uint32_t ts = tmem + lane_off + g * KT;
+    const uint32_t to = tmem + lane_off + L::kTmemO + g * D;
+    const uint32_t tp = tmem + lane_off + L::tmem_p(g);
+    float unit = 0.f;
+    {
+      // the query row in f16, divided by a power of two that brings its largest number to [1, 2)
+      const uint4* src = reinterpret_cast<const uint4*>(p.q + static_cast<int64_t>(tok) * p.q_token + head * p.q_head);
+      uint8_t* dst = smem + g * L::kQBytes + row * 128;
+      float m = 0.f;
+      if (real) {
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          const uint4 w = __ldg(src + c);
+          const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&w);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = __bfloat1622float2(x[i]);
+            m = fmaxf(m, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+        }
+      }
+      const int e = min(max(static_cast<int>(__float_as_uint(m) >> 23) - 127, -100), 126);
+      const bool fine = m > 0.f && m <= 3.4028234e38f;  // zero or infinite rows as they are
+      const float inv = fine ? exp2i(-e) : 1.f;
+      unit = (fine ? exp2i(e) : 1.f) * p.scale * kLog2e;
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        uint4 out = make_uint4(0, 0, 0, 0);
+        if (real) {
+          const uint4 w = __ldg(src + c);
+          const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&w);
+          const float2 f0 = __bfloat1622float2(x[0]), f1 = __bfloat1622float2(x[1]), f2 = __bfloat1622float2(x[2]),
+                       f3 = __bfloat1622float2(x[3]);
+          out = make_uint4(pack_f16(f0.x * inv, f0.y * inv), pack_f16(f1.x * inv, f1.y * inv),
+                           pack_f16(f2.x * inv, f2.y * inv), pack_f16(f3.x * inv, f3.y * inv));
+        }
+        *reinterpret_cast<uint4*>(dst + (c / 8) * (kGroupRows * 128) + ((c % 8) ^ (row & 7)) * 16) = out;
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    }
+    const int lim = lim_of(r);
+    const int lim_group = lim_of(g * kGroupRows);  // the group's first row sees the fewest keys
+    float m_run = -INFINITY, l_run = 0.f, v_ref = 0.f, v_up = 0.f;
+    bool ok = true;
+    for (int j = 0; j < n_g; ++j) {
+      const int st = j % kStages;
+      if (__any_sync(0xffffffffu, *abort_flag != 0)) { ok = false; break; }
+      if (!__all_sync(0xffffffffu, mbar_sleep_wait(&s_full[g], j & 1, kTimeoutAccum))) { ok = false; break; }
+      // the tile's scales: written before k_full and v_full completed
+      if (!__all_sync(0xffffffffu, mbar_sleep_wait(&k_full[st], (j / kStages) & 1, kTimeoutFull) &&
+                                       mbar_sleep_wait(&v_full[st], (j / kStages) & 1, kTimeoutFull))) { ok = false; break; }
+      tc_fence_after();
+      const int k0 = (t0 + j) * KT;
+      const float* sc = s_scale + st * 16;
+      float ks[8], vs[8];
+#pragma unroll
+      for (int i = 0; i < 8; i += 4) {
+        const float4 a = *reinterpret_cast<const float4*>(sc + i), c = *reinterpret_cast<const float4*>(sc + 8 + i);
+        ks[i] = a.x; ks[i + 1] = a.y; ks[i + 2] = a.z; ks[i + 3] = a.w;
+        vs[i] = c.x; vs[i + 1] = c.y; vs[i + 2] = c.z; vs[i + 3] = c.w;
+      }
+      const int lim_tile = lim - k0;
+      bool plain = k0 + KT <= lim_group;  // uniform over the warp: all 128 keys are seen by all rows
+#pragma unroll
+      for (int i = 0; i < 8; ++i) plain = plain && ks[i] >= 0.f;
+      float v_top = 0.f;  // the largest value scale that this row sees
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v_top = fmaxf(v_top, plain || i * 16 < lim_tile ? vs[i] : 0.f);
+      // scores of 32 columns, scaled, masked ones at -inf
+      auto scores = [&](int c, float* v) {
+        tmem_ld32(ts + c, v);
+        const float f0 = unit * ks[c / 16], f1 = unit * ks[c / 16 + 1];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] *= i < 16 ? f0 : f1;
+        if (!plain) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (c + i >= lim_tile || ks[c / 16 + i / 16] < 0.f) v[i] = -INFINITY;
+        }
+      };
+      float mx = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < KT; c += 32) {
+        float v[32];
+        scores(c, v);
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) mx = fmax3(mx, v[i], v[i + 1]);
+      }
+      float factor = 1.f;
+      bool rescale = false;
+      if (__any_sync(0xffffffffu, mx > m_run + kLazy || v_top > v_ref)) {
+        const float m_new = fmaxf(m_run, mx), v_new = fmaxf(v_ref, v_top);
+        const float f = m_run == -INFINITY ? 0.f : exp2f_approx(m_run - m_new);
+        factor = f * (v_ref > 0.f ? v_ref / v_new : 0.f);
+        l_run *= f;
+        m_run = m_new;
+        v_ref = v_new;
+        v_up = v_new > 0.f ? kWeightUp / v_new : 0.f;
+        rescale = j > 0;
+      }
+      // O_g += P_g V of the tile before has to be complete before P_g (head_dim 64) or O_g is written
+      if (j > 0 && !__all_sync(0xffffffffu, mbar_sleep_wait(&o_full[g], (j - 1) & 1, kTimeoutAccum))) { ok = false; break; }
+      tc_fence_after();
+      if (rescale) {
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          float o[32];
+          tmem_ld32(to + c, o);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] *= factor;
+          tmem_st32(to + c, o);
+        }
+      }
+      const float m = m_run == -INFINITY ? 0.f : m_run;
+      float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < KT; c += 32) {
+        float v[32];
+        scores(c, v);
+        uint32_t w[16];
+        const float u0 = v_up * vs[c / 16], u1 = v_up * vs[c / 16 + 1];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float2 e = make_float2(exp2f_approx(v[2 * i] - m), exp2f_approx(v[2 * i + 1] - m));
+          sum = add_f32x2(sum, e);
+          const float u = i < 8 ? u0 : u1;
+          w[i] = pack_f16(e.x * u, e.y * u);
+        }
+        tmem_st16u(tp + c / 2, w);
+      }
+      l_run += sum.x + sum.y;
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (!L::kAlias) mbar_arrive(&s_free[g]);
+        mbar_arrive(&p_full[g]);
+      }
+    }
+    if (ok && n_g > 0 && !__all_sync(0xffffffffu, mbar_sleep_wait(&o_full[g], (n_g - 1) & 1, kTimeoutAccum))) ok = false;
+    if (!ok) {
+      *abort_flag = 1;
+    } else {
+      tc_fence_after();
+      const bool part = args.splits > 1;
+      const float up = v_ref * (1.f / kWeightUp);
+      const float inv = part ? up : (m_run == -INFINITY ? 0.f : up / l_run);  // a row that sees no key is zero
+      const int64_t slot = ((static_cast<int64_t>(s_item[2]) - 1 - blockIdx.x / p.Hkv) * p.Hkv + h) * args.splits + blockIdx.y;
+      bf16* out = p.out + static_cast<int64_t>(tok) * p.o_token + head * p.o_head;
+      float* part_o = p.part_o + (slot * kRows + r) * D;
+#pragma unroll
+      for (int c = 0; c < D; c += 32) {
+        float o[32];
+        if (n_g > 0) {
+          tmem_ld32(to + c, o);  // by whole warps
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0.f;
+        }
+        if (real) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            o[i] *= inv;
+            if (s_poison[c + i] < lim) o[i] = __int_as_float(0x7fffffff);
+          }
+          if (part) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<float4*>(part_o + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8)
+              *reinterpret_cast<uint4*>(out + c + i) = make_uint4(pack_bf16(o[i], o[i + 1]), pack_bf16(o[i + 2], o[i + 3]),
+                                                                  pack_bf16(o[i + 4], o[i + 5]), pack_bf16(o[i + 6], o[i + 7]));
+          }
+        }
+      }
+      if (part && real) *reinterpret_cast<float2*>(p.part_ml + (slot * kRows + r) * 2) = make_float2(m_run, l_run);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 12) tmem_dealloc(tmem, kTmemCols);
+  griddep_launch();
+}
+
+// One warp per (token, query head): adds the splits' results in their order.
+template <int D>
+__global__ void __launch_bounds__(128) cached_attn_tc_join_kernel(CachedAttn p, int splits) {
+  const int lane = threadIdx.x % 32;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 32;
+  griddep_wait();
+  griddep_launch();
+  if (i >= static_cast<int64_t>(p.T) * p.Hkv * p.group) return;
+  const int tok = static_cast<int>(i / (p.Hkv * p.group)), hq = static_cast<int>(i % (p.Hkv * p.group));
+  int lo = 0, hi = p.B;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (p.query_start[mid] <= tok) lo = mid;
+    else hi = mid;
+  }
+  const NewRows fresh = p.B > 0 ? new_rows(p, lo) : NewRows{0, 0};
+  if (tok < fresh.first || tok >= fresh.first + fresh.n) return;  // zeroed by the attention kernel
+  const int r = (tok - fresh.first) * p.group + hq % p.group;
+  const int64_t slot0 = ((p.prefix[lo] + r / kRows) * p.Hkv + hq / p.group) * splits;
+  float m = -INFINITY;
+  for (int s = lane; s < splits; s += 32) m = fmaxf(m, p.part_ml[((slot0 + s) * kRows + r % kRows) * 2]);
+  m = warp_max(m);
+  constexpr int PER = D / 32;
+  float acc[PER], l = 0.f;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const int64_t at = (slot0 + s) * kRows + r % kRows;
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
+    const float f = ml.x == -INFINITY ? 0.f : exp2f_approx(ml.x - m);
+    l += ml.y * f;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) acc[e] += p.part_o[at * D + lane * PER + e] * f;
+  }
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  bf16* dst = p.out + static_cast<int64_t>(tok) * p.o_token + hq * p.o_head + lane * PER;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) dst[e] = __float2bfloat16(acc[e] * inv);
+}
+
+template <int FMT, int D>
+void launch(const CachedAttn& p, int tiles_max, int splits, cudaStream_t stream) {
+  auto kernel = cached_attn_tc_kernel<FMT, D>;
+  static const bool configured = [&] {
+    check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kTotal),
+               "cached_attention tc smem");
+    return true;
+  }();
+  (void)configured;
+  launch_pdl(kernel, dim3(static_cast<unsigned>(tiles_max) * p.Hkv, splits), dim3(kThreads), Layout<D>::kTotal, stream,
+             "cached_attention tc", TcArgs{p, splits});
+  if (splits > 1) {
+    const int64_t rows = static_cast<int64_t>(p.T) * p.Hkv * p.group;
+    launch_pdl(cached_attn_tc_join_kernel<D>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), 0, stream,
+               "cached_attention tc join", p, splits);
+  }
+}
+
+}  // namespace
+
+void cached_attention_prompt(const CachedAttn& p, int D, int fmt, int tiles_max, int splits, cudaStream_t stream) {
+  if (fmt == kKvFp8) {
+    if (D == 64) launch<kKvFp8, 64>(p, tiles_max, splits, stream);
+    else launch<kKvFp8, 128>(p, tiles_max, splits, stream);
+  } else {
+    if (D == 64) launch<kKvInt8, 64>(p, tiles_max, splits, stream);
+    else launch<kKvInt8, 128>(p, tiles_max, splits, stream);
+  }
+}
+
+int cached_attention_tc_status(bool clear) { return read_status_word(clear); }
+
+}  // namespace qw

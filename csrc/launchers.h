@@ -247,6 +247,7 @@ void cached_attention(const bf16* q, int64_t q_token, int64_t q_head, bf16* out,
 // bytes of the workspace for these sizes
 int64_t cached_attention_workspace(int T, int B, int Hq, int Hkv, int D, int max_query, int max_context);
 int cached_attention_status(bool clear);
+int cached_attention_tc_status(bool clear);
 // ---- logits.cu ----
 struct LogitsArgs {
   const void* logits;
