@@ -743,6 +743,10 @@ qw::KvPages kv_pages(const Tensor& cache, const Tensor& scale, const char* what)
   bool ok = reinterpret_cast<uintptr_t>(cache.data_ptr()) % 16 == 0;
   for (int i = 0; i < 3; ++i) ok = ok && (cache.size(i) <= 1 || cache.stride(i) % 16 == 0);
   TORCH_CHECK(ok, what, ": storage and strides must be multiples of 16 bytes");
+  const int64_t far = int64_t{1} << 32;
+  for (int i = 0; i < 3; ++i) ok = ok && (cache.size(i) <= 1 || (cache.stride(i) >= 0 && cache.stride(i) < far));
+  ok = ok && (scale.dim() != 2 || (scale.stride(0) >= 0 && scale.stride(0) < far));
+  TORCH_CHECK(ok && cache.size(2) * cache.stride(2) < far, what, ": strides must be below 4 GB");
   TORCH_CHECK(scale.is_cuda() && scale.scalar_type() == torch::kFloat32 && scale.dim() == 2 && scale.size(0) == cache.size(0) &&
                   scale.size(1) == cache.size(1) && (scale.size(1) <= 1 || scale.stride(1) == 1),
               what, ": scales must be float32 [blocks, kv_heads] with unit inner stride");

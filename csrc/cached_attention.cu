@@ -4,7 +4,7 @@
 //   o_i = sum_j p_ij v_j / sum_j p_ij,   p_ij = exp2(s_ij - m_i),   s_ij = (q_i . k_j) * scale * log2(e)
 //   over the keys j <= context - new + i of the request's own blocks.
 //
-// The query heads that share a kv head, and the new tokens, are rows of one tile (16 MT rows), so the cache is read once
+// The query heads that share a kv head, and the new tokens, are rows of one tile (8 to 32 rows), so the cache is read once
 // for all of them. Bound by HBM: 2 D bytes per cached token and kv head against 4 D flops per row.
 //
 // Codes go from global memory into the registers of the tensor-core fragments: the contraction indices of an MMA may be
@@ -18,6 +18,7 @@
 // consecutive ranges, one per resident block of threads, so ragged lengths cost nothing; a range that ends inside an item
 // leaves a partial result (at most two per block), which the join kernel adds up in a fixed order.
 #include <algorithm>
+#include <type_traits>
 
 #include "cached_attention.cuh"
 #include "common.cuh"
@@ -32,13 +33,22 @@ constexpr int kUnit = 64;    // keys of a unit: 16 per warp
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNone = -3e38f;      // running maximum of a row that has seen no key
 constexpr float kLazy = 6.f;        // the running maximum moves when a row grows by more than 2^6
 constexpr float kWeightUp = 256.f;  // probabilities (<= 2^6) times value scale over the largest: at most 2^14 in f16
 
-__device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// c (16 x 8) += a (16 x 16) b (16 x 8), f16 operands
+__device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 8 x 8 transpose of 16-bit numbers, two per lane
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
@@ -46,46 +56,34 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-__device__ __forceinline__ float quad_max(float v) {
+__device__ __forceinline__ float quad_max(float v) {  // over the four lanes that hold one row of q
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
   return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
 }
-__device__ __forceinline__ float quad_sum(float v) {
-  v += __shfl_xor_sync(0xffffffffu, v, 1);
-  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+__device__ __forceinline__ float column_max(float v) {  // over the eight lanes that hold one column of an MMA tile
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+}
+__device__ __forceinline__ float column_sum(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 4);
+  v += __shfl_xor_sync(0xffffffffu, v, 8);
+  return v + __shfl_xor_sync(0xffffffffu, v, 16);
 }
 
-// N bytes per lane as 32-bit words
-template <int N>
-struct Bytes {
-  uint32_t w[N / 4];
-  __device__ __forceinline__ void load(const uint8_t* p) {
-    if constexpr (N == 16) {
-      const uint4 x = __ldg(reinterpret_cast<const uint4*>(p));
-      w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
-    } else if constexpr (N == 8) {
-      const uint2 x = __ldg(reinterpret_cast<const uint2*>(p));
-      w[0] = x.x; w[1] = x.y;
-    } else {
-      w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
-    }
-  }
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int i = 0; i < N / 4; ++i) w[i] = 0;
-  }
-};
-
-// The items of a request: row tiles x kv heads, each `units` long.
+// The items of a request: row tiles x kv heads, each `units` long. The first `kLead` units of an item stand for what a
+// piece costs apart from its keys (query rows, the sum over the warps): without them the ranges that hold many short
+// requests took 1.3 times as long as the others.
 struct Shape {
   int units, tiles;
 };
+constexpr int kLead = 3;
 __device__ __forceinline__ Shape shape_of(const CachedAttn& p, int b, int rows_per_tile) {
   const int n = new_rows(p, b).n;
   const int ctx = min(p.context[b], p.max_table_tokens);
   Shape s;
   s.tiles = n > 0 ? (n * p.group + rows_per_tile - 1) / rows_per_tile : 0;
-  s.units = ctx > 0 ? (ctx + kUnit - 1) / kUnit : 0;
+  s.units = ctx > 0 ? (ctx + kUnit - 1) / kUnit + kLead : 0;
   return s;
 }
 __device__ __forceinline__ int64_t work_of(const CachedAttn& p, int b, int rows_per_tile) {
@@ -97,25 +95,111 @@ __device__ __forceinline__ int worker_of(int64_t unit, int64_t total, int worker
   return static_cast<int>(((unit + 1) * workers - 1) / total);
 }
 
-// One 16-key step of a warp, as loaded: codes, scales, and whether the keys have a block at all.
-template <int D>
-struct Raw {
-  static constexpr int VB = D / 4 < 16 ? D / 4 : 16;  // bytes of a key that a lane loads at a time
-  static constexpr int CH = D / 4 / VB;
-  Bytes<VB> k[2][CH];    // key n of the two 8-key halves: dims c * 4 VB + t * VB ...
-  Bytes<D / 8> v[4];     // values 2t, 2t + 1, 2t + 8, 2t + 9: dims g * D / 8 ...
-  float ks, vs;
+// Bytes of shared memory.
+template <int D, int ROWS>
+struct Layout {
+  static constexpr int kStages = D == 128 ? 3 : D == 64 ? 4 : 6;
+  static constexpr int kStep = 16 * 2 * D;                       // one 16-key step: keys, then values
+  static constexpr int kJoinRows = 8;                            // rows that the warps add up at a time
+  static constexpr int kRing = kWarps * kStages * kStep;
+  static constexpr int kJoin = kWarps * kJoinRows * D * 4;
+  static constexpr int kQ = ROWS > 16 ? ROWS / 8 * (D / 16) * 32 * 8 : 0;  // query fragments (fewer: in registers)
+  static constexpr int kTotal = kRing + kJoin + kQ;
+  // blocks of threads per SM: registers and shared memory allow no more
+  static constexpr int kPerSm = D == 128 ? (ROWS > 16 ? 2 : 3) : ROWS > 16 ? 3 : ROWS > 8 ? 4 : 5;
 };
 
-template <int FMT, int D, int MT>
-__global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) cached_attn_kernel(CachedAttn p) {
-  constexpr int R = 16 * MT;      // rows of a tile
-  constexpr int VB = Raw<D>::VB;
-  constexpr int CH = Raw<D>::CH;
-  constexpr int NT = D / 8;       // 8-wide output tiles
-  extern __shared__ float attn_smem[];
-  float* s_o = attn_smem;                     // [kWarps][R][D]
-  __shared__ float s_mlv[kWarps][R][3];      // maximum, sum, largest value scale
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Where the 16-byte piece c of row r (of 16) of a step lies. The lanes that read shared memory together hold the rows
+// g, g + 1 (keys) or the rows 0, 2, 4, 6 (values); the order of the pieces keeps them on different banks. Row r + 8 lies
+// 8 D bytes after row r.
+template <int D>
+__device__ __forceinline__ int piece_at(int r, int c) {
+  if constexpr (D == 128) return r * 128 + ((c ^ ((((r >> 1) & 3) << 1) ^ ((r & 1) << 2))) * 16);
+  else if constexpr (D == 64) return (r >> 1) * 128 + ((r ^ (r >> 1)) & 1) * 64 + ((c ^ (((r >> 2) & 1) << 1)) * 16);
+  else return r * 32 + c * 16;
+}
+
+// N bytes of shared memory as 32-bit words
+template <int N>
+__device__ __forceinline__ void lds(uint32_t* w, const uint8_t* p) {
+  if constexpr (N == 16) {
+    const uint4 x = *reinterpret_cast<const uint4*>(p);
+    w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+  } else if constexpr (N == 8) {
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
+    w[0] = x.x; w[1] = x.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+}
+
+// Walks the pieces (one item's consecutive units) of a range.
+struct Walk {
+  int64_t u, at;  // next unit; first unit of request b
+  int b;
+  Shape shape;
+  // the piece
+  int h, tile, u0, units, first_key, q0, n, ctx, row0, rows;
+
+  template <int R>
+  __device__ __forceinline__ void next(const CachedAttn& p, int64_t end) {
+    int64_t size = static_cast<int64_t>(shape.units) * shape.tiles * p.Hkv;
+    while (u >= at + size) {  // ends: u < end <= the sum of all requests' units
+      at += size;
+      shape = shape_of(p, ++b, R);
+      size = static_cast<int64_t>(shape.units) * shape.tiles * p.Hkv;
+    }
+    const int64_t local = u - at;
+    const int item = (local >> 32) == 0 ? static_cast<int>(static_cast<uint32_t>(local) / static_cast<uint32_t>(shape.units))
+                                        : static_cast<int>(local / shape.units);
+    u0 = static_cast<int>(local - static_cast<int64_t>(item) * shape.units);
+    units = static_cast<int>(min(static_cast<int64_t>(shape.units - u0), end - u));
+    u += units;
+    first_key = max(u0 - kLead, 0) * kUnit;
+    tile = item / p.Hkv;
+    h = item - tile * p.Hkv;
+    const NewRows fresh = new_rows(p, b);
+    q0 = fresh.first;
+    n = fresh.n;
+    ctx = min(p.context[b], p.max_table_tokens);
+    row0 = tile * R;
+    rows = min(R, n * p.group - row0);
+  }
+  // keys that a row of the piece's tile sees: [0, lim)
+  __device__ __forceinline__ int lim_of(const CachedAttn& p, int row) const {
+    return min(ctx, p.context[b] - n + (row0 + min(row, rows - 1)) / p.group + 1);
+  }
+  __device__ __forceinline__ int key_end(const CachedAttn& p) const { return min(lim_of(p, rows - 1), (u0 + units - kLead) * kUnit); }
+};
+
+template <int FMT, int D, int ROWS>
+__global__ void __launch_bounds__(kThreads, Layout<D, ROWS>::kPerSm) cached_attn_kernel(CachedAttn p) {
+  using L = Layout<D, ROWS>;
+  constexpr int R = ROWS;                         // rows of a tile
+  constexpr int N = ROWS / 8;                     // 8-row tiles of queries
+  constexpr int VB = D / 4 < 16 ? D / 4 : 16;     // bytes of a key that a lane reads at a time
+  constexpr int CH = D / 4 / VB;
+  constexpr int NT = D / 16;                      // 16-wide output tiles
+  constexpr bool kQInSmem = L::kQ > 0;
+  constexpr int S = L::kStages;
+  extern __shared__ __align__(16) uint8_t smem[];
+  float* s_o = reinterpret_cast<float*>(smem + L::kRing);  // [kWarps][kJoinRows][D]
+  uint2* s_q = reinterpret_cast<uint2*>(smem + L::kRing + L::kJoin);  // [N][D / 16][32]
+  __shared__ __align__(8) float s_scale[kWarps][S][2];
+  __shared__ float s_unit[R];
+  __shared__ float s_mlv[kWarps][R][3];       // maximum, sum, largest value scale
   __shared__ int s_poison[D];                 // the first key whose value is NaN in this dim, among masked steps
   __shared__ int64_t s_find[3];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -161,292 +245,369 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) cached_attn_kernel(
     return;
   }
   const int64_t begin = blockIdx.x * total / workers, end = (blockIdx.x + 1) * total / workers;
-  int b = static_cast<int>(s_find[1]);
-  int64_t at = s_find[2];
-  Shape shape = shape_of(p, b, R);
 
-  for (int64_t u = begin; u < end;) {
-    while (u >= at + static_cast<int64_t>(shape.units) * shape.tiles * p.Hkv) {  // ends: u < end <= total
-      at += static_cast<int64_t>(shape.units) * shape.tiles * p.Hkv;
-      shape = shape_of(p, ++b, R);
+  // ---- the warp's 16-key steps, fetched S - 1 steps ahead across the pieces
+  uint8_t* ring = smem + warp * S * L::kStep;
+  const uint32_t ring_u32 = smem_u32(ring), scale_u32 = smem_u32(&s_scale[warp][0][0]);
+  Walk ahead;
+  ahead.u = begin;
+  ahead.b = static_cast<int>(s_find[1]);
+  ahead.at = s_find[2];
+  ahead.shape = shape_of(p, ahead.b, R);
+  Walk now = ahead;
+  constexpr int CPR = D / 16;                         // 16-byte pieces of a row
+  constexpr int RPI = 32 / CPR < 16 ? 32 / CPR : 16;  // rows per instruction
+  // Shared-memory offsets of a step that the lane needs; the others differ by constants (see piece_at). Kept in registers:
+  // worked out again in every step they cost as much as the arithmetic.
+  const int put[2] = {piece_at<D>(lane / CPR, lane % CPR), piece_at<D>(RPI < 16 ? RPI + lane / CPR : 0, lane % CPR)};
+  int key_at[CH], val_at[2];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) key_at[c] = piece_at<D>(g, (c * 4 * VB + t * VB) / 16) + (t * VB) % 16;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) val_at[x] = 16 * D + piece_at<D>(2 * t + x, g * (D / 8) / 16) + (g * (D / 8)) % 16;
+  // row r + 8 lies 8 rows further
+  const uint32_t k_lane = (lane / CPR) * p.k.token_stride + (lane % CPR) * 16;
+  const uint32_t v_lane = (lane / CPR) * p.v.token_stride + (lane % CPR) * 16;
+  const float* const my_scale = lane == 0 ? p.k.scale : p.v.scale;  // lane 0 fetches the key scale, lane 1 the value's
+  const uint32_t my_scale_stride = lane == 0 ? p.k.scale_stride : p.v.scale_stride;
+  int a_j = -kUnit, a_end = 0, a_stage = 0;
+  int a_id = -1, a_in = 0;              // the step's block, and where in it the step begins
+  const int* a_entry = p.table;         // its table entry
+  const uint8_t *a_k = nullptr, *a_v = nullptr;  // the lane's first byte in block 0
+  bool a_done = false;
+  auto a_next = [&]() {  // to the next step
+    a_j += kUnit;
+    a_in += kUnit;
+    if (a_j >= a_end) {
+      do {
+        if (ahead.u >= end) {
+          a_done = true;
+          return;
+        }
+        ahead.next<R>(p, end);
+        a_j = ahead.first_key + warp * 16;
+        a_end = ahead.key_end(p);
+      } while (a_j >= a_end);
+      a_entry = p.table + static_cast<int64_t>(ahead.b) * p.table_stride + a_j / p.block;
+      a_in = a_j % p.block;
+      a_k = p.k.codes + static_cast<int64_t>(ahead.h) * p.k.head_stride + k_lane;
+      a_v = p.v.codes + static_cast<int64_t>(ahead.h) * p.v.head_stride + v_lane;
     }
-    const int64_t local = u - at;
-    const int item = static_cast<int>(local / shape.units), u0 = static_cast<int>(local % shape.units);
-    const int n_units = static_cast<int>(min(static_cast<int64_t>(shape.units - u0), end - u));
-    u += n_units;
-    const int h = item % p.Hkv, tile = item / p.Hkv;
-    const NewRows fresh = new_rows(p, b);
-    const int q0 = fresh.first, n = fresh.n;
-    const int ctx = min(p.context[b], p.max_table_tokens);
-    const int row0 = tile * R, rows = min(R, n * p.group - row0);
-    // keys that a row sees: [0, lim)
-    auto lim_of = [&](int row) { return min(ctx, p.context[b] - n + (row0 + min(row, rows - 1)) / p.group + 1); };
-    const int lim_first = lim_of(0), lim_last = lim_of(rows - 1);
-    const int* table = p.table + static_cast<int64_t>(b) * p.table_stride;
-    const uint8_t* kbase = p.k.codes + h * p.k.head_stride + t * VB;
-    const uint8_t* vbase = p.v.codes + h * p.v.head_stride + g * (D / 8);
-    const int key_end = min(lim_last, (u0 + n_units) * kUnit);
-    const int step0 = u0 * kUnit + warp * 16;
-
-    auto block_of = [&](int j) { return j < key_end ? __ldg(table + j / p.block) : -1; };
-    auto load = [&](Raw<D>& r, int j, int id) {
-      // a key without a block (none given, or outside the cache) counts as masked: nothing is read for it
-      if (static_cast<unsigned>(id) >= static_cast<unsigned>(p.blocks)) {
-        r.ks = -1.f;
-        return;
+    while (a_in >= p.block) {
+      a_in -= p.block;
+      ++a_entry;
+    }
+    a_id = __ldg(a_entry);
+  };
+  auto fetch = [&]() {
+    if (!a_done) {
+      const uint32_t dst = ring_u32 + a_stage * L::kStep;
+      if (static_cast<uint32_t>(a_id) < static_cast<uint32_t>(p.blocks)) {
+        const uint32_t id = a_id;
+        const uint8_t* kp = a_k + static_cast<uint64_t>(id) * p.k.block_stride + a_in * p.k.token_stride;
+        const uint8_t* vp = a_v + static_cast<uint64_t>(id) * p.v.block_stride + a_in * p.v.token_stride;
+#pragma unroll
+        for (int i = 0; i < 16 / RPI; ++i) {
+          const int at = put[i & 1] + (i >> 1) * (2 * RPI * D);
+          cp_async16(dst + at, kp);
+          cp_async16(dst + 16 * D + at, vp);
+          kp += RPI * p.k.token_stride;
+          vp += RPI * p.v.token_stride;
+        }
+        if (lane < 2) cp_async4(scale_u32 + a_stage * 8 + lane * 4, my_scale + static_cast<uint64_t>(id) * my_scale_stride + ahead.h);
+      } else if (lane == 0) {  // a key without a block (none given, or outside the cache) counts as masked
+        s_scale[warp][a_stage][0] = -1.f;
       }
-      const int in = j % p.block;
-      r.ks = __ldg(p.k.scale + static_cast<int64_t>(id) * p.k.scale_stride + h);
-      r.vs = __ldg(p.v.scale + static_cast<int64_t>(id) * p.v.scale_stride + h);
-      const uint8_t* kp = kbase + static_cast<int64_t>(id) * p.k.block_stride + (in + g) * p.k.token_stride;
-      const uint8_t* vp = vbase + static_cast<int64_t>(id) * p.v.block_stride + (in + 2 * t) * p.v.token_stride;
+      a_stage = a_stage + 1 == S ? 0 : a_stage + 1;
+      a_next();
+    }
+    cp_async_commit();
+  };
+  a_next();
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int c = 0; c < CH; ++c) r.k[x][c].load(kp + x * 8 * p.k.token_stride + c * 4 * VB);
-#pragma unroll
-      for (int x = 0; x < 4; ++x) r.v[x].load(vp + ((x & 1) + (x >> 1) * 8) * p.v.token_stride);
-    };
-    Raw<D> cur, next;
-    int id_next = block_of(step0 + kUnit);
-    if (step0 < key_end) load(cur, step0, block_of(step0));
+  for (int i = 0; i < S - 1; ++i) fetch();
+  int stage = 0;
+
+  while (now.u < end) {
+    now.next<R>(p, end);
+    const int rows = now.rows;
+    const int lim_first = now.lim_of(p, 0), lim_last = now.lim_of(p, rows - 1);
+    const int key_end = now.key_end(p);
 
     // ---- query rows as f16 fragments: each row divided by a power of two that brings its largest number to [1, 2)
-    uint32_t q[MT][D / 16][4];
-    float unit[MT][2];
+    uint32_t q[kQInSmem ? 1 : N][D / 16][2];
+    float unit[N][2];  // of the rows 2t, 2t + 1: what a product of codes and fragments is worth, but for the key's scale
+    auto load_q = [&](int n, uint32_t (*frag)[2]) {  // row g of tile n; returns the row's unit
+      const int row = n * 8 + g;
+      float x[D / 4];
+      float m = 0.f;
+      if (row < rows) {
+        const int r = now.row0 + row;
+        const bf16* src = p.q + static_cast<int64_t>(now.q0 + r / p.group) * p.q_token + (now.h * p.group + r % p.group) * p.q_head;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+        for (int c = 0; c < CH; ++c)
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int row = mt * 16 + half * 8 + g;
-        float x[D / 4];
-        float m = 0.f;
-        if (row < rows) {
-          const int r = row0 + row;
-          const bf16* src = p.q + static_cast<int64_t>(q0 + r / p.group) * p.q_token + (h * p.group + r % p.group) * p.q_head;
+          for (int i = 0; i < VB; i += 8) {
+            const uint4 w = __ldg(reinterpret_cast<const uint4*>(src + c * 4 * VB + t * VB + i));
+            const __nv_bfloat162* y = reinterpret_cast<const __nv_bfloat162*>(&w);
 #pragma unroll
-          for (int c = 0; c < CH; ++c)
-#pragma unroll
-            for (int i = 0; i < VB; i += 4) {
-              const uint2 w = *reinterpret_cast<const uint2*>(src + c * 4 * VB + t * VB + i);
-              const float2 lo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w.x));
-              const float2 hi = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w.y));
-              float* y = x + c * VB + i;
-              y[0] = lo.x; y[1] = lo.y; y[2] = hi.x; y[3] = hi.y;
+            for (int e = 0; e < 4; ++e) {
+              const float2 f = __bfloat1622float2(y[e]);
+              x[c * VB + i + 2 * e] = f.x;
+              x[c * VB + i + 2 * e + 1] = f.y;
             }
+          }
 #pragma unroll
-          for (int i = 0; i < D / 4; ++i) m = fmaxf(m, fabsf(x[i]));
-        } else {
+        for (int i = 0; i < D / 4; ++i) m = fmaxf(m, fabsf(x[i]));
+      } else {
 #pragma unroll
-          for (int i = 0; i < D / 4; ++i) x[i] = 0.f;
-        }
-        m = quad_max(m);
-        const uint32_t bits = __float_as_uint(m);
-        const int e = min(max(static_cast<int>(bits >> 23) - 127, -100), 126);
-        const bool fine = m > 0.f && m <= 3.4028234e38f;  // zero or infinite rows as they are
-        const float inv = fine ? exp2i(-e) : 1.f;
-        unit[mt][half] = (fine ? exp2i(e) : 1.f) * p.scale * kLog2e;
-#pragma unroll
-        for (int s = 0; s < D / 16; ++s) {
-          q[mt][s][half] = pack_f16(x[4 * s] * inv, x[4 * s + 1] * inv);
-          q[mt][s][2 + half] = pack_f16(x[4 * s + 2] * inv, x[4 * s + 3] * inv);
-        }
+        for (int i = 0; i < D / 4; ++i) x[i] = 0.f;
       }
-
-    float o[MT][NT][4];
-    float m_run[MT][2], l_run[MT][2];
-    float v_ref[MT][2], v_up[MT][2];  // the largest value scale that the row has seen, and kWeightUp over it
+      m = quad_max(m);
+      const int e = min(max(static_cast<int>(__float_as_uint(m) >> 23) - 127, -100), 126);
+      const bool fine = m > 0.f && m <= 3.4028234e38f;  // zero or infinite rows as they are
+      const float inv = fine ? exp2i(-e) : 1.f;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
+      for (int s = 0; s < D / 16; ++s) {
+        frag[s][0] = pack_f16(x[4 * s] * inv, x[4 * s + 1] * inv);
+        frag[s][1] = pack_f16(x[4 * s + 2] * inv, x[4 * s + 3] * inv);
+      }
+      return (fine ? exp2i(e) : 1.f) * p.scale * kLog2e;
+    };
+    if constexpr (!kQInSmem) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
+      for (int n = 0; n < N; ++n) {
+        const float u = load_q(n, q[n]);
+        unit[n][0] = __shfl_sync(0xffffffffu, u, 8 * t);
+        unit[n][1] = __shfl_sync(0xffffffffu, u, 8 * t + 4);
+      }
+    } else {  // a warp makes each tile's fragments, all read them from shared memory
+      if (warp < N) {
+        uint32_t frag[D / 16][2];
+        const float u = load_q(warp, frag);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[mt][i][e] = 0.f;
-      m_run[mt][0] = m_run[mt][1] = -INFINITY;
-      l_run[mt][0] = l_run[mt][1] = 0.f;
-      v_ref[mt][0] = v_ref[mt][1] = v_up[mt][0] = v_up[mt][1] = 0.f;
+        for (int s = 0; s < D / 16; ++s) s_q[(warp * (D / 16) + s) * 32 + lane] = make_uint2(frag[s][0], frag[s][1]);
+        if (t == 0) s_unit[warp * 8 + g] = u;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        unit[n][0] = s_unit[n * 8 + 2 * t];
+        unit[n][1] = s_unit[n * 8 + 2 * t + 1];
+      }
     }
 
-    for (int j = step0; j < key_end; j += kUnit) {
-      const int id_after = block_of(j + 2 * kUnit);
-      if (j + kUnit < key_end) load(next, j + kUnit, id_next);
-      if (cur.ks >= 0.f) {
+    // o[n][i]: dims g * D / 8 + 2i (first two: rows 2t, 2t + 1) and + 2i + 1 (last two)
+    float o[N][NT][4];
+    float m_run[N][2], l_run[N][2];
+    float v_ref[N][2], v_up[N][2];  // the largest value scale that the row has seen, and kWeightUp over it
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m_run[n][e] = kNone;
+        l_run[n][e] = v_ref[n][e] = v_up[n][e] = 0.f;
+      }
+    }
+
+    for (int j = now.first_key + warp * 16; j < key_end; j += kUnit) {
+      cp_async_wait<S - 2>();
+      __syncwarp();
+      const uint8_t* step = ring + stage * L::kStep;
+      const float2 sc = *reinterpret_cast<const float2*>(s_scale[warp][stage]);
+      const float ks = sc.x, vs = sc.y;
+      if (ks >= 0.f) {
         const bool edge = j + 16 > lim_first;
+        // ---- scores: 16 keys x rows. Keys g, 8 + g are the rows of the MMA, queries its columns
+        float s[N][4];
+#pragma unroll
+        for (int n = 0; n < N; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          uint32_t kw[2][VB / 4];  // dims c * 4 VB + t * VB ...
+#pragma unroll
+          for (int x = 0; x < 2; ++x) lds<VB>(kw[x], step + key_at[c] + x * 8 * D);
+#pragma unroll
+          for (int i = 0; i < VB / 4; ++i) {
+            uint32_t lo[2], hi[2];
+            Kv<FMT>::decode4(kw[0][i], lo[0], hi[0]);
+            Kv<FMT>::decode4(kw[1][i], lo[1], hi[1]);
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+              if constexpr (kQInSmem) {
+                const uint2 w = s_q[(n * (D / 16) + c * (VB / 4) + i) * 32 + lane];
+                mma_f16(s[n], lo[0], lo[1], hi[0], hi[1], w.x, w.y);
+              } else {
+                mma_f16(s[n], lo[0], lo[1], hi[0], hi[1], q[n][c * (VB / 4) + i][0], q[n][c * (VB / 4) + i][1]);
+              }
+            }
+          }
+        }
+        // ---- probabilities of the rows 2t, 2t + 1 (e) and the keys j + g, j + g + 8
+        bool moved = false;
+        float top[N][2], v_top[N][2];
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float f = unit[n][e] * ks;
+            s[n][e] *= f;
+            s[n][2 + e] *= f;
+            v_top[n][e] = vs;
+            if (edge) {
+              const int lim = now.lim_of(p, n * 8 + 2 * t + e) - j;
+              if (lim <= g) s[n][e] = -INFINITY;
+              if (lim <= g + 8) s[n][2 + e] = -INFINITY;
+              if (lim <= 0) v_top[n][e] = 0.f;
+            }
+            top[n][e] = fmaxf(s[n][e], s[n][2 + e]);
+            moved = moved || top[n][e] > m_run[n][e] + kLazy || v_top[n][e] > v_ref[n][e];
+          }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+          for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float v_new = fmaxf(v_ref[n][e], v_top[n][e]);
+              const float m_new = fmaxf(m_run[n][e], column_max(top[n][e]));
+              const float f = exp2f_approx(m_run[n][e] - m_new);
+              const float fo = v_ref[n][e] > 0.f ? f * (v_ref[n][e] / v_new) : 0.f;
+              m_run[n][e] = m_new;
+              l_run[n][e] *= f;
+#pragma unroll
+              for (int i = 0; i < NT; ++i) {
+                o[n][i][e] *= fo;
+                o[n][i][2 + e] *= fo;
+              }
+              v_ref[n][e] = v_new;
+              v_up[n][e] = v_new > 0.f ? kWeightUp / v_new : 0.f;
+            }
+        }
+        uint32_t w[N][2];  // weights as the second operand: keys 2t, 2t + 1 (and + 8) of row g
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          float pr[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) pr[e] = exp2f_approx(s[n][e] - m_run[n][e & 1]);
+          l_run[n][0] += pr[0] + pr[2];
+          l_run[n][1] += pr[1] + pr[3];
+          const float u0 = v_up[n][0] * vs, u1 = v_up[n][1] * vs;
+          w[n][0] = transpose8(pack_f16(pr[0] * u0, pr[1] * u1));
+          w[n][1] = transpose8(pack_f16(pr[2] * u0, pr[3] * u1));
+        }
+        // ---- output: values 2t, 2t + 1, 2t + 8, 2t + 9, dims g * D / 8 ..., four dims at a time
+        uint32_t vw[4][D / 32];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) lds<D / 8>(vw[x], step + val_at[x & 1] + (x >> 1) * 8 * D);
         if (edge) {  // values past the last row's limit may be anything: they count as zero
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             const int key = j + 2 * t + (x & 1) + (x >> 1) * 8;
-            if (key >= lim_last) {
-              cur.v[x].zero();
-            } else if (key >= lim_first) {  // seen by some rows only: a NaN must not reach the others
 #pragma unroll
-              for (int i = 0; i < D / 32; ++i) {
-                const uint32_t bad = Kv<FMT>::nan_bytes(cur.v[x].w[i]);
-                if (bad) {
+            for (int i = 0; i < D / 32; ++i) {
+              if (key >= lim_last) {
+                vw[x][i] = 0;
+              } else if (key >= lim_first) {  // seen by some rows only: a NaN must not reach the others
+                const uint32_t bad = Kv<FMT>::nan_bytes(vw[x][i]);
+                if (bad)
                   for (int e = 0; e < 4; ++e)
                     if ((bad >> (8 * e + 7)) & 1) {
                       atomicMin(&s_poison[g * (D / 8) + 4 * i + e], key);
-                      cur.v[x].w[i] &= ~(0xffu << (8 * e));
+                      vw[x][i] &= ~(0xffu << (8 * e));
                     }
-                }
               }
             }
           }
         }
-        // ---- scores: rows x 16 keys
-        float s[MT][2][4];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[mt][x][e] = 0.f;
-#pragma unroll
-        for (int c = 0; c < CH; ++c)
-#pragma unroll
-          for (int i = 0; i < VB / 4; ++i)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              uint32_t b0, b1;
-              Kv<FMT>::decode4(cur.k[x][c].w[i], b0, b1);
-#pragma unroll
-              for (int mt = 0; mt < MT; ++mt) mma_f16(s[mt][x], q[mt][c * (VB / 4) + i], b0, b1);
-            }
-        // ---- probabilities
-        bool moved = false;
-        float top[MT][2], v_top[MT][2];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const float f = unit[mt][half] * cur.ks;
-            const int lim = edge ? lim_of(mt * 16 + half * 8 + g) - j : 16;
-            float mx = -INFINITY;
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                float& y = s[mt][x][half * 2 + e];
-                y = x * 8 + 2 * t + e < lim ? y * f : -INFINITY;
-                mx = fmaxf(mx, y);
-              }
-            top[mt][half] = mx;
-            v_top[mt][half] = lim > 0 ? cur.vs : 0.f;
-            moved = moved || mx > m_run[mt][half] + kLazy || v_top[mt][half] > v_ref[mt][half];
-          }
-        if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const float v_new = fmaxf(v_ref[mt][half], v_top[mt][half]);
-              const float vf = v_ref[mt][half] > 0.f ? v_ref[mt][half] / v_new : 0.f;
-              const float m_new = fmaxf(m_run[mt][half], quad_max(top[mt][half]));
-              const float f = m_run[mt][half] == -INFINITY ? 0.f : exp2f_approx(m_run[mt][half] - m_new);
-              m_run[mt][half] = m_new;
-              l_run[mt][half] *= f;
-#pragma unroll
-              for (int i = 0; i < NT; ++i) {
-                o[mt][i][half * 2] *= f * vf;
-                o[mt][i][half * 2 + 1] *= f * vf;
-              }
-              v_ref[mt][half] = v_new;
-              v_up[mt][half] = v_new > 0.f ? kWeightUp / v_new : 0.f;
-            }
-        }
-        uint32_t w[MT][4];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const float m = m_run[mt][half] == -INFINITY ? 0.f : m_run[mt][half];
-            const float up = v_up[mt][half] * cur.vs;
-            float pr[2][2];
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) pr[x][e] = exp2f_approx(s[mt][x][half * 2 + e] - m);
-            l_run[mt][half] += (pr[0][0] + pr[0][1]) + (pr[1][0] + pr[1][1]);
-            w[mt][half] = pack_f16(pr[0][0] * up, pr[0][1] * up);
-            w[mt][2 + half] = pack_f16(pr[1][0] * up, pr[1][1] * up);
-          }
-        // ---- output: four dims of the lane's values at a time
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
           uint32_t b0[4], b1[4];
-          Kv<FMT>::decode4(__byte_perm(cur.v[0].w[i], cur.v[1].w[i], 0x5140), b0[0], b0[1]);
-          Kv<FMT>::decode4(__byte_perm(cur.v[0].w[i], cur.v[1].w[i], 0x7362), b0[2], b0[3]);
-          Kv<FMT>::decode4(__byte_perm(cur.v[2].w[i], cur.v[3].w[i], 0x5140), b1[0], b1[1]);
-          Kv<FMT>::decode4(__byte_perm(cur.v[2].w[i], cur.v[3].w[i], 0x7362), b1[2], b1[3]);
+          Kv<FMT>::decode4(__byte_perm(vw[0][i], vw[1][i], 0x5140), b0[0], b0[1]);
+          Kv<FMT>::decode4(__byte_perm(vw[0][i], vw[1][i], 0x7362), b0[2], b0[3]);
+          Kv<FMT>::decode4(__byte_perm(vw[2][i], vw[3][i], 0x5140), b1[0], b1[1]);
+          Kv<FMT>::decode4(__byte_perm(vw[2][i], vw[3][i], 0x7362), b1[2], b1[3]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+          for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) mma_f16(o[mt][4 * i + e], w[mt], b0[e], b1[e]);
+            for (int n = 0; n < N; ++n)
+              mma_f16(o[n][2 * i + e], b0[2 * e], b0[2 * e + 1], b1[2 * e], b1[2 * e + 1], w[n][0], w[n][1]);
         }
       }
-      cur = next;
-      id_next = id_after;
+      stage = stage + 1 == S ? 0 : stage + 1;
+      __syncwarp();  // every lane has read the stage that is filled next
+      fetch();
     }
 
-    // ---- the four warps' results of this piece into one
+    // ---- the four warps' results of this piece into one, a few rows at a time
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int n = 0; n < N; ++n)
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int row = mt * 16 + half * 8 + g;
-        const float l = quad_sum(l_run[mt][half]);
-        if (t == 0) {
-          s_mlv[warp][row][0] = m_run[mt][half];
-          s_mlv[warp][row][1] = l;
-          s_mlv[warp][row][2] = v_ref[mt][half];
+      for (int e = 0; e < 2; ++e) {
+        const float l = column_sum(l_run[n][e]);
+        if (g == 0) {
+          float* dst = s_mlv[warp][n * 8 + 2 * t + e];
+          dst[0] = m_run[n][e];
+          dst[1] = l;
+          dst[2] = v_ref[n][e];
         }
-        if (row < rows) {
-          float* dst = s_o + (warp * R + row) * D;
+      }
+    const bool whole = now.units == now.shape.units;
+    const int64_t slot = now.u0 > 0 ? 2 * static_cast<int64_t>(blockIdx.x) : 2 * static_cast<int64_t>(blockIdx.x) + 1;
 #pragma unroll
-          for (int i = 0; i < NT; ++i) {  // lane t holds the dims (2t) D/8 + i and (2t + 1) D/8 + i
-            dst[2 * t * (D / 8) + i] = o[mt][i][half * 2];
-            dst[(2 * t + 1) * (D / 8) + i] = o[mt][i][half * 2 + 1];
+    for (int n = 0; n < N; ++n) {
+      const int first = n * 8;  // rows of this turn
+      if (first < rows) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (first + 2 * t + e < rows) {
+            float* dst = s_o + (warp * 8 + 2 * t + e) * D + g * (D / 8);
+#pragma unroll
+            for (int i = 0; i < NT; i += 2)
+              *reinterpret_cast<float4*>(dst + 2 * i) = make_float4(o[n][i][e], o[n][i][2 + e], o[n][i + 1][e], o[n][i + 1][2 + e]);
+          }
+        __syncthreads();
+        for (int i = threadIdx.x; i < min(8, rows - first) * (D / 4); i += kThreads) {
+          const int in = i / (D / 4), row = first + in, d = (i % (D / 4)) * 4;
+          float m = kNone;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_mlv[w][row][0]);
+          float l = 0.f;
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) {
+            const float mw = s_mlv[w][row][0];
+            const float f = exp2f_approx(mw - m);
+            const float fv = f * s_mlv[w][row][2] * (1.f / kWeightUp);
+            l += s_mlv[w][row][1] * f;
+            const float4 x = *reinterpret_cast<const float4*>(s_o + (w * 8 + in) * D + d);
+            acc.x += x.x * fv; acc.y += x.y * fv; acc.z += x.z * fv; acc.w += x.w * fv;
+          }
+          const int lim = now.lim_of(p, row);
+          if (s_poison[d] < lim) acc.x = __int_as_float(0x7fffffff);
+          if (s_poison[d + 1] < lim) acc.y = __int_as_float(0x7fffffff);
+          if (s_poison[d + 2] < lim) acc.z = __int_as_float(0x7fffffff);
+          if (s_poison[d + 3] < lim) acc.w = __int_as_float(0x7fffffff);
+          if (whole) {
+            const float inv = m == kNone ? 0.f : 1.f / l;  // a row that sees no key is zero
+            const int r = now.row0 + row;
+            bf16* dst = p.out + static_cast<int64_t>(now.q0 + r / p.group) * p.o_token + (now.h * p.group + r % p.group) * p.o_head + d;
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+          } else {
+            *reinterpret_cast<float4*>(p.part_o + (slot * R + row) * D + d) = acc;
+            if (d == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * R + row) * 2) = make_float2(m, l);
           }
         }
-      }
-    __syncthreads();
-    const bool whole = n_units == shape.units;
-    const int64_t slot = u0 > 0 ? 2 * static_cast<int64_t>(blockIdx.x) : 2 * static_cast<int64_t>(blockIdx.x) + 1;
-    for (int i = threadIdx.x; i < rows * (D / 4); i += kThreads) {
-      const int row = i / (D / 4), d = (i % (D / 4)) * 4;
-      float m = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_mlv[w][row][0]);
-      float l = 0.f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float mw = s_mlv[w][row][0];
-        const float f = mw == -INFINITY ? 0.f : exp2f_approx(mw - m);
-        const float fv = f * s_mlv[w][row][2] * (1.f / kWeightUp);
-        l += s_mlv[w][row][1] * f;
-        const float4 x = *reinterpret_cast<const float4*>(s_o + (w * R + row) * D + d);
-        acc.x += x.x * fv; acc.y += x.y * fv; acc.z += x.z * fv; acc.w += x.w * fv;
-      }
-      const int lim = lim_of(row);
-      if (s_poison[d] < lim) acc.x = __int_as_float(0x7fffffff);
-      if (s_poison[d + 1] < lim) acc.y = __int_as_float(0x7fffffff);
-      if (s_poison[d + 2] < lim) acc.z = __int_as_float(0x7fffffff);
-      if (s_poison[d + 3] < lim) acc.w = __int_as_float(0x7fffffff);
-      if (whole) {
-        const float inv = m == -INFINITY ? 0.f : 1.f / l;  // a row that sees no key is zero
-        const int r = row0 + row;
-        bf16* dst = p.out + static_cast<int64_t>(q0 + r / p.group) * p.o_token + (h * p.group + r % p.group) * p.o_head + d;
-        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
-      } else {
-        *reinterpret_cast<float4*>(p.part_o + (slot * R + row) * D + d) = acc;
-        if (d == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * R + row) * 2) = make_float2(m, l);
+        __syncthreads();
       }
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < D; i += kThreads) s_poison[i] = 0x7fffffff;
-    __syncthreads();
+    if (FMT == kKvFp8 && key_end > lim_first) {  // uniform: only then a NaN may have been noted
+      for (int i = threadIdx.x; i < D; i += kThreads) s_poison[i] = 0x7fffffff;
+      __syncthreads();
+    }
   }
+  cp_async_wait<0>();
   griddep_launch();
 }
 
@@ -484,16 +645,16 @@ __global__ void __launch_bounds__(128) cached_attn_join_kernel(CachedAttn p, int
       const int workers = static_cast<int>(min(static_cast<int64_t>(workers_max), total));
       const int w0 = worker_of(u0, total, workers), w1 = worker_of(u0 + s.units - 1, total, workers);
       if (w0 == w1) return;  // one range had the whole item
-      float m = -INFINITY;
+      float m = kNone;
       for (int w = w0 + lane; w <= w1; w += 32)
         m = fmaxf(m, p.part_ml[((2 * static_cast<int64_t>(w) + (w == w0)) * R + row) * 2]);
       m = warp_max(m);
-      if (m > -INFINITY) {
+      {
 #pragma unroll 4
         for (int w = w0; w <= w1; ++w) {
           const int64_t at = (2 * static_cast<int64_t>(w) + (w == w0)) * R + row;
           const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
-          const float f = ml.x == -INFINITY ? 0.f : exp2f_approx(ml.x - m);
+          const float f = exp2f_approx(ml.x - m);
           l += ml.y * f;
           const float* src = p.part_o + at * D + lane * PER;
 #pragma unroll
@@ -507,41 +668,45 @@ __global__ void __launch_bounds__(128) cached_attn_join_kernel(CachedAttn p, int
   for (int e = 0; e < PER; ++e) dst[e] = __float2bfloat16(acc[e] * inv);
 }
 
-// Resident blocks of threads on 148 SMs: two per SM with one row tile (the registers), one with two.
-int cached_attn_workers(int mt) { return 148 * (mt == 1 ? 2 : 1); }
+template <typename F>
+auto with_shape(int D, int rows, F&& f) {
+  using std::integral_constant;
+  auto by_rows = [&](auto d) {
+    if (rows <= 8) return f(d, integral_constant<int, 8>{});
+    if (rows <= 16) return f(d, integral_constant<int, 16>{});
+    if (rows <= 24) return f(d, integral_constant<int, 24>{});
+    return f(d, integral_constant<int, 32>{});
+  };
+  if (D == 32) return by_rows(integral_constant<int, 32>{});
+  if (D == 64) return by_rows(integral_constant<int, 64>{});
+  return by_rows(integral_constant<int, 128>{});
+}
 
-template <int FMT, int D, int MT>
+int workers_of(int D, int rows) {
+  return 148 * with_shape(D, rows, [](auto d, auto r) { return Layout<d(), r()>::kPerSm; });
+}
+
+template <int FMT, int D, int ROWS>
 void launch(const CachedAttn& p, cudaStream_t stream) {
-  auto kernel = cached_attn_kernel<FMT, D, MT>;
-  constexpr int smem = kWarps * 16 * MT * D * static_cast<int>(sizeof(float));
+  auto kernel = cached_attn_kernel<FMT, D, ROWS>;
+  constexpr int smem = Layout<D, ROWS>::kTotal;
   static const bool configured = [&] {
     check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cached_attention smem");
     return true;
   }();
   (void)configured;
-  const int workers = cached_attn_workers(MT);
+  const int workers = 148 * Layout<D, ROWS>::kPerSm;
   launch_pdl(kernel, dim3(workers), dim3(kThreads), smem, stream, "cached_attention", p);
   const int64_t rows = static_cast<int64_t>(p.T) * p.Hkv * p.group;
   launch_pdl(cached_attn_join_kernel<D>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), 0, stream,
-             "cached_attention join", p, workers, 16 * MT);
+             "cached_attention join", p, workers, ROWS);
 }
 
-template <int FMT>
-void dispatch(const CachedAttn& p, int D, int mt, cudaStream_t stream) {
-  if (mt == 1) {
-    if (D == 32) launch<FMT, 32, 1>(p, stream);
-    else if (D == 64) launch<FMT, 64, 1>(p, stream);
-    else launch<FMT, 128, 1>(p, stream);
-  } else {
-    if (D == 32) launch<FMT, 32, 2>(p, stream);
-    else if (D == 64) launch<FMT, 64, 2>(p, stream);
-    else launch<FMT, 128, 2>(p, stream);
-  }
-}
-
-void cached_attention_rows(const CachedAttn& p, int D, int fmt, int mt, cudaStream_t stream) {
-  if (fmt == kKvFp8) dispatch<kKvFp8>(p, D, mt, stream);
-  else dispatch<kKvInt8>(p, D, mt, stream);
+void cached_attention_rows(const CachedAttn& p, int D, int fmt, int rows, cudaStream_t stream) {
+  with_shape(D, rows, [&](auto d, auto r) {
+    if (fmt == kKvFp8) launch<kKvFp8, d(), r()>(p, stream);
+    else launch<kKvInt8, d(), r()>(p, stream);
+  });
 }
 
 int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
@@ -549,7 +714,7 @@ int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 // Which kernel, and how its work is split.
 struct Way {
   bool prompt;
-  int mt;                   // few rows: 16-row tiles per block of threads
+  int tile;                 // few rows: rows of a tile
   int tiles_max, splits;    // prompts
   int64_t part_o, part_ml, bytes;  // of the workspace; the prefix sums are at its beginning
 };
@@ -559,7 +724,7 @@ Way way_of(int T, int B, int Hq, int Hkv, int D, int max_query, int max_context)
   const int group = Hq / Hkv;
   const int64_t rows = static_cast<int64_t>(std::min(max_query, T)) * group;
   w.prompt = D != 32 && rows > 32;
-  w.mt = rows <= 16 ? 1 : 2;
+  w.tile = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 24 ? 24 : 32;
   int64_t slots;
   if (w.prompt) {
     w.tiles_max = static_cast<int>(static_cast<int64_t>(T) * group / kPromptRows + B);
@@ -568,7 +733,7 @@ Way way_of(int T, int B, int Hq, int Hkv, int D, int max_query, int max_context)
     w.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(148 / std::max<int64_t>(blocks, 1), max_context / 256)));
     slots = w.splits > 1 ? blocks * w.splits * kPromptRows : 0;
   } else {
-    slots = 2 * static_cast<int64_t>(cached_attn_workers(w.mt)) * 16 * w.mt;
+    slots = 2 * static_cast<int64_t>(workers_of(D, w.tile)) * w.tile;
   }
   w.part_o = align256((static_cast<int64_t>(B) + 1) * sizeof(int64_t));
   w.part_ml = w.part_o + align256(slots * D * sizeof(float));
@@ -596,8 +761,13 @@ void cached_attention(const bf16* q, int64_t q_token, int64_t q_head, bf16* out,
   p.out = out;
   p.o_token = o_token;
   p.o_head = o_head;
-  p.k = {static_cast<const uint8_t*>(k.codes), k.block_stride, k.head_stride, k.token_stride, k.scale, k.scale_stride};
-  p.v = {static_cast<const uint8_t*>(v.codes), v.block_stride, v.head_stride, v.token_stride, v.scale, v.scale_stride};
+  auto pages = [](const KvPages& x) {
+    return CachedPages{static_cast<const uint8_t*>(x.codes), static_cast<uint32_t>(x.block_stride),
+                       static_cast<uint32_t>(x.head_stride), static_cast<uint32_t>(x.token_stride), x.scale,
+                       static_cast<uint32_t>(x.scale_stride)};
+  };
+  p.k = pages(k);
+  p.v = pages(v);
   p.table = table;
   p.table_stride = table_stride;
   p.context = context;
@@ -614,7 +784,7 @@ void cached_attention(const bf16* q, int64_t q_token, int64_t q_head, bf16* out,
   p.part_o = reinterpret_cast<float*>(base + w.part_o);
   p.part_ml = reinterpret_cast<float*>(base + w.part_ml);
   if (w.prompt) cached_attention_prompt(p, D, fmt, w.tiles_max, w.splits, stream);
-  else cached_attention_rows(p, D, fmt, w.mt, stream);
+  else cached_attention_rows(p, D, fmt, w.tile, stream);
 }
 
 int cached_attention_status(bool clear) { return read_status_word(clear); }

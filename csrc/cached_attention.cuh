@@ -5,11 +5,13 @@
 
 namespace qw {
 
-struct CachedPages {  // keys or values: [blocks, Hkv, block, D] codes, [blocks, Hkv] scales
+// Keys or values: [blocks, Hkv, block, D] codes, [blocks, Hkv] scales. Strides below 2^32 (checked where tensors come in),
+// so that an address takes 32 x 32-bit products.
+struct CachedPages {
   const uint8_t* codes;
-  int64_t block_stride, head_stride, token_stride;
+  uint32_t block_stride, head_stride, token_stride;
   const float* scale;
-  int64_t scale_stride;
+  uint32_t scale_stride;
 };
 
 struct CachedAttn {

@@ -214,9 +214,10 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
     constexpr int NP = 64 / KPP;         // pieces per thread of a half tile (64 keys)
     const int piece = threadIdx.x % CPK, key_in = threadIdx.x / CPK;
     const int* table = p.table + static_cast<int64_t>(b) * p.table_stride;
-    const uint8_t* base[2] = {p.k.codes + h * p.k.head_stride + piece * 16, p.v.codes + h * p.v.head_stride + piece * 16};
-    const int64_t block_stride[2] = {p.k.block_stride, p.v.block_stride};
-    const int64_t token_stride[2] = {p.k.token_stride, p.v.token_stride};
+    const uint8_t* base[2] = {p.k.codes + static_cast<int64_t>(h) * p.k.head_stride + piece * 16,
+                              p.v.codes + static_cast<int64_t>(h) * p.v.head_stride + piece * 16};
+    const uint32_t block_stride[2] = {p.k.block_stride, p.v.block_stride};
+    const uint32_t token_stride[2] = {p.k.token_stride, p.v.token_stride};
     // half tiles in the order K lower, K upper, V lower, V upper of each tile; two in flight
     uint4 raw[2][NP];
     float scale[2];
