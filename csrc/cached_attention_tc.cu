@@ -39,19 +39,21 @@ constexpr int kRows = kPromptRows;  // rows of a block of threads
 constexpr int kThreads = 13 * 32;
 constexpr int kTmemCols = 512;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLazy = 6.f;
-constexpr float kWeightUp = 256.f;
+constexpr float kNone = -3e38f;       // running maximum of a row that has seen no key
+constexpr float kLazy = 6.f;          // the running maximum moves when a row grows by more than 2^6
+constexpr float kWeightUpLog2 = 8.f;  // weights in f16: at most 2^14
 
 template <int D>
 struct Layout {
   static constexpr bool kAlias = D == 128;                  // P_g in S_g's columns
-  static constexpr int kStages = D == 64 ? 4 : 2;
+  static constexpr int kStages = D == 64 ? 4 : 2;  // all that fits
   static constexpr int kBoxes = D / 64;                      // 64-wide (128-byte) column boxes
   static constexpr int kQBytes = kBoxes * kGroupRows * 128;  // one group's rows
   static constexpr int kTileBytes = kBoxes * KT * 128;       // one K or V tile
   static constexpr int kKV = 2 * kQBytes;                    // stages of [K | V]
   static constexpr int kScale = kKV + kStages * 2 * kTileBytes;  // stages of k_scale[8], v_scale[8]
-  static constexpr int kPoison = kScale + kStages * 64;
+  static constexpr int kRaw = kScale + kStages * 64;         // codes of one K and one V tile on their way
+  static constexpr int kPoison = kRaw + 2 * KT * D;
   static constexpr int kBar = kPoison + D * 4;
   static constexpr int kTotal = kBar + 512 + 1024;           // barriers, and slack to align the base to 1 KB
   static constexpr int kTmemO = 256;
@@ -76,6 +78,11 @@ __device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t* v) {
       "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
       "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
+}
+
+// 16 bytes of global memory into shared memory, or zeros.
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const uint8_t* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 
 struct TcArgs {
@@ -214,71 +221,92 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
     constexpr int NP = 64 / KPP;         // pieces per thread of a half tile (64 keys)
     const int piece = threadIdx.x % CPK, key_in = threadIdx.x / CPK;
     const int* table = p.table + static_cast<int64_t>(b) * p.table_stride;
-    const uint8_t* base[2] = {p.k.codes + static_cast<int64_t>(h) * p.k.head_stride + piece * 16,
-                              p.v.codes + static_cast<int64_t>(h) * p.v.head_stride + piece * 16};
-    const uint32_t block_stride[2] = {p.k.block_stride, p.v.block_stride};
-    const uint32_t token_stride[2] = {p.k.token_stride, p.v.token_stride};
-    // half tiles in the order K lower, K upper, V lower, V upper of each tile; two in flight
-    uint4 raw[2][NP];
-    float scale[2];
-    auto fetch = [&](auto which, int slot, int j, int half) {
-      constexpr int kv = decltype(which)::value;
-      const int k0 = (t0 + j) * KT + half * 64;
-#pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        const int key = k0 + key_in + i * KPP;
-        raw[slot][i] = make_uint4(0, 0, 0, 0);
-        if (key < lim_any) {
-          const int id = __ldg(table + key / p.block);
-          if (static_cast<unsigned>(id) < static_cast<unsigned>(p.blocks))
-            raw[slot][i] = __ldg(reinterpret_cast<const uint4*>(base[kv] + static_cast<int64_t>(id) * block_stride[kv] +
-                                                                static_cast<int64_t>(key % p.block) * token_stride[kv]));
+    // the thread's byte in a 16-key group, and its places in a tile (they repeat every 8 keys)
+    const uint8_t* base[2] = {p.k.codes + static_cast<int64_t>(h) * p.k.head_stride + (key_in % 16) * p.k.token_stride + piece * 16,
+                              p.v.codes + static_cast<int64_t>(h) * p.v.head_stride + (key_in % 16) * p.v.token_stride + piece * 16};
+    const int sw = key_in & 7, c0 = (piece % 4) * 2;
+    // the pieces of the second column box store their halves in the other order: no bank is hit twice
+    const bool swap = piece >= 4;
+    const int put0 = (piece / 4) * (KT * 128) + key_in * 128 + ((c0 + (swap ? 1 : 0)) ^ sw) * 16;
+    const int put1 = (piece / 4) * (KT * 128) + key_in * 128 + ((c0 + (swap ? 0 : 1)) ^ sw) * 16;
+    // Lanes 0-7 look up the tile's 16-key groups: where the keys and values begin (-1: masked, without a block or past the
+    // last key that a row sees) and their scales. The block's id is read three tiles ahead and used two ahead, so that no
+    // thread waits for the dependent reads.
+    struct Groups {
+      int64_t at[2];
+      float scale[2];
+    };
+    auto id_of = [&](int j) {
+      const int key = (t0 + j) * KT + lane * 16;
+      return lane < 8 && j < nk && key < lim_any ? __ldg(table + key / p.block) : -1;
+    };
+    auto groups_of = [&](int j, int id) {
+      Groups x{{-1, -1}, {-1.f, 0.f}};
+      if (static_cast<unsigned>(id) < static_cast<unsigned>(p.blocks)) {
+        const uint32_t in = static_cast<uint32_t>((t0 + j) * KT + lane * 16) % static_cast<uint32_t>(p.block);
+        const uint64_t u = static_cast<uint32_t>(id);
+        x.at[0] = static_cast<int64_t>(u * p.k.block_stride + in * p.k.token_stride);
+        x.at[1] = static_cast<int64_t>(u * p.v.block_stride + in * p.v.token_stride);
+        if (warp == 0) {
+          x.scale[0] = __ldg(p.k.scale + u * p.k.scale_stride + h);
+          x.scale[1] = __ldg(p.v.scale + u * p.v.scale_stride + h);
         }
       }
-      // scales of the four 16-key groups; a group without a block counts as masked
-      scale[slot] = -1.f;
-      if (threadIdx.x < 4) {
-        const int key = k0 + threadIdx.x * 16;
-        const int id = key < lim_any ? __ldg(table + key / p.block) : -1;
-        if (static_cast<unsigned>(id) < static_cast<unsigned>(p.blocks))
-          scale[slot] = kv == 0 ? __ldg(p.k.scale + static_cast<int64_t>(id) * p.k.scale_stride + h)
-                                : __ldg(p.v.scale + static_cast<int64_t>(id) * p.v.scale_stride + h);
-      }
+      return x;
     };
-    auto store = [&](auto which, int slot, int j, int half) {
+    // The half tiles K lower, K upper, V lower, V upper: each fetched a whole tile before it is widened, into places of
+    // the thread's own (loads into registers wait for one another: a warp has few scoreboards).
+    uint8_t* raw = smem + L::kRaw + threadIdx.x * 16;
+    const uint32_t raw_u32 = smem_u32(raw);
+    auto fetch = [&](auto which, int half, const Groups& x) {
       constexpr int kv = decltype(which)::value;
-      const int st = j % kStages;
-      uint8_t* dst = smem + L::kKV + st * 2 * L::kTileBytes + kv * L::kTileBytes + (piece / 4) * (KT * 128);
-      const bool edge = kv == 1 && (t0 + j + 1) * KT > lim_all;
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
-        const int in = half * 64 + key_in + i * KPP;  // key in the tile
-        uint32_t w[4] = {raw[slot][i].x, raw[slot][i].y, raw[slot][i].z, raw[slot][i].w};
-        if (edge && (t0 + j) * KT + in >= lim_all) {  // seen by some rows only: a NaN must not reach the others
+        const int64_t at = __shfl_sync(0xffffffffu, x.at[kv], half * 4 + (key_in + i * KPP) / 16);
+        cp_async16_or_zero(raw_u32 + ((2 * kv + half) * NP + i) * 2048, at >= 0 ? base[kv] + at : base[kv], at >= 0);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto store = [&](auto which, int half, int j) {
+      constexpr int kv = decltype(which)::value;
+      asm volatile("cp.async.wait_group 3;" ::: "memory");  // four groups are on their way: the oldest has come
+      uint4 r[NP];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const uint32_t bad = Kv<FMT>::nan_bytes(w[c]);
-            if (bad)
-              for (int e = 0; e < 4; ++e)
-                if ((bad >> (8 * e + 7)) & 1) {
-                  atomicMin(&s_poison[piece * 16 + c * 4 + e], (t0 + j) * KT + in);
-                  w[c] &= ~(0xffu << (8 * e));
-                }
+      for (int i = 0; i < NP; ++i) r[i] = *reinterpret_cast<const uint4*>(raw + ((2 * kv + half) * NP + i) * 2048);
+      uint8_t* dst = smem + L::kKV + (j % kStages) * 2 * L::kTileBytes + kv * L::kTileBytes + half * 64 * 128;
+      if (kv == 1 && (t0 + j + 1) * KT > lim_all) {
+        // Keys that only some rows see: values past the last one may be anything and count as zero, and a NaN must not
+        // reach the rows that do not see it.
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const int key = (t0 + j) * KT + half * 64 + key_in + i * KPP;
+          if (key >= lim_any) r[i] = make_uint4(0, 0, 0, 0);
+          if (key >= lim_all) {
+            uint32_t w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const uint32_t bad = Kv<FMT>::nan_bytes(w[c]);
+              if (bad)
+                for (int e = 0; e < 4; ++e)
+                  if ((bad >> (8 * e + 7)) & 1) {
+                    atomicMin(&s_poison[piece * 16 + c * 4 + e], key);
+                    w[c] &= ~(0xffu << (8 * e));
+                  }
+            }
+            r[i] = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
-        uint4 lo, hi;
-        Kv<FMT>::decode4(w[0], lo.x, lo.y);
-        Kv<FMT>::decode4(w[1], lo.z, lo.w);
-        Kv<FMT>::decode4(w[2], hi.x, hi.y);
-        Kv<FMT>::decode4(w[3], hi.z, hi.w);
-        uint8_t* row = dst + in * 128;
-        const int c = (piece % 4) * 2, sw = in & 7;
-        // the pieces of the second column box store their halves in the other order: no bank is hit twice
-        const bool swap = piece >= 4;
-        *reinterpret_cast<uint4*>(row + ((c + (swap ? 1 : 0)) ^ sw) * 16) = swap ? hi : lo;
-        *reinterpret_cast<uint4*>(row + ((c + (swap ? 0 : 1)) ^ sw) * 16) = swap ? lo : hi;
       }
-      if (threadIdx.x < 4) s_scale[st * 16 + kv * 8 + half * 4 + threadIdx.x] = scale[slot];
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        uint4 lo, hi;
+        Kv<FMT>::decode4(r[i].x, lo.x, lo.y);
+        Kv<FMT>::decode4(r[i].y, lo.z, lo.w);
+        Kv<FMT>::decode4(r[i].z, hi.x, hi.y);
+        Kv<FMT>::decode4(r[i].w, hi.z, hi.w);
+        *reinterpret_cast<uint4*>(dst + put0 + i * KPP * 128) = swap ? hi : lo;
+        *reinterpret_cast<uint4*>(dst + put1 + i * KPP * 128) = swap ? lo : hi;
+      }
     };
     auto arrive = [&](uint64_t* bar) {
       fence_async_smem();
@@ -287,10 +315,12 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
     };
     using K_ = std::integral_constant<int, 0>;
     using V_ = std::integral_constant<int, 1>;
-    if (nk > 0) {
-      fetch(K_{}, 0, 0, 0);
-      fetch(K_{}, 1, 0, 1);
-    }
+    Groups now = groups_of(0, id_of(0)), next = groups_of(1, id_of(1));
+    int id = id_of(2);
+    fetch(K_{}, 0, now);
+    fetch(K_{}, 1, now);
+    fetch(V_{}, 0, now);
+    fetch(V_{}, 1, now);
     for (int j = 0; j < nk; ++j) {
       const int st = j % kStages;
       const bool ok = mbar_sleep_wait(&kv_empty[st], ((j / kStages) & 1) ^ 1, kTimeoutEmpty);
@@ -298,17 +328,25 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
         *abort_flag = 1;
         break;
       }
-      store(K_{}, 0, j, 0);
-      fetch(V_{}, 0, j, 0);
-      store(K_{}, 1, j, 1);
+      if (warp == 0 && lane < 8) {
+        s_scale[st * 16 + lane] = now.scale[0];
+        s_scale[st * 16 + 8 + lane] = __log2f(now.scale[1]);
+      }
+      store(K_{}, 0, j);
+      fetch(K_{}, 0, next);
+      store(K_{}, 1, j);
+      fetch(K_{}, 1, next);
       arrive(&k_full[st]);
-      fetch(V_{}, 1, j, 1);
-      store(V_{}, 0, j, 0);
-      if (j + 1 < nk) fetch(K_{}, 0, j + 1, 0);
-      store(V_{}, 1, j, 1);
+      store(V_{}, 0, j);
+      fetch(V_{}, 0, next);
+      store(V_{}, 1, j);
+      fetch(V_{}, 1, next);
       arrive(&v_full[st]);
-      if (j + 1 < nk) fetch(K_{}, 1, j + 1, 1);
+      now = next;
+      next = groups_of(j + 2, id);
+      id = id_of(j + 3);
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == 12) {
     // ------------------------------------------------------------------ MMA issuer
     if (lane == 0) {
@@ -436,69 +474,74 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
     }
     const int lim = lim_of(r);
     const int lim_group = lim_of(g * kGroupRows);  // the group's first row sees the fewest keys
-    float m_run = -INFINITY, l_run = 0.f, v_ref = 0.f, v_up = 0.f;
+    // running maximum, sum, and log2 of the largest value scale that the row has seen
+    float m_run = kNone, l_run = 0.f, v_ref = -INFINITY;
     bool ok = true;
     for (int j = 0; j < n_g; ++j) {
       const int st = j % kStages;
       if (__any_sync(0xffffffffu, *abort_flag != 0)) { ok = false; break; }
-      if (!__all_sync(0xffffffffu, mbar_sleep_wait(&s_full[g], j & 1, kTimeoutAccum))) { ok = false; break; }
-      // the tile's scales: written before k_full and v_full completed
+      // the scales are written before k_full completes; S_g comes after it
       if (!__all_sync(0xffffffffu, mbar_sleep_wait(&k_full[st], (j / kStages) & 1, kTimeoutFull) &&
-                                       mbar_sleep_wait(&v_full[st], (j / kStages) & 1, kTimeoutFull))) { ok = false; break; }
+                                       mbar_sleep_wait(&s_full[g], j & 1, kTimeoutAccum))) { ok = false; break; }
       tc_fence_after();
       const int k0 = (t0 + j) * KT;
-      const float* sc = s_scale + st * 16;
-      float ks[8], vs[8];
+      const int lim_tile = lim - k0;
+      const float* sc = s_scale + st * 16;  // [8] key scales, [8] log2 of value scales
+      bool plain = k0 + KT <= lim_group;    // the same for the whole warp: all rows see all 128 keys
+      float v_top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 8; i += 4) {
         const float4 a = *reinterpret_cast<const float4*>(sc + i), c = *reinterpret_cast<const float4*>(sc + 8 + i);
-        ks[i] = a.x; ks[i + 1] = a.y; ks[i + 2] = a.z; ks[i + 3] = a.w;
-        vs[i] = c.x; vs[i + 1] = c.y; vs[i + 2] = c.z; vs[i + 3] = c.w;
+        plain = plain && fminf(fminf(a.x, a.y), fminf(a.z, a.w)) >= 0.f;
+        v_top = fmaxf(fmax3(v_top, c.x, c.y), fmaxf(c.z, c.w));
       }
-      const int lim_tile = lim - k0;
-      bool plain = k0 + KT <= lim_group;  // uniform over the warp: all 128 keys are seen by all rows
-#pragma unroll
-      for (int i = 0; i < 8; ++i) plain = plain && ks[i] >= 0.f;
-      float v_top = 0.f;  // the largest value scale that this row sees
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v_top = fmaxf(v_top, plain || i * 16 < lim_tile ? vs[i] : 0.f);
-      // scores of 32 columns, scaled, masked ones at -inf
-      auto scores = [&](int c, float* v) {
-        tmem_ld32(ts + c, v);
-        const float f0 = unit * ks[c / 16], f1 = unit * ks[c / 16 + 1];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] *= i < 16 ? f0 : f1;
-        if (!plain) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (c + i >= lim_tile || ks[c / 16 + i / 16] < 0.f) v[i] = -INFINITY;
-        }
-      };
+      // ---- the row's maximum
       float mx = -INFINITY;
+      if (plain) {
 #pragma unroll
-      for (int c = 0; c < KT; c += 32) {
-        float v[32];
-        scores(c, v);
+        for (int c = 0; c < KT; c += 64) {
+          float v[64];
+          tmem_ld32_pair(ts + c, ts + c + 32, v, v + 32);
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) mx = fmax3(mx, v[i], v[i + 1]);
+          for (int i = 0; i < 64; i += 16) {
+            float a = fmax3(v[i], v[i + 1], v[i + 2]), d = fmax3(v[i + 3], v[i + 4], v[i + 5]);
+            a = fmax3(a, v[i + 6], v[i + 7]);
+            d = fmax3(d, v[i + 8], v[i + 9]);
+            a = fmax3(a, v[i + 10], v[i + 11]);
+            d = fmax3(d, v[i + 12], v[i + 13]);
+            mx = fmaxf(mx, fmaxf(fmax3(a, v[i + 14], v[i + 15]), d) * sc[(c + i) / 16]);
+          }
+        }
+      } else {
+        v_top = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < KT; c += 16) {
+          float v[16];
+          tmem_ld16(ts + c, v);
+          const float f = sc[c / 16];
+          if (f >= 0.f && c < lim_tile) v_top = fmaxf(v_top, sc[8 + c / 16]);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, f >= 0.f && c + i < lim_tile ? v[i] * f : -INFINITY);
+        }
       }
+      mx *= unit;
       float factor = 1.f;
       bool rescale = false;
       if (__any_sync(0xffffffffu, mx > m_run + kLazy || v_top > v_ref)) {
         const float m_new = fmaxf(m_run, mx), v_new = fmaxf(v_ref, v_top);
-        const float f = m_run == -INFINITY ? 0.f : exp2f_approx(m_run - m_new);
-        factor = f * (v_ref > 0.f ? v_ref / v_new : 0.f);
+        const float f = exp2f_approx(m_run - m_new);
+        factor = v_ref == -INFINITY ? 0.f : f * exp2f_approx(v_ref - v_new);
         l_run *= f;
         m_run = m_new;
         v_ref = v_new;
-        v_up = v_new > 0.f ? kWeightUp / v_new : 0.f;
         rescale = j > 0;
       }
-      // O_g += P_g V of the tile before has to be complete before P_g (head_dim 64) or O_g is written
+      // O_g += P_g V of the tile before has to be complete before P_g (head_dim 64) or O_g is written; its values are in
+      // shared memory before P_g is handed on (v_full is the issuer's to wait for)
       if (j > 0 && !__all_sync(0xffffffffu, mbar_sleep_wait(&o_full[g], (j - 1) & 1, kTimeoutAccum))) { ok = false; break; }
       tc_fence_after();
       if (rescale) {
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           float o[32];
           tmem_ld32(to + c, o);
@@ -507,24 +550,54 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
           tmem_st32(to + c, o);
         }
       }
-      const float m = m_run == -INFINITY ? 0.f : m_run;
-      float2 sum = make_float2(0.f, 0.f);
+      // ---- weights. A group's value scale goes into the exponent (at most 2^8 up, and not below 2^-60, where an f16 weight
+      // is zero and the sum would lose it), so that the sum takes it out again once per 16 keys.
+      const float neg_m = -m_run, v_off = kWeightUpLog2 - v_ref;
+      if (plain) {
 #pragma unroll
-      for (int c = 0; c < KT; c += 32) {
-        float v[32];
-        scores(c, v);
-        uint32_t w[16];
-        const float u0 = v_up * vs[c / 16], u1 = v_up * vs[c / 16 + 1];
+        for (int c = 0; c < KT; c += 32) {
+          float v[32];
+          uint32_t w[16];
+          tmem_ld32(ts + c, v);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float2 e = make_float2(exp2f_approx(v[2 * i] - m), exp2f_approx(v[2 * i + 1] - m));
-          sum = add_f32x2(sum, e);
-          const float u = i < 8 ? u0 : u1;
-          w[i] = pack_f16(e.x * u, e.y * u);
+          for (int i = 0; i < 32; i += 16) {
+            const float f = unit * sc[(c + i) / 16], up = fmaxf(sc[8 + (c + i) / 16] + v_off, -60.f);
+            const float2 f2 = make_float2(f, f), off = make_float2(neg_m + up, neg_m + up);
+            float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int k = i; k < i + 16; k += 2) {
+              const float2 x = fma_f32x2(make_float2(v[k], v[k + 1]), f2, off);
+              const float2 e = make_float2(exp2f_approx(x.x), exp2f_approx(x.y));
+              sum = add_f32x2(sum, e);
+              w[k / 2] = pack_f16(e.x, e.y);
+            }
+            l_run = fmaf(sum.x + sum.y, exp2f_approx(-up), l_run);
+          }
+          tmem_st16u(tp + c / 2, w);
         }
-        tmem_st16u(tp + c / 2, w);
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < KT; c += 32) {
+          float v[32];
+          uint32_t w[16];
+          tmem_ld32(ts + c, v);
+#pragma unroll
+          for (int i = 0; i < 32; i += 16) {
+            const float ks = sc[(c + i) / 16], up = fmaxf(sc[8 + (c + i) / 16] + v_off, -60.f);
+            const float f = unit * ks;
+            float sum = 0.f;
+#pragma unroll
+            for (int k = i; k < i + 16; k += 2) {
+              const float e0 = ks >= 0.f && c + k < lim_tile ? exp2f_approx(fmaf(v[k], f, neg_m + up)) : 0.f;
+              const float e1 = ks >= 0.f && c + k + 1 < lim_tile ? exp2f_approx(fmaf(v[k + 1], f, neg_m + up)) : 0.f;
+              sum += e0 + e1;
+              w[k / 2] = pack_f16(e0, e1);
+            }
+            l_run = fmaf(sum, exp2f_approx(-up), l_run);
+          }
+          tmem_st16u(tp + c / 2, w);
+        }
       }
-      l_run += sum.x + sum.y;
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -539,8 +612,8 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
     } else {
       tc_fence_after();
       const bool part = args.splits > 1;
-      const float up = v_ref * (1.f / kWeightUp);
-      const float inv = part ? up : (m_run == -INFINITY ? 0.f : up / l_run);  // a row that sees no key is zero
+      const float up = exp2f_approx(v_ref - kWeightUpLog2);
+      const float inv = part ? up : (m_run == kNone ? 0.f : up / l_run);  // a row that sees no key is zero
       const int64_t slot = ((static_cast<int64_t>(s_item[2]) - 1 - blockIdx.x / p.Hkv) * p.Hkv + h) * args.splits + blockIdx.y;
       bf16* out = p.out + static_cast<int64_t>(tok) * p.o_token + head * p.o_head;
       float* part_o = p.part_o + (slot * kRows + r) * D;
@@ -601,7 +674,7 @@ __global__ void __launch_bounds__(128) cached_attn_tc_join_kernel(CachedAttn p, 
   if (tok < fresh.first || tok >= fresh.first + fresh.n) return;  // zeroed by the attention kernel
   const int r = (tok - fresh.first) * p.group + hq % p.group;
   const int64_t slot0 = ((p.prefix[lo] + r / kRows) * p.Hkv + hq / p.group) * splits;
-  float m = -INFINITY;
+  float m = kNone;
   for (int s = lane; s < splits; s += 32) m = fmaxf(m, p.part_ml[((slot0 + s) * kRows + r % kRows) * 2]);
   m = warp_max(m);
   constexpr int PER = D / 32;
@@ -612,7 +685,7 @@ __global__ void __launch_bounds__(128) cached_attn_tc_join_kernel(CachedAttn p, 
   for (int s = 0; s < splits; ++s) {
     const int64_t at = (slot0 + s) * kRows + r % kRows;
     const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
-    const float f = ml.x == -INFINITY ? 0.f : exp2f_approx(ml.x - m);
+    const float f = exp2f_approx(ml.x - m);
     l += ml.y * f;
 #pragma unroll
     for (int e = 0; e < PER; ++e) acc[e] += p.part_o[at * D + lane * PER + e] * f;
