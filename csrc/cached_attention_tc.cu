@@ -18,11 +18,12 @@
 // TMEM (512 columns): S_0, S_1 at 0 and 128, O_0, O_1 at 256 (D columns each). head_dim 64 has room for P_0, P_1 at 384 and
 // 448; head_dim 128 has none, so P_g takes the first 64 columns of S_g, and the next S_g is issued only once P_g V has
 // completed. A softmax thread reads its row twice (maximum, then exponentials, 32 columns at a time), so that it needs no
-// 128 registers for it: 13 warps with 152 registers each fit the SM.
+// 128 registers for it: 14 warps with 128 registers each fit the SM.
 //
-// Warps: 0-3 widen, 4-7 softmax of group 0, 8-11 of group 1, 12 issues the MMAs. Every wait is bounded (common.cuh); on a
+// Warps: 0-3 widen, 4-7 softmax of group 0, 8-11 of group 1, 12 and 13 issue the groups' MMAs. Every wait is bounded (common.cuh); on a
 // timeout all roles stop, MMAs in flight are waited for, TMEM is freed and the status word records the cause.
 #include <algorithm>
+#include <type_traits>
 
 #include "cached_attention.cuh"
 #include "common.cuh"
@@ -36,7 +37,7 @@ namespace {
 constexpr int KT = 128;        // keys of a tile
 constexpr int kGroupRows = 128;
 constexpr int kRows = kPromptRows;  // rows of a block of threads
-constexpr int kThreads = 13 * 32;
+constexpr int kThreads = 14 * 32;
 constexpr int kTmemCols = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNone = -3e38f;       // running maximum of a row that has seen no key
@@ -104,11 +105,10 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
   uint64_t* v_full = k_full + kStages;
   uint64_t* kv_empty = v_full + kStages;
   uint64_t* s_full = kv_empty + kStages;  // [2] S_g of the next tile is in TMEM
-  uint64_t* s_free = s_full + 2;          // [2] S_g has been read (head_dim 64)
-  uint64_t* p_full = s_free + 2;          // [2] P_g is written, O_g rescaled if it had to be
-  uint64_t* o_full = p_full + 2;          // [2] O_g += P_g V has completed
+  uint64_t* p_full = s_full + 2;          // [2][2] a half of P_g is written (O_g rescaled if it had to be)
+  uint64_t* o_full = p_full + 4;          // [2] O_g += P_g V has completed
   uint64_t* teardown = o_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(teardown + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(teardown + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_item = reinterpret_cast<int*>(tmem_slot + 2);  // request, row tile, number of tiles
 
@@ -157,15 +157,16 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&k_full[s], 4);
       mbar_init(&v_full[s], 4);
-      mbar_init(&kv_empty[s], 1);
+      mbar_init(&kv_empty[s], 2);
     }
     for (int g = 0; g < 2; ++g) {
       mbar_init(&s_full[g], 1);
-      mbar_init(&s_free[g], 4);
-      mbar_init(&p_full[g], 4);
+      mbar_init(&p_full[2 * g], 4);
+      mbar_init(&p_full[2 * g + 1], 4);
       mbar_init(&o_full[g], 1);
     }
-    mbar_init(teardown, 1);
+    mbar_init(&teardown[0], 1);
+    mbar_init(&teardown[1], 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -216,19 +217,18 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
 
   if (warp < 4) {
     // ------------------------------------------------------------------ codes -> f16 tiles in shared memory
-    constexpr int CPK = D / 16;          // 16-byte pieces of a key
-    constexpr int KPP = 128 / CPK;       // keys that the 128 threads cover at a time
-    constexpr int NP = 64 / KPP;         // pieces per thread of a half tile (64 keys)
-    const int piece = threadIdx.x % CPK, key_in = threadIdx.x / CPK;
+    // A thread widens one 16-byte piece of every KPP-th key. Four lanes hold a key's pieces of one 64-column box and the next
+    // four the next key's: their f16 halves, swizzled, fall on different banks.
+    constexpr int KPP = 128 / (D / 16);
+    constexpr int NP = 64 / KPP;         // keys per thread of a half tile (64 keys)
+    const int key_in = (threadIdx.x / 4) % KPP, box = threadIdx.x / (4 * KPP);
+    const int piece = box * 4 + threadIdx.x % 4;
     const int* table = p.table + static_cast<int64_t>(b) * p.table_stride;
     // the thread's byte in a 16-key group, and its places in a tile (they repeat every 8 keys)
     const uint8_t* base[2] = {p.k.codes + static_cast<int64_t>(h) * p.k.head_stride + (key_in % 16) * p.k.token_stride + piece * 16,
                               p.v.codes + static_cast<int64_t>(h) * p.v.head_stride + (key_in % 16) * p.v.token_stride + piece * 16};
-    const int sw = key_in & 7, c0 = (piece % 4) * 2;
-    // the pieces of the second column box store their halves in the other order: no bank is hit twice
-    const bool swap = piece >= 4;
-    const int put0 = (piece / 4) * (KT * 128) + key_in * 128 + ((c0 + (swap ? 1 : 0)) ^ sw) * 16;
-    const int put1 = (piece / 4) * (KT * 128) + key_in * 128 + ((c0 + (swap ? 0 : 1)) ^ sw) * 16;
+    const int put = box * (KT * 128) + key_in * 128;
+    const int put0 = put + (((piece % 4) * 2) ^ (key_in & 7)) * 16, put1 = put + (((piece % 4) * 2 + 1) ^ (key_in & 7)) * 16;
     // Lanes 0-7 look up the tile's 16-key groups: where the keys and values begin (-1: masked, without a block or past the
     // last key that a row sees) and their scales. The block's id is read three tiles ahead and used two ahead, so that no
     // thread waits for the dependent reads.
@@ -304,8 +304,8 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
         Kv<FMT>::decode4(r[i].y, lo.z, lo.w);
         Kv<FMT>::decode4(r[i].z, hi.x, hi.y);
         Kv<FMT>::decode4(r[i].w, hi.z, hi.w);
-        *reinterpret_cast<uint4*>(dst + put0 + i * KPP * 128) = swap ? hi : lo;
-        *reinterpret_cast<uint4*>(dst + put1 + i * KPP * 128) = swap ? lo : hi;
+        *reinterpret_cast<uint4*>(dst + put0 + i * KPP * 128) = lo;
+        *reinterpret_cast<uint4*>(dst + put1 + i * KPP * 128) = hi;
       }
     };
     auto arrive = [&](uint64_t* bar) {
@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
     for (int j = 0; j < nk; ++j) {
       const int st = j % kStages;
       const bool ok = mbar_sleep_wait(&kv_empty[st], ((j / kStages) & 1) ^ 1, kTimeoutEmpty);
-      if (!__all_sync(0xffffffffu, ok && *abort_flag == 0)) {
+      if (!__all_sync(0xffffffffu, ok)) {
         *abort_flag = 1;
         break;
       }
@@ -347,80 +347,67 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
       id = id_of(j + 3);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-  } else if (warp == 12) {
-    // ------------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t id_s = idesc_f16(KT, false);
-      constexpr uint32_t id_o = idesc_f16(D, true);
-      int ns[2] = {0, 0};  // next S to issue, per group
-      int no[2] = {0, 0};  // next P V to issue
-      int released = 0;
-      const uint64_t dq0 = smem_desc_sw128(smem_u32(smem), 16, 1024);
-      const uint64_t dk0 = smem_desc_sw128(smem_u32(smem + L::kKV), 16, 1024);
-      const uint64_t dv0 = smem_desc_sw128(smem_u32(smem + L::kKV + L::kTileBytes), KT * 128, 1024);
-      auto issue_s = [&](int g, int j) {
-        const uint64_t dq = dq0 + static_cast<uint32_t>(g * (L::kQBytes >> 4));
-        const uint64_t dk = dk0 + static_cast<uint32_t>((j % kStages) * ((2 * L::kTileBytes) >> 4));
-        tc_fence_after();
+  } else if (warp >= 12) {
+    // ------------------------------------------------------------------ MMA issuers, one warp per group
+    // The whole warp runs this, converged (umma_f16_warp); one lane issues. A warp of its own for each group waits for
+    // exactly the next thing that the group needs; one that polled for both took 500 cycles to notice.
+    constexpr uint32_t kAll = 0xffffffffu;
+    constexpr uint32_t id_s = idesc_f16(KT, false);
+    constexpr uint32_t id_o = idesc_f16(D, true);
+    const uint32_t elect = elect_one();
+    const int g = __shfl_sync(kAll, warp, 0) - 12;
+    const int count = __shfl_sync(kAll, g == 0 ? n0 : n1, 0), all = __shfl_sync(kAll, nk, 0);
+    const uint32_t acc = __shfl_sync(kAll, tmem, 0);
+    const uint32_t t_s = acc + g * KT, t_o = acc + L::kTmemO + g * D, t_p = acc + L::tmem_p(g);
+    const uint64_t dq = smem_desc_sw128(smem_u32(smem) + g * L::kQBytes, 16, 1024);
+    const uint64_t dk0 = smem_desc_sw128(smem_u32(smem + L::kKV), 16, 1024);
+    const uint64_t dv0 = smem_desc_sw128(smem_u32(smem + L::kKV + L::kTileBytes), KT * 128, 1024);
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, int phase, int code) {
+      ok = ok && __all_sync(kAll, mbar_wait(bar, phase & 1, code)) != 0;
+      return ok;
+    };
+    auto issue_s = [&](int j) {
+      const uint64_t dk = dk0 + static_cast<uint32_t>((j % kStages) * ((2 * L::kTileBytes) >> 4));
+      tc_fence_after();
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          umma_bf16(tmem + g * KT, dq + (((k / 4) * (kGroupRows * 128) + (k % 4) * 32) >> 4),
-                    dk + (((k / 4) * (KT * 128) + (k % 4) * 32) >> 4), id_s, k > 0 ? 1u : 0u);
-        umma_commit(&s_full[g]);
-      };
-      auto issue_o = [&](int g, int j) {
-        const uint64_t dv = dv0 + static_cast<uint32_t>((j % kStages) * ((2 * L::kTileBytes) >> 4));
-        const uint32_t a0 = tmem + L::tmem_p(g);
-        const uint32_t d = tmem + L::kTmemO + g * D;
-        tc_fence_after();
+      for (int k = 0; k < D / 16; ++k)
+        umma_f16_warp(t_s, dq + (((k / 4) * (kGroupRows * 128) + (k % 4) * 32) >> 4),
+                      dk + (((k / 4) * (KT * 128) + (k % 4) * 32) >> 4), id_s, k > 0 ? 1u : 0u, elect);
+      umma_commit_warp(&s_full[g], elect);
+    };
+    auto issue_o = [&](int j, int half) {
+      const uint64_t dv = dv0 + static_cast<uint32_t>((j % kStages) * ((2 * L::kTileBytes) >> 4) + half * ((4 * 2048) >> 4));
+      tc_fence_after();
 #pragma unroll
-        for (int k = 0; k < KT / 16; ++k)
-          umma_bf16_ts(d, a0 + k * 8, dv + ((k * 2048) >> 4), id_o, k > 0 || j > 0 ? 1u : 0u);
-        umma_commit(&o_full[g]);
-      };
-      bool ok = mbar_sleep_wait(q_full, 0, kTimeoutFull);
-      int idle = 0;
-      uint64_t idle_start = 0;
-      auto step = [&](int g, int n_g) -> bool {
-        bool moved = false;
-        if (no[g] < ns[g] && mbar_test(&p_full[g], no[g] & 1) && mbar_test(&v_full[no[g] % kStages], (no[g] / kStages) & 1)) {
-          issue_o(g, no[g]++);
-          moved = true;
-        }
-        if (ns[g] < n_g && mbar_test(&k_full[ns[g] % kStages], (ns[g] / kStages) & 1)) {
-          bool free = ns[g] == 0;
-          if (!free) free = L::kAlias ? no[g] == ns[g] && mbar_test(&o_full[g], (ns[g] - 1) & 1)
-                                      : mbar_test(&s_free[g], (ns[g] - 1) & 1);
-          if (free) {
-            issue_s(g, ns[g]++);
-            moved = true;
-          }
-        }
-        return moved;
-      };
-      while (ok && (no[0] < n0 || no[1] < n1)) {
-        bool progress = step(0, n0);
-        progress = step(1, n1) || progress;
-        while (released < nk && (released >= n0 || no[0] > released) && (released >= n1 || no[1] > released)) {
-          umma_commit(&kv_empty[released % kStages]);
-          ++released;
-          progress = true;
-        }
-        if (progress) {
-          idle = 0;
-          continue;
-        }
-        if ((++idle & 1023) == 0) {
-          if (*abort_flag) { ok = false; break; }
-          const uint64_t now = globaltimer();
-          if (idle == 1024) idle_start = now;
-          else if (now - idle_start > QW_WAIT_TIMEOUT_NS) { set_status(kTimeoutAccum); ok = false; break; }
-        }
+      for (int k = 0; k < KT / 32; ++k)
+        umma_f16_ts_warp(t_o, t_p + half * 32 + k * 8, dv + ((k * 2048) >> 4), id_o, k > 0 || half > 0 || j > 0 ? 1u : 0u,
+                         elect);
+    };
+    if (count > 0 && wait(q_full, 0, kTimeoutFull) && wait(&k_full[0], 0, kTimeoutFull)) issue_s(0);
+    for (int j = 0; ok && j < count; ++j) {
+      const bool more = j + 1 < count;
+      if (!wait(&v_full[j % kStages], j / kStages, kTimeoutFull) || !wait(&p_full[2 * g], j, kTimeoutAccum)) break;
+      issue_o(j, 0);
+      if (more && !wait(&k_full[(j + 1) % kStages], (j + 1) / kStages, kTimeoutFull)) break;
+      if (!wait(&p_full[2 * g + 1], j, kTimeoutAccum)) break;
+      if (!L::kAlias && more) issue_s(j + 1);  // S_g has been read when all weights are written
+      issue_o(j, 1);
+      umma_commit_warp(&o_full[g], elect);
+      umma_commit_warp(&kv_empty[j % kStages], elect);
+      if (L::kAlias && more) {
+        if (!wait(&o_full[g], j, kTimeoutAccum)) break;
+        issue_s(j + 1);
       }
-      if (!ok) *abort_flag = 1;
-      umma_commit(teardown);  // fires once every MMA issued above has completed
-      mbar_sleep_wait(teardown, 0, kTimeoutAccum);
     }
+    if (!ok) *abort_flag = 1;
+    for (int j = count; ok && j < all; ++j) {  // tiles that only the other group needs
+      if (!wait(&v_full[j % kStages], j / kStages, kTimeoutFull)) break;
+      if (elect) mbar_arrive(&kv_empty[j % kStages]);
+    }
+    umma_commit_warp(&teardown[g], elect);  // fires once every MMA issued above has completed
+    mbar_wait(&teardown[g], 0, kTimeoutAccum);
+    __syncwarp();
   } else {
     // ------------------------------------------------------------------ softmax
     const int g = (warp - 4) / 4;
@@ -479,7 +466,6 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
     bool ok = true;
     for (int j = 0; j < n_g; ++j) {
       const int st = j % kStages;
-      if (__any_sync(0xffffffffu, *abort_flag != 0)) { ok = false; break; }
       // the scales are written before k_full completes; S_g comes after it
       if (!__all_sync(0xffffffffu, mbar_sleep_wait(&k_full[st], (j / kStages) & 1, kTimeoutFull) &&
                                        mbar_sleep_wait(&s_full[g], j & 1, kTimeoutAccum))) { ok = false; break; }
@@ -552,28 +538,38 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
       }
       // ---- weights. A group's value scale goes into the exponent (at most 2^8 up, and not below 2^-60, where an f16 weight
       // is zero and the sum would lose it), so that the sum takes it out again once per 16 keys.
+      auto hand_on = [&](int half) {  // the first 64 keys' weights are used while the others are made
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[2 * g + half]);
+      };
       const float neg_m = -m_run, v_off = kWeightUpLog2 - v_ref;
       if (plain) {
 #pragma unroll
-        for (int c = 0; c < KT; c += 32) {
-          float v[32];
-          uint32_t w[16];
-          tmem_ld32(ts + c, v);
+        for (int c = 0; c < KT; c += 64) {
+          float v[64];
+          tmem_ld32_pair(ts + c, ts + c + 32, v, v + 32);
 #pragma unroll
-          for (int i = 0; i < 32; i += 16) {
-            const float f = unit * sc[(c + i) / 16], up = fmaxf(sc[8 + (c + i) / 16] + v_off, -60.f);
-            const float2 f2 = make_float2(f, f), off = make_float2(neg_m + up, neg_m + up);
-            float2 sum = make_float2(0.f, 0.f);
+          for (int q = 0; q < 64; q += 32) {
+            uint32_t w[16];
 #pragma unroll
-            for (int k = i; k < i + 16; k += 2) {
-              const float2 x = fma_f32x2(make_float2(v[k], v[k + 1]), f2, off);
-              const float2 e = make_float2(exp2f_approx(x.x), exp2f_approx(x.y));
-              sum = add_f32x2(sum, e);
-              w[k / 2] = pack_f16(e.x, e.y);
+            for (int i = q; i < q + 32; i += 16) {
+              const float f = unit * sc[(c + i) / 16], up = fmaxf(sc[8 + (c + i) / 16] + v_off, -60.f);
+              const float2 f2 = make_float2(f, f), off = make_float2(neg_m + up, neg_m + up);
+              float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+              for (int k = i; k < i + 16; k += 2) {
+                const float2 x = fma_f32x2(make_float2(v[k], v[k + 1]), f2, off);
+                const float2 e = make_float2(exp2f_approx(x.x), exp2f_approx(x.y));
+                sum = k == i ? e : add_f32x2(sum, e);
+                w[(k - q) / 2] = pack_f16(e.x, e.y);
+              }
+              l_run = fmaf(sum.x + sum.y, exp2f_approx(-up), l_run);
             }
-            l_run = fmaf(sum.x + sum.y, exp2f_approx(-up), l_run);
+            tmem_st16u(tp + (c + q) / 2, w);
           }
-          tmem_st16u(tp + c / 2, w);
+          hand_on(c / 64);
         }
       } else {
 #pragma unroll 1
@@ -596,14 +592,8 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
             l_run = fmaf(sum, exp2f_approx(-up), l_run);
           }
           tmem_st16u(tp + c / 2, w);
+          if (c % 64 == 32) hand_on(c / 64);
         }
-      }
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (!L::kAlias) mbar_arrive(&s_free[g]);
-        mbar_arrive(&p_full[g]);
       }
     }
     if (ok && n_g > 0 && !__all_sync(0xffffffffu, mbar_sleep_wait(&o_full[g], (n_g - 1) & 1, kTimeoutAccum))) ok = false;
