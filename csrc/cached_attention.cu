@@ -727,11 +727,11 @@ Way way_of(int T, int B, int Hq, int Hkv, int D, int max_query, int max_context)
   w.tile = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 24 ? 24 : 32;
   int64_t slots;
   if (w.prompt) {
-    w.tiles_max = static_cast<int>(static_cast<int64_t>(T) * group / kPromptRows + B);
+    w.tiles_max = static_cast<int>(static_cast<int64_t>(T) * group / prompt_rows(D) + B);
     // too few row tiles for the SMs: split the keys, two tiles of 128 at least for each part
     const int64_t blocks = static_cast<int64_t>(w.tiles_max) * Hkv;
-    w.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(148 / std::max<int64_t>(blocks, 1), max_context / 256)));
-    slots = w.splits > 1 ? blocks * w.splits * kPromptRows : 0;
+    w.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(148 * prompt_per_sm(D) / std::max<int64_t>(blocks, 1), max_context / 256)));
+    slots = w.splits > 1 ? blocks * w.splits * prompt_rows(D) : 0;
   } else {
     slots = 2 * static_cast<int64_t>(workers_of(D, w.tile)) * w.tile;
   }

@@ -41,8 +41,9 @@ __device__ __forceinline__ NewRows new_rows(const CachedAttn& p, int b) {
   return {first, min(p.query_start[b + 1], p.T) - first};
 }
 
-// tcgen05 kernel for prompts (head_dim 64 and 128): 256 rows per block of threads, `splits` parts of the keys
-constexpr int kPromptRows = 256;
+// tcgen05 kernel for prompts (head_dim 64 and 128), `splits` parts of the keys; rows and resident blocks of threads per SM
+constexpr int prompt_rows(int D) { return D == 64 ? 128 : 256; }
+constexpr int prompt_per_sm(int D) { return D == 64 ? 2 : 1; }
 void cached_attention_prompt(const CachedAttn& p, int D, int fmt, int tiles_max, int splits, cudaStream_t stream);
 
 }  // namespace qw

@@ -16,8 +16,8 @@
 // their argument costs 2^-8 relative at arguments of 8.
 //
 // TMEM (512 columns): S_0, S_1 at 0 and 128, O_0, O_1 at 256 (D columns each). head_dim 64 has room for P_0, P_1 at 384 and
-// 448; head_dim 128 has none, so P_g takes the first 64 columns of S_g, and the next S_g is issued only once P_g V has
-// completed. A softmax thread reads its row twice (maximum, then exponentials, 32 columns at a time), so that it needs no
+// 448; head_dim 128 has none, so P_g lies in S_g (each half of the weights in the columns of its own keys), and the next S_g
+// is issued only once P_g V has completed. A softmax thread reads its row twice (maximum, then exponentials, 32 columns at a time), so that it needs no
 // 128 registers for it: 14 warps with 128 registers each fit the SM.
 //
 // Warps: 0-3 widen, 4-7 softmax of group 0, 8-11 of group 1, 12 and 13 issue the groups' MMAs. Every wait is bounded (common.cuh); on a
@@ -36,9 +36,6 @@ namespace {
 
 constexpr int KT = 128;        // keys of a tile
 constexpr int kGroupRows = 128;
-constexpr int kRows = kPromptRows;  // rows of a block of threads
-constexpr int kThreads = 14 * 32;
-constexpr int kTmemCols = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNone = -3e38f;       // running maximum of a row that has seen no key
 constexpr float kLazy = 6.f;          // the running maximum moves when a row grows by more than 2^6
@@ -46,20 +43,30 @@ constexpr float kWeightUpLog2 = 8.f;  // weights in f16: at most 2^14
 
 template <int D>
 struct Layout {
-  static constexpr bool kAlias = D == 128;                  // P_g in S_g's columns
-  static constexpr int kStages = D == 64 ? 4 : 2;  // all that fits
+  static constexpr int kGroups = D == 64 ? 1 : 2;
+  static constexpr int kRows = kGroups * kGroupRows;         // rows of a block of threads
+  static constexpr int kIssuer = 4 + 8 * kGroups;            // first of the issuing warps
+  static constexpr int kThreads = (kIssuer + kGroups) * 32;
+  static constexpr bool kAlias = D == 128;                   // P_g in S_g's columns
+  static constexpr int kStages = 2;
   static constexpr int kBoxes = D / 64;                      // 64-wide (128-byte) column boxes
   static constexpr int kQBytes = kBoxes * kGroupRows * 128;  // one group's rows
   static constexpr int kTileBytes = kBoxes * KT * 128;       // one K or V tile
-  static constexpr int kKV = 2 * kQBytes;                    // stages of [K | V]
+  static constexpr int kKV = kGroups * kQBytes;              // stages of [K | V]
   static constexpr int kScale = kKV + kStages * 2 * kTileBytes;  // stages of k_scale[8], v_scale[8]
   static constexpr int kRaw = kScale + kStages * 64;         // codes of one K and one V tile on their way
   static constexpr int kPoison = kRaw + 2 * KT * D;
-  static constexpr int kBar = kPoison + D * 4;
-  static constexpr int kTotal = kBar + 512 + 1024;           // barriers, and slack to align the base to 1 KB
-  static constexpr int kTmemO = 256;
-  static constexpr int tmem_p(int g) { return kAlias ? g * 128 : 384 + g * 64; }
-  static_assert(kTotal <= 227 * 1024, "shared memory per block");
+  static constexpr int kJoin = kPoison + D * 4;              // [groups][2 halves][128 rows]: maxima, at the end sums
+  static constexpr int kBar = kJoin + kGroups * 1024;
+  static constexpr int kBarriers = 21 + 3 * kStages;         // at most (see the pointers in the kernel)
+  static constexpr int kTotal = kBar + kBarriers * 8 + 24;   // and six words
+  static constexpr int kTmemO = kGroups * KT;
+  static constexpr int kTmemP = kAlias ? 0 : kTmemO + kGroups * D;  // 128 columns apart where P_g lies in S_g
+  static constexpr int kTmemCols = kGroups * 256;
+  static constexpr int kPHalf = kAlias ? 64 : 32;            // columns from the first 64 keys' weights to the others'
+  static_assert(kTotal <= (kGroups == 1 ? 113 : 227) * 1024, "shared memory per block");
+  static_assert(kRows == prompt_rows(D) && prompt_per_sm(D) == 3 - kGroups, "what the host counts on");
+  static_assert(kAlias || kTmemP + kGroups * KT / 2 <= kTmemCols, "tensor memory");
 };
 
 // Instruction descriptor, kind::f16 with f16 operands and fp32 accumulators.
@@ -92,27 +99,38 @@ struct TcArgs {
 };
 
 template <int FMT, int D>
-__global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __grid_constant__ TcArgs args) {
+__global__ void __launch_bounds__(Layout<D>::kThreads, 3 - Layout<D>::kGroups) cached_attn_tc_kernel(const __grid_constant__ TcArgs args) {
   using L = Layout<D>;
   constexpr int kStages = L::kStages;
+  constexpr int G = L::kGroups;
+  constexpr int kRows = L::kRows;
+  constexpr int kIssuer = L::kIssuer;
+  constexpr int kThreads = L::kThreads;
   const CachedAttn& p = args.p;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* smem = smem_raw;  // the swizzle wants 1 KB; checked below
   float* s_scale = reinterpret_cast<float*>(smem + L::kScale);  // [stage][2][8]
   int* s_poison = reinterpret_cast<int*>(smem + L::kPoison);
+  float* s_join = reinterpret_cast<float*>(smem + L::kJoin);
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + L::kBar);
   uint64_t* k_full = q_full + 1;
   uint64_t* v_full = k_full + kStages;
   uint64_t* kv_empty = v_full + kStages;
   uint64_t* s_full = kv_empty + kStages;  // [2] S_g of the next tile is in TMEM
-  uint64_t* p_full = s_full + 2;          // [2][2] a half of P_g is written (O_g rescaled if it had to be)
+  uint64_t* p_full = s_full + 2;          // [2][2] P_g's keys 0-31, 64-95 (then the others) are written, O_g rescaled
   uint64_t* o_full = p_full + 4;          // [2] O_g += P_g V has completed
-  uint64_t* teardown = o_full + 2;
+  uint64_t* met = o_full + 2;             // [8] the two warps of 32 rows meet
+  uint64_t* turn = met + 8;               // [2]
+  uint64_t* teardown = turn + 2;          // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(teardown + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_item = reinterpret_cast<int*>(tmem_slot + 2);  // request, row tile, number of tiles
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (smem_u32(smem) & 1023) {  // never with dynamic shared memory alone
+    if (threadIdx.x == 0) set_status(kBoundsError);
+    return;
+  }
   griddep_wait();
 
   // ---- which request and row tile: the last tiles, which see the most keys, come first
@@ -153,18 +171,21 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
   }
   for (int i = threadIdx.x; i < D; i += kThreads) s_poison[i] = 0x7fffffff;
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 8);
+    mbar_init(q_full, 8 * G);
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&k_full[s], 4);
       mbar_init(&v_full[s], 4);
-      mbar_init(&kv_empty[s], 2);
+      mbar_init(&kv_empty[s], G);
     }
-    for (int g = 0; g < 2; ++g) {
+    for (int g = 0; g < G; ++g) {
       mbar_init(&s_full[g], 1);
-      mbar_init(&p_full[2 * g], 4);
-      mbar_init(&p_full[2 * g + 1], 4);
+      mbar_init(&p_full[2 * g], 8);
+      mbar_init(&p_full[2 * g + 1], 8);
       mbar_init(&o_full[g], 1);
     }
+    for (int i = 0; i < 8; ++i) mbar_init(&met[i], 2);
+    mbar_init(&turn[0], 8);
+    mbar_init(&turn[1], 8);
     mbar_init(&teardown[0], 1);
     mbar_init(&teardown[1], 1);
     *abort_flag = 0;
@@ -206,10 +227,10 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
     const int lim = lim_of(min(rows, (g + 1) * kGroupRows) - 1);
     return max(0, min(t1, lim > 0 ? (lim + KT - 1) / KT : 0) - t0);
   };
-  const int n0 = tiles_of_group(0), n1 = tiles_of_group(1);
+  const int n0 = tiles_of_group(0), n1 = G == 2 ? tiles_of_group(1) : 0;
   const int nk = max(n0, n1);
 
-  if (warp == 12) tmem_alloc(tmem_slot, kTmemCols);
+  if (warp == kIssuer) tmem_alloc(tmem_slot, L::kTmemCols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -323,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
     fetch(V_{}, 1, now);
     for (int j = 0; j < nk; ++j) {
       const int st = j % kStages;
-      const bool ok = mbar_sleep_wait(&kv_empty[st], ((j / kStages) & 1) ^ 1, kTimeoutEmpty);
+      const bool ok = mbar_wait(&kv_empty[st], ((j / kStages) & 1) ^ 1, kTimeoutEmpty);
       if (!__all_sync(0xffffffffu, ok)) {
         *abort_flag = 1;
         break;
@@ -347,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
       id = id_of(j + 3);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-  } else if (warp >= 12) {
+  } else if (warp >= kIssuer) {
     // ------------------------------------------------------------------ MMA issuers, one warp per group
     // The whole warp runs this, converged (umma_f16_warp); one lane issues. A warp of its own for each group waits for
     // exactly the next thing that the group needs; one that polled for both took 500 cycles to notice.
@@ -355,10 +376,10 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
     constexpr uint32_t id_s = idesc_f16(KT, false);
     constexpr uint32_t id_o = idesc_f16(D, true);
     const uint32_t elect = elect_one();
-    const int g = __shfl_sync(kAll, warp, 0) - 12;
+    const int g = __shfl_sync(kAll, warp, 0) - kIssuer;
     const int count = __shfl_sync(kAll, g == 0 ? n0 : n1, 0), all = __shfl_sync(kAll, nk, 0);
     const uint32_t acc = __shfl_sync(kAll, tmem, 0);
-    const uint32_t t_s = acc + g * KT, t_o = acc + L::kTmemO + g * D, t_p = acc + L::tmem_p(g);
+    const uint32_t t_s = acc + g * KT, t_o = acc + L::kTmemO + g * D, t_p = acc + L::kTmemP + g * KT;
     const uint64_t dq = smem_desc_sw128(smem_u32(smem) + g * L::kQBytes, 16, 1024);
     const uint64_t dk0 = smem_desc_sw128(smem_u32(smem + L::kKV), 16, 1024);
     const uint64_t dv0 = smem_desc_sw128(smem_u32(smem + L::kKV + L::kTileBytes), KT * 128, 1024);
@@ -376,18 +397,21 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
                       dk + (((k / 4) * (KT * 128) + (k % 4) * 32) >> 4), id_s, k > 0 ? 1u : 0u, elect);
       umma_commit_warp(&s_full[g], elect);
     };
-    auto issue_o = [&](int j, int half) {
-      const uint64_t dv = dv0 + static_cast<uint32_t>((j % kStages) * ((2 * L::kTileBytes) >> 4) + half * ((4 * 2048) >> 4));
+    auto issue_o = [&](int j, int part) {
+      const uint64_t dv = dv0 + static_cast<uint32_t>((j % kStages) * ((2 * L::kTileBytes) >> 4));
       tc_fence_after();
 #pragma unroll
-      for (int k = 0; k < KT / 32; ++k)
-        umma_f16_ts_warp(t_o, t_p + half * 32 + k * 8, dv + ((k * 2048) >> 4), id_o, k > 0 || half > 0 || j > 0 ? 1u : 0u,
-                         elect);
+      for (int i = 0; i < 4; ++i) {
+        const int k = (i & 1) + (i >> 1) * 4 + part * 2;
+        umma_f16_ts_warp(t_o, t_p + (k / 4) * L::kPHalf + (k % 4) * 8, dv + ((k * 2048) >> 4), id_o,
+                         i > 0 || part > 0 || j > 0 ? 1u : 0u, elect);
+      }
     };
     if (count > 0 && wait(q_full, 0, kTimeoutFull) && wait(&k_full[0], 0, kTimeoutFull)) issue_s(0);
     for (int j = 0; ok && j < count; ++j) {
       const bool more = j + 1 < count;
-      if (!wait(&v_full[j % kStages], j / kStages, kTimeoutFull) || !wait(&p_full[2 * g], j, kTimeoutAccum)) break;
+      if (!wait(&v_full[j % kStages], j / kStages, kTimeoutFull)) break;
+      if (!wait(&p_full[2 * g], j, kTimeoutAccum)) break;
       issue_o(j, 0);
       if (more && !wait(&k_full[(j + 1) % kStages], (j + 1) / kStages, kTimeoutFull)) break;
       if (!wait(&p_full[2 * g + 1], j, kTimeoutAccum)) break;
@@ -410,16 +434,27 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
     __syncwarp();
   } else {
     // ------------------------------------------------------------------ softmax
-    const int g = (warp - 4) / 4;
+    // Two threads share a row: each makes the weights of 64 of a tile's keys and rescales and writes half of the row's output.
+    // Four such warps on a sub-partition hide each other's latencies; two took 1.5 times as long for a tile.
+    const int g = (warp - 4) / 8, half = (warp - 4) / 4 % 2;
     const int row = (warp % 4) * 32 + lane;     // of the group = TMEM lane
     const int r = g * kGroupRows + row;         // of the tile
     const int n_g = g == 0 ? n0 : n1;
     const bool real = r < rows;
     const int tok = q0 + (row0 + r) / p.group, head = h * p.group + (row0 + r) % p.group;
     const uint32_t lane_off = static_cast<uint32_t>((warp % 4) * 32) << 16;
-    const uint32_t ts = tmem + lane_off + g * KT;
-    const uint32_t to = tmem + lane_off + L::kTmemO + g * D;
-    const uint32_t tp = tmem + lane_off + L::tmem_p(g);
+    const uint32_t ts = tmem + lane_off + g * KT + half * 64;
+    const uint32_t to = tmem + lane_off + L::kTmemO + g * D + half * (D / 2);
+    const uint32_t tp = tmem + lane_off + L::kTmemP + g * KT + half * L::kPHalf;
+    float* const s_mine = s_join + (g * 2 + half) * kGroupRows + row;
+    const float* const s_other = s_join + (g * 2 + 1 - half) * kGroupRows + row;
+    // the two warps of the same 32 rows (a barrier whose wait is bounded)
+    uint64_t* const my_met = &met[g * 4 + warp % 4];
+    auto meet = [&](int phase) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(my_met);
+      return __all_sync(0xffffffffu, mbar_wait(my_met, phase & 1, kTimeoutAccum)) != 0;
+    };
     float unit = 0.f;
     {
       // the query row in f16, divided by a power of two that brings its largest number to [1, 2)
@@ -443,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
       const float inv = fine ? exp2i(-e) : 1.f;
       unit = (fine ? exp2i(e) : 1.f) * p.scale * kLog2e;
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
+      for (int c = half * (D / 16); c < (half + 1) * (D / 16); ++c) {
         uint4 out = make_uint4(0, 0, 0, 0);
         if (real) {
           const uint4 w = __ldg(src + c);
@@ -461,19 +496,20 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
     }
     const int lim = lim_of(r);
     const int lim_group = lim_of(g * kGroupRows);  // the group's first row sees the fewest keys
-    // running maximum, sum, and log2 of the largest value scale that the row has seen
+    // running maximum, sum (of this thread's keys), and log2 of the largest value scale that the row has seen
     float m_run = kNone, l_run = 0.f, v_ref = -INFINITY;
     bool ok = true;
     for (int j = 0; j < n_g; ++j) {
       const int st = j % kStages;
       // the scales are written before k_full completes; S_g comes after it
-      if (!__all_sync(0xffffffffu, mbar_sleep_wait(&k_full[st], (j / kStages) & 1, kTimeoutFull) &&
-                                       mbar_sleep_wait(&s_full[g], j & 1, kTimeoutAccum))) { ok = false; break; }
+      if (!__all_sync(0xffffffffu, mbar_wait(&k_full[st], (j / kStages) & 1, kTimeoutFull) &&
+                                       mbar_wait(&s_full[g], j & 1, kTimeoutAccum))) { ok = false; break; }
       tc_fence_after();
       const int k0 = (t0 + j) * KT;
-      const int lim_tile = lim - k0;
-      const float* sc = s_scale + st * 16;  // [8] key scales, [8] log2 of value scales
-      bool plain = k0 + KT <= lim_group;    // the same for the whole warp: all rows see all 128 keys
+      const int lim_tile = lim - k0 - half * 64;       // of this thread's 64 keys
+      const float* sc = s_scale + st * 16;             // [8] key scales, [8] log2 of value scales
+      const float* my_sc = sc + half * 4;
+      bool plain = k0 + KT <= lim_group;               // the same for the whole warp: all rows see all 128 keys
       float v_top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 8; i += 4) {
@@ -484,36 +520,37 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
       // ---- the row's maximum
       float mx = -INFINITY;
       if (plain) {
+        float v[64];
+        tmem_ld32_pair(ts, ts + 32, v, v + 32);
 #pragma unroll
-        for (int c = 0; c < KT; c += 64) {
-          float v[64];
-          tmem_ld32_pair(ts + c, ts + c + 32, v, v + 32);
-#pragma unroll
-          for (int i = 0; i < 64; i += 16) {
-            float a = fmax3(v[i], v[i + 1], v[i + 2]), d = fmax3(v[i + 3], v[i + 4], v[i + 5]);
-            a = fmax3(a, v[i + 6], v[i + 7]);
-            d = fmax3(d, v[i + 8], v[i + 9]);
-            a = fmax3(a, v[i + 10], v[i + 11]);
-            d = fmax3(d, v[i + 12], v[i + 13]);
-            mx = fmaxf(mx, fmaxf(fmax3(a, v[i + 14], v[i + 15]), d) * sc[(c + i) / 16]);
-          }
+        for (int i = 0; i < 64; i += 16) {
+          float a = fmax3(v[i], v[i + 1], v[i + 2]), d = fmax3(v[i + 3], v[i + 4], v[i + 5]);
+          a = fmax3(a, v[i + 6], v[i + 7]);
+          d = fmax3(d, v[i + 8], v[i + 9]);
+          a = fmax3(a, v[i + 10], v[i + 11]);
+          d = fmax3(d, v[i + 12], v[i + 13]);
+          mx = fmaxf(mx, fmaxf(fmax3(a, v[i + 14], v[i + 15]), d) * my_sc[i / 16]);
         }
       } else {
         v_top = -INFINITY;
 #pragma unroll 1
-        for (int c = 0; c < KT; c += 16) {
+        for (int i = 0; i < 8; ++i)
+          if (sc[i] >= 0.f && i * 16 < lim - k0) v_top = fmaxf(v_top, sc[8 + i]);
+#pragma unroll 1
+        for (int c = 0; c < 64; c += 16) {
           float v[16];
           tmem_ld16(ts + c, v);
-          const float f = sc[c / 16];
-          if (f >= 0.f && c < lim_tile) v_top = fmaxf(v_top, sc[8 + c / 16]);
+          const float f = my_sc[c / 16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) mx = fmaxf(mx, f >= 0.f && c + i < lim_tile ? v[i] * f : -INFINITY);
         }
       }
-      mx *= unit;
+      *s_mine = mx * unit;
+      if (!meet(j)) { ok = false; break; }
+      mx = fmaxf(mx * unit, *s_other);
       float factor = 1.f;
       bool rescale = false;
-      if (__any_sync(0xffffffffu, mx > m_run + kLazy || v_top > v_ref)) {
+      if (__any_sync(0xffffffffu, mx > m_run + kLazy || v_top > v_ref)) {  // the same in both warps
         const float m_new = fmaxf(m_run, mx), v_new = fmaxf(v_ref, v_top);
         const float f = exp2f_approx(m_run - m_new);
         factor = v_ref == -INFINITY ? 0.f : f * exp2f_approx(v_ref - v_new);
@@ -522,13 +559,15 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
         v_ref = v_new;
         rescale = j > 0;
       }
-      // O_g += P_g V of the tile before has to be complete before P_g (head_dim 64) or O_g is written; its values are in
-      // shared memory before P_g is handed on (v_full is the issuer's to wait for)
-      if (j > 0 && !__all_sync(0xffffffffu, mbar_sleep_wait(&o_full[g], (j - 1) & 1, kTimeoutAccum))) { ok = false; break; }
-      tc_fence_after();
+      // O_g += P_g V of the tile before has to be complete before P_g (head_dim 64) or O_g is written
+      // (head_dim 128: S_g came after it)
+      if constexpr (!L::kAlias) {
+        if (j > 0 && !__all_sync(0xffffffffu, mbar_wait(&o_full[g], (j - 1) & 1, kTimeoutAccum))) { ok = false; break; }
+        tc_fence_after();
+      }
       if (rescale) {
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
+        for (int c = 0; c < D / 2; c += 32) {
           float o[32];
           tmem_ld32(to + c, o);
 #pragma unroll
@@ -536,50 +575,51 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
           tmem_st32(to + c, o);
         }
       }
+      if (G == 2 && (g == 0 ? j > 0 && j - 1 < n1 : j < n0)) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&turn[1 - g], (g == 0 ? j - 1 : j) & 1, kTimeoutAccum))) { ok = false; break; }
+      }
       // ---- weights. A group's value scale goes into the exponent (at most 2^8 up, and not below 2^-60, where an f16 weight
       // is zero and the sum would lose it), so that the sum takes it out again once per 16 keys.
-      auto hand_on = [&](int half) {  // the first 64 keys' weights are used while the others are made
+      auto hand_on = [&](int part) {
+        if (part == 1 && lane == 0) mbar_arrive(&turn[g]);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[2 * g + half]);
+        if (lane == 0) mbar_arrive(&p_full[2 * g + part]);
       };
       const float neg_m = -m_run, v_off = kWeightUpLog2 - v_ref;
       if (plain) {
 #pragma unroll
-        for (int c = 0; c < KT; c += 64) {
-          float v[64];
-          tmem_ld32_pair(ts + c, ts + c + 32, v, v + 32);
-#pragma unroll
-          for (int q = 0; q < 64; q += 32) {
-            uint32_t w[16];
-#pragma unroll
-            for (int i = q; i < q + 32; i += 16) {
-              const float f = unit * sc[(c + i) / 16], up = fmaxf(sc[8 + (c + i) / 16] + v_off, -60.f);
-              const float2 f2 = make_float2(f, f), off = make_float2(neg_m + up, neg_m + up);
-              float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-              for (int k = i; k < i + 16; k += 2) {
-                const float2 x = fma_f32x2(make_float2(v[k], v[k + 1]), f2, off);
-                const float2 e = make_float2(exp2f_approx(x.x), exp2f_approx(x.y));
-                sum = k == i ? e : add_f32x2(sum, e);
-                w[(k - q) / 2] = pack_f16(e.x, e.y);
-              }
-              l_run = fmaf(sum.x + sum.y, exp2f_approx(-up), l_run);
-            }
-            tmem_st16u(tp + (c + q) / 2, w);
-          }
-          hand_on(c / 64);
-        }
-      } else {
-#pragma unroll 1
-        for (int c = 0; c < KT; c += 32) {
+        for (int c = 0; c < 64; c += 32) {
           float v[32];
           uint32_t w[16];
           tmem_ld32(ts + c, v);
 #pragma unroll
           for (int i = 0; i < 32; i += 16) {
-            const float ks = sc[(c + i) / 16], up = fmaxf(sc[8 + (c + i) / 16] + v_off, -60.f);
+            const float f = unit * my_sc[(c + i) / 16], up = fmaxf(my_sc[8 + (c + i) / 16] + v_off, -60.f);
+            const float2 f2 = make_float2(f, f), off = make_float2(neg_m + up, neg_m + up);
+            float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int k = i; k < i + 16; k += 2) {
+              const float2 x = fma_f32x2(make_float2(v[k], v[k + 1]), f2, off);
+              const float2 e = make_float2(exp2f_approx(x.x), exp2f_approx(x.y));
+              sum = k == i ? e : add_f32x2(sum, e);
+              w[k / 2] = pack_f16(e.x, e.y);
+            }
+            l_run = fmaf(sum.x + sum.y, exp2f_approx(-up), l_run);
+          }
+          tmem_st16u(tp + c / 2, w);
+          hand_on(c / 32);
+        }
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < 64; c += 32) {
+          float v[32];
+          uint32_t w[16];
+          tmem_ld32(ts + c, v);
+#pragma unroll
+          for (int i = 0; i < 32; i += 16) {
+            const float ks = my_sc[(c + i) / 16], up = fmaxf(my_sc[8 + (c + i) / 16] + v_off, -60.f);
             const float f = unit * ks;
             float sum = 0.f;
 #pragma unroll
@@ -592,23 +632,28 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
             l_run = fmaf(sum, exp2f_approx(-up), l_run);
           }
           tmem_st16u(tp + c / 2, w);
-          if (c % 64 == 32) hand_on(c / 64);
+          hand_on(c / 32);
         }
       }
     }
-    if (ok && n_g > 0 && !__all_sync(0xffffffffu, mbar_sleep_wait(&o_full[g], (n_g - 1) & 1, kTimeoutAccum))) ok = false;
+    if (ok && n_g > 0 && !__all_sync(0xffffffffu, mbar_wait(&o_full[g], (n_g - 1) & 1, kTimeoutAccum))) ok = false;
+    if (ok) {
+      *s_mine = l_run;
+      ok = meet(n_g);
+    }
     if (!ok) {
       *abort_flag = 1;
     } else {
       tc_fence_after();
+      l_run += *s_other;
       const bool part = args.splits > 1;
       const float up = exp2f_approx(v_ref - kWeightUpLog2);
       const float inv = part ? up : (m_run == kNone ? 0.f : up / l_run);  // a row that sees no key is zero
       const int64_t slot = ((static_cast<int64_t>(s_item[2]) - 1 - blockIdx.x / p.Hkv) * p.Hkv + h) * args.splits + blockIdx.y;
-      bf16* out = p.out + static_cast<int64_t>(tok) * p.o_token + head * p.o_head;
-      float* part_o = p.part_o + (slot * kRows + r) * D;
+      bf16* out = p.out + static_cast<int64_t>(tok) * p.o_token + head * p.o_head + half * (D / 2);
+      float* part_o = p.part_o + (slot * kRows + r) * D + half * (D / 2);
 #pragma unroll
-      for (int c = 0; c < D; c += 32) {
+      for (int c = 0; c < D / 2; c += 32) {
         float o[32];
         if (n_g > 0) {
           tmem_ld32(to + c, o);  // by whole warps
@@ -620,7 +665,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             o[i] *= inv;
-            if (s_poison[c + i] < lim) o[i] = __int_as_float(0x7fffffff);
+            if (s_poison[half * (D / 2) + c + i] < lim) o[i] = __int_as_float(0x7fffffff);
           }
           if (part) {
 #pragma unroll
@@ -634,20 +679,21 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attn_tc_kernel(const __gri
           }
         }
       }
-      if (part && real) *reinterpret_cast<float2*>(p.part_ml + (slot * kRows + r) * 2) = make_float2(m_run, l_run);
+      if (part && real && half == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * kRows + r) * 2) = make_float2(m_run, l_run);
     }
   }
 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 12) tmem_dealloc(tmem, kTmemCols);
+  if (warp == kIssuer) tmem_dealloc(tmem, L::kTmemCols);
   griddep_launch();
 }
 
 // One warp per (token, query head): adds the splits' results in their order.
 template <int D>
 __global__ void __launch_bounds__(128) cached_attn_tc_join_kernel(CachedAttn p, int splits) {
+  constexpr int kRows = Layout<D>::kRows;
   const int lane = threadIdx.x % 32;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 32;
   griddep_wait();
@@ -695,7 +741,7 @@ void launch(const CachedAttn& p, int tiles_max, int splits, cudaStream_t stream)
     return true;
   }();
   (void)configured;
-  launch_pdl(kernel, dim3(static_cast<unsigned>(tiles_max) * p.Hkv, splits), dim3(kThreads), Layout<D>::kTotal, stream,
+  launch_pdl(kernel, dim3(static_cast<unsigned>(tiles_max) * p.Hkv, splits), dim3(Layout<D>::kThreads), Layout<D>::kTotal, stream,
              "cached_attention tc", TcArgs{p, splits});
   if (splits > 1) {
     const int64_t rows = static_cast<int64_t>(p.T) * p.Hkv * p.group;
