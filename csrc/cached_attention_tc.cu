@@ -59,7 +59,7 @@ struct Layout {
   static constexpr int kJoin = kPoison + D * 4;              // [groups][2 halves][128 rows]: maxima, at the end sums
   static constexpr int kBar = kJoin + kGroups * 1024;
   static constexpr int kBarriers = 21 + 3 * kStages;         // at most (see the pointers in the kernel)
-  static constexpr int kTotal = kBar + kBarriers * 8 + 24;   // and six words
+  static constexpr int kTotal = kBar + kBarriers * 8 + 32;   // and eight words
   static constexpr int kTmemO = kGroups * KT;
   static constexpr int kTmemP = kAlias ? 0 : kTmemO + kGroups * D;  // 128 columns apart where P_g lies in S_g
   static constexpr int kTmemCols = kGroups * 256;
@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 3 - Layout<D>::kGroups) c
   uint64_t* teardown = turn + 2;          // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(teardown + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* s_item = reinterpret_cast<int*>(tmem_slot + 2);  // request, row tile, number of tiles
+  int* s_item = reinterpret_cast<int*>(tmem_slot + 2);  // request, row tile, number of tiles, first row, new rows, context
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (smem_u32(smem) & 1023) {  // never with dynamic shared memory alone
@@ -135,12 +135,14 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 3 - Layout<D>::kGroups) c
 
   // ---- which request and row tile: the last tiles, which see the most keys, come first
   if (warp == 0) {
-    int total = 0;
-    auto tiles_of = [&](int b) {
-      const int n = new_rows(p, b).n;
-      return n > 0 ? static_cast<int>((static_cast<int64_t>(n) * p.group + kRows - 1) / kRows) : 0;
+    auto tiles_of = [&](const NewRows& x) {
+      return x.n > 0 ? static_cast<int>((static_cast<int64_t>(x.n) * p.group + kRows - 1) / kRows) : 0;
     };
-    for (int b = lane; b < p.B; b += 32) total += tiles_of(b);
+    // the first 32 requests stay in registers between the two passes
+    const NewRows mine = lane < p.B ? new_rows(p, lane) : NewRows{0, 0};
+    const int my_ctx = lane < p.B ? p.context[lane] : 0;
+    int total = tiles_of(mine);
+    for (int b = lane + 32; b < p.B; b += 32) total += tiles_of(new_rows(p, b));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     const int want = total - 1 - static_cast<int>(blockIdx.x) / p.Hkv;
@@ -153,7 +155,8 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 3 - Layout<D>::kGroups) c
     int before = 0;
     for (int b0 = 0; b0 < p.B; b0 += 32) {
       const int b = b0 + lane;
-      const int w = b < p.B ? tiles_of(b) : 0;
+      const NewRows rows_b = b0 == 0 ? mine : b < p.B ? new_rows(p, b) : NewRows{0, 0};
+      const int w = tiles_of(rows_b);
       int x = w;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -164,10 +167,15 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 3 - Layout<D>::kGroups) c
       if (want >= at && want < at + w) {
         s_item[0] = b;
         s_item[1] = want - at;
+        s_item[3] = rows_b.first;
+        s_item[4] = rows_b.n;
+        s_item[5] = b0 == 0 ? my_ctx : p.context[b];
       }
       if (publish && b < p.B) p.prefix[b] = at;
       before += __shfl_sync(0xffffffffu, x, 31);
     }
+  } else if (warp == kIssuer) {
+    tmem_alloc(tmem_slot, L::kTmemCols);  // freed below where the block has nothing to do
   }
   for (int i = threadIdx.x; i < D; i += kThreads) s_poison[i] = 0x7fffffff;
   if (threadIdx.x == 0) {
@@ -191,6 +199,7 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 3 - Layout<D>::kGroups) c
     *abort_flag = 0;
     fence_barrier_init();
   }
+  tc_fence_before();
   __syncthreads();
   const int b = s_item[0], row_tile = s_item[1];
   const int h = static_cast<int>(blockIdx.x) % p.Hkv;
@@ -206,18 +215,20 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 3 - Layout<D>::kGroups) c
           make_uint4(0, 0, 0, 0);
     }
   }
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
   if (b < 0) {  // the grid is an upper bound
+    if (warp == kIssuer) tmem_dealloc(tmem, L::kTmemCols);
     griddep_launch();
     return;
   }
 
-  const NewRows fresh = new_rows(p, b);
-  const int q0 = fresh.first, n = fresh.n;
-  const int ctx = min(p.context[b], p.max_table_tokens);
+  const int q0 = s_item[3], n = s_item[4], all_ctx = s_item[5];
+  const int ctx = min(all_ctx, p.max_table_tokens);
   const int row0 = row_tile * kRows;
   const int rows = static_cast<int>(min(static_cast<int64_t>(kRows), static_cast<int64_t>(n) * p.group - row0));
   // keys that a row of the tile sees: [0, lim)
-  auto lim_of = [&](int row) { return min(ctx, p.context[b] - n + (row0 + min(row, rows - 1)) / p.group + 1); };
+  auto lim_of = [&](int row) { return min(ctx, all_ctx - n + (row0 + min(row, rows - 1)) / p.group + 1); };
   const int lim_all = lim_of(0), lim_any = lim_of(rows - 1);
   const int tiles = lim_any > 0 ? (lim_any + KT - 1) / KT : 0;
   const int per = (tiles + args.splits - 1) / args.splits;
@@ -229,12 +240,6 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 3 - Layout<D>::kGroups) c
   };
   const int n0 = tiles_of_group(0), n1 = G == 2 ? tiles_of_group(1) : 0;
   const int nk = max(n0, n1);
-
-  if (warp == kIssuer) tmem_alloc(tmem_slot, L::kTmemCols);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
 
   if (warp < 4) {
     // ------------------------------------------------------------------ codes -> f16 tiles in shared memory
@@ -455,51 +460,49 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 3 - Layout<D>::kGroups) c
       if (lane == 0) mbar_arrive(my_met);
       return __all_sync(0xffffffffu, mbar_wait(my_met, phase & 1, kTimeoutAccum)) != 0;
     };
-    float unit = 0.f;
     {
-      // the query row in f16, divided by a power of two that brings its largest number to [1, 2)
-      const uint4* src = reinterpret_cast<const uint4*>(p.q + static_cast<int64_t>(tok) * p.q_token + head * p.q_head);
-      uint8_t* dst = smem + g * L::kQBytes + row * 128;
-      float m = 0.f;
-      if (real) {
+      // Query rows in f16, each divided by a power of two that brings its largest number to [1, 2). D / 8 lanes read a row.
+      constexpr int LPR = D / 8, RPI = 32 / LPR, NI = 16 / RPI;  // a warp has 16 rows
+      const int c = lane % LPR, w16 = (warp - 4) % 8;
+      uint4 w[NI];
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          const uint4 w = __ldg(src + c);
-          const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&w);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = __bfloat1622float2(x[i]);
-            m = fmaxf(m, fmaxf(fabsf(f.x), fabsf(f.y)));
-          }
-        }
+      for (int i = 0; i < NI; ++i) {
+        const int rr = g * kGroupRows + w16 * 16 + i * RPI + lane / LPR, rq = row0 + rr;
+        w[i] = make_uint4(0, 0, 0, 0);
+        if (rr < rows)
+          w[i] = __ldg(reinterpret_cast<const uint4*>(p.q + static_cast<int64_t>(q0 + rq / p.group) * p.q_token +
+                                                      (h * p.group + rq % p.group) * p.q_head) + c);
       }
-      const int e = min(max(static_cast<int>(__float_as_uint(m) >> 23) - 127, -100), 126);
-      const bool fine = m > 0.f && m <= 3.4028234e38f;  // zero or infinite rows as they are
-      const float inv = fine ? exp2i(-e) : 1.f;
-      unit = (fine ? exp2i(e) : 1.f) * p.scale * kLog2e;
 #pragma unroll
-      for (int c = half * (D / 16); c < (half + 1) * (D / 16); ++c) {
-        uint4 out = make_uint4(0, 0, 0, 0);
-        if (real) {
-          const uint4 w = __ldg(src + c);
-          const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&w);
-          const float2 f0 = __bfloat1622float2(x[0]), f1 = __bfloat1622float2(x[1]), f2 = __bfloat1622float2(x[2]),
-                       f3 = __bfloat1622float2(x[3]);
-          out = make_uint4(pack_f16(f0.x * inv, f0.y * inv), pack_f16(f1.x * inv, f1.y * inv),
-                           pack_f16(f2.x * inv, f2.y * inv), pack_f16(f3.x * inv, f3.y * inv));
-        }
-        *reinterpret_cast<uint4*>(dst + (c / 8) * (kGroupRows * 128) + ((c % 8) ^ (row & 7)) * 16) = out;
+      for (int i = 0; i < NI; ++i) {
+        const int in = w16 * 16 + i * RPI + lane / LPR;  // row of the group
+        const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&w[i]);
+        const float2 f0 = __bfloat1622float2(x[0]), f1 = __bfloat1622float2(x[1]), f2 = __bfloat1622float2(x[2]),
+                     f3 = __bfloat1622float2(x[3]);
+        float m = fmaxf(fmaxf(fmaxf(fabsf(f0.x), fabsf(f0.y)), fmaxf(fabsf(f1.x), fabsf(f1.y))),
+                        fmaxf(fmaxf(fabsf(f2.x), fabsf(f2.y)), fmaxf(fabsf(f3.x), fabsf(f3.y))));
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const int e = min(max(static_cast<int>(__float_as_uint(m) >> 23) - 127, -100), 126);
+        const bool fine = m > 0.f && m <= 3.4028234e38f;  // zero or infinite rows as they are
+        const float inv = fine ? exp2i(-e) : 1.f;
+        *reinterpret_cast<uint4*>(smem + g * L::kQBytes + (c / 8) * (kGroupRows * 128) + in * 128 + ((c % 8) ^ (in & 7)) * 16) =
+            make_uint4(pack_f16(f0.x * inv, f0.y * inv), pack_f16(f1.x * inv, f1.y * inv), pack_f16(f2.x * inv, f2.y * inv),
+                       pack_f16(f3.x * inv, f3.y * inv));
+        if (c < 2)  // for the two threads of the row
+          s_join[(g * 2 + c) * kGroupRows + in] = (fine ? exp2i(e) : 1.f) * p.scale * kLog2e;
       }
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
     }
+    bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0, kTimeoutFull)) != 0;
+    const float unit = *s_mine;  // what a product of codes and fragments is worth, but for the key's scale
     const int lim = lim_of(r);
     const int lim_group = lim_of(g * kGroupRows);  // the group's first row sees the fewest keys
     // running maximum, sum (of this thread's keys), and log2 of the largest value scale that the row has seen
     float m_run = kNone, l_run = 0.f, v_ref = -INFINITY;
-    bool ok = true;
-    for (int j = 0; j < n_g; ++j) {
+    for (int j = 0; ok && j < n_g; ++j) {
       const int st = j % kStages;
       // the scales are written before k_full completes; S_g comes after it
       if (!__all_sync(0xffffffffu, mbar_wait(&k_full[st], (j / kStages) & 1, kTimeoutFull) &&
