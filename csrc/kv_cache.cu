@@ -214,11 +214,14 @@ struct AppendArgs {
   int64_t c_block[2], c_head[2], c_token[2];
   float* scale[2];  // [blocks, Hkv]
   int64_t s_block[2];
-  int T, Hkv, block, blocks, rows;  // rows: tokens of a block of threads
+  int T, Hkv, block, blocks;
+  int rows;   // tokens of a block of threads
+  int turns;  // (head, keys or values) pairs of a team
 };
 
-constexpr int kAppendThreads = 128;
-constexpr int kKeep = 8;  // 16-byte pieces of a run that a thread keeps between its two passes
+constexpr int kAppendThreads = 256;
+constexpr int kAppendRows = 128;  // most tokens of a block of threads
+constexpr int kKeep = 8;          // 16-byte pieces of a run that a thread keeps between its two passes
 
 __device__ __forceinline__ float finite_abs(float v) {
   const float a = fabsf(v);
@@ -245,9 +248,9 @@ __device__ __forceinline__ uint2 encode8(const uint4& w, float inv) {
                     Kv<FMT>::encode4(c.x * inv, c.y * inv, d.x * inv, d.y * inv));
 }
 
-// The tokens [t0, t0 + n) of one (block, head), written by NT threads (a warp or the whole block of threads).
+// The tokens [t0, t0 + n) of one (block, head), written by a team of NT threads.
 template <int FMT, int D, int NT>
-__device__ __forceinline__ void append_run(const AppendArgs& a, int kv, int h, int t0, int n, int me, float* red) {
+__device__ __forceinline__ void append_run(const AppendArgs& a, int kv, int h, int t0, int n, int team, int me, float* red) {
   constexpr int PPR = D / 8;  // 16-byte pieces of a token's row
   const int slot0 = a.slots[t0];
   const int64_t id = slot0 / a.block;
@@ -272,9 +275,13 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, int kv, int h, i
     if (me + k * NT < pieces) m = fmaxf(m, amax8(keep[k]));
   for (int i = me + kKeep * NT; i < pieces; i += NT) m = fmaxf(m, amax8(__ldg(source(i))));
   m = warp_max(m);
+  auto team_sync = [&]() {
+    if constexpr (NT > 32) asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(NT) : "memory");
+    else __syncwarp();
+  };
   if constexpr (NT > 32) {
     if (me % 32 == 0) red[me / 32] = m;
-    __syncthreads();
+    team_sync();
     m = red[0];
 #pragma unroll
     for (int w = 1; w < NT / 32; ++w) m = fmaxf(m, red[w]);
@@ -306,26 +313,26 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, int kv, int h, i
   for (int k = 0; k < kKeep; ++k)
     if (me + k * NT < pieces) put(me + k * NT, keep[k]);
   for (int i = me + kKeep * NT; i < pieces; i += NT) put(i, __ldg(source(i)));
-  if constexpr (NT > 32) __syncthreads();  // `red` and the old scale have been read
-  else __syncwarp();
+  team_sync();  // `red` and the old scale have been read
   if (me == 0) *sp = scale;
 }
 
-// A block of threads owns the runs (neighbouring tokens of one cache block) that begin in its `rows` tokens, for one
-// head of the keys or the values: one owner per (cache block, head), so the scale needs no atomics. With few runs all
-// threads share one, with many (decode: every token is a run) each warp takes its own. A run is read once: its pieces
-// stay in registers between the search for the largest magnitude and the rounding (up to 64 tokens of 128 numbers; the
-// rest of a longer one is read again, from L1 or L2).
-// Bound by HBM for prompts (2 bytes read, 1 written per number), by the latency of two dependent reads for decode.
-template <int FMT, int D>
+// A block of threads owns the runs (neighbouring tokens of one cache block) that begin in its `rows` tokens; each of its
+// teams writes them for `turns` (head, keys or values) pairs. So every (cache block, head) has one owner and the scale needs
+// no atomics. A run is read once: a thread keeps its pieces in registers between the search for the largest magnitude and
+// the rounding, which sets the team's size (NT = block * D / 64 threads; a longer run's rest is read again, from L2).
+// Bound by HBM for prompts (2 bytes read, 1 written per number), by the latency of dependent reads for decode. With a block
+// of threads per (run, head) and 4 KB of each run in flight, prompts ran at 16% of HBM; with a warp per pair the runs are
+// looked for once per eight pairs.
+template <int FMT, int D, int NT>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(AppendArgs a) {
-  __shared__ int s_first[kAppendThreads];
+  constexpr int kTeams = kAppendThreads / NT;
+  __shared__ int s_first[kAppendRows];
   __shared__ int s_n;
   __shared__ float s_red[kAppendThreads / 32];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int lane = threadIdx.x % 32, team = threadIdx.x / NT, me = threadIdx.x % NT;
   griddep_wait();
   griddep_launch();
-  const int kv = blockIdx.y & 1, h = blockIdx.y >> 1;
   const int r0 = blockIdx.x * a.rows, r1 = min(r0 + a.rows, a.T);
   if (threadIdx.x == 0) s_n = 0;
   __syncthreads();
@@ -353,26 +360,41 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(AppendArgs a) {
       if (same != 0xffffffffu) return n;
     }
   };
-  if (runs >= kAppendThreads / 32) {
-    for (int i = warp; i < runs; i += kAppendThreads / 32)
-      append_run<FMT, D, 32>(a, kv, h, s_first[i], length(s_first[i]), lane, nullptr);
-  } else {
-    for (int i = 0; i < runs; ++i) {
-      const int n = length(s_first[i]);
-      if (n * (D / 8) <= 32) {  // a short one: a warp is enough
-        if (warp == i) append_run<FMT, D, 32>(a, kv, h, s_first[i], n, lane, nullptr);
-      } else {
-        append_run<FMT, D, kAppendThreads>(a, kv, h, s_first[i], n, threadIdx.x, s_red);
-      }
+  for (int i = 0; i < runs; ++i) {
+    const int t0 = s_first[i], n = length(t0);
+    for (int k = 0; k < a.turns; ++k) {
+      const int pair = (blockIdx.y * a.turns + k) * kTeams + team;
+      if (pair < 2 * a.Hkv) append_run<FMT, D, NT>(a, pair & 1, pair >> 1, t0, n, team, me, s_red + team * (NT / 32));
     }
   }
 }
 
+template <int FMT, int D, int NT>
+void append_launch(AppendArgs a, cudaStream_t stream) {
+  constexpr int kTeams = kAppendThreads / NT;
+  const int groups = (2 * a.Hkv + kTeams - 1) / kTeams;
+  // few tokens: one per block of threads and one pair per team, for latency; many: a cache block of tokens, so that a
+  // prompt's runs have one owner each, and all pairs of a few hundred blocks per SM in one
+  a.rows = std::max(1, std::min({a.block, kAppendRows, static_cast<int>(static_cast<int64_t>(a.T) * groups / (148 * 4))}));
+  const int64_t tiles = (a.T + a.rows - 1) / a.rows;
+  a.turns = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(groups, tiles * groups / (148 * 16))));
+  const dim3 grid(static_cast<unsigned>(tiles), (groups + a.turns - 1) / a.turns);
+  launch_pdl(append_kernel<FMT, D, NT>, grid, dim3(kAppendThreads), 0, stream, "append_kv", a);
+}
+
+template <int FMT, int D>
+void append_team(const AppendArgs& a, cudaStream_t stream) {
+  const int pieces = a.block * (D / 8);
+  if (pieces <= 32 * kKeep) append_launch<FMT, D, 32>(a, stream);
+  else if (pieces <= 64 * kKeep) append_launch<FMT, D, 64>(a, stream);
+  else append_launch<FMT, D, 128>(a, stream);
+}
+
 template <int FMT>
-void append_launch(const AppendArgs& a, int D, dim3 grid, cudaStream_t stream) {
-  if (D == 32) launch_pdl(append_kernel<FMT, 32>, grid, dim3(kAppendThreads), 0, stream, "append_kv", a);
-  else if (D == 64) launch_pdl(append_kernel<FMT, 64>, grid, dim3(kAppendThreads), 0, stream, "append_kv", a);
-  else launch_pdl(append_kernel<FMT, 128>, grid, dim3(kAppendThreads), 0, stream, "append_kv", a);
+void append_dim(const AppendArgs& a, int D, cudaStream_t stream) {
+  if (D == 32) append_team<FMT, 32>(a, stream);
+  else if (D == 64) append_team<FMT, 64>(a, stream);
+  else append_team<FMT, 128>(a, stream);
 }
 
 }  // namespace
@@ -418,12 +440,8 @@ void append_kv(const KvSource& k, const KvSource& v, const int* slots, const KvP
   a.Hkv = Hkv;
   a.block = block;
   a.blocks = blocks;
-  // few tokens: one per block of threads, for latency; many: up to a cache block of them, so that a prompt's runs are
-  // found by one owner each without a block of threads per token
-  a.rows = std::max(1, std::min(std::min(block, kAppendThreads), static_cast<int>(static_cast<int64_t>(T) * Hkv * 2 / (148 * 8))));
-  const dim3 grid((T + a.rows - 1) / a.rows, Hkv * 2);
-  if (fmt == kKvFp8) append_launch<kKvFp8>(a, D, grid, stream);
-  else append_launch<kKvInt8>(a, D, grid, stream);
+  if (fmt == kKvFp8) append_dim<kKvFp8>(a, D, stream);
+  else append_dim<kKvInt8>(a, D, stream);
 }
 
 }  // namespace qw
