@@ -223,29 +223,47 @@ constexpr int kAppendThreads = 256;
 constexpr int kAppendRows = 128;  // most tokens of a block of threads
 constexpr int kKeep = 8;          // 16-byte pieces of a run that a thread keeps between its two passes
 
-__device__ __forceinline__ float finite_abs(float v) {
-  const float a = fabsf(v);
-  return a <= 3.4028234e38f ? a : 0.f;  // infinities saturate and NaN is no size: neither sets a block's scale
+// Largest magnitude of eight numbers as bf16 bits, two at a time: without the sign they order like unsigned integers.
+// Infinities and NaN come out as 0x7f80 and above.
+__device__ __forceinline__ uint32_t amax_bits(const uint4& w) {
+  const uint32_t m = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
+  return max(m & 0xffffu, m >> 16);
 }
+constexpr uint32_t kInfBits = 0x7f80u;
 
-__device__ __forceinline__ float amax8(const uint4& w) {
-  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
-  float m = 0.f;
+// The same without infinities and NaN: neither sets a block's scale.
+__device__ __forceinline__ uint32_t amax_bits_finite(const uint4& w) {
+  const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+  uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 f = __bfloat1622float2(h[i]);
-    m = fmaxf(m, fmaxf(finite_abs(f.x), finite_abs(f.y)));
+    const uint32_t lo = x[i] & 0x7fffu, hi = (x[i] >> 16) & 0x7fffu;
+    m = max(m, max(lo < kInfBits ? lo : 0u, hi < kInfBits ? hi : 0u));
   }
   return m;
 }
 
-template <int FMT>
+template <int FMT, bool FINITE>
 __device__ __forceinline__ uint2 encode8(const uint4& w, float inv) {
-  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
-  const float2 a = __bfloat1622float2(h[0]), b = __bfloat1622float2(h[1]), c = __bfloat1622float2(h[2]),
-               d = __bfloat1622float2(h[3]);
-  return make_uint2(Kv<FMT>::encode4(a.x * inv, a.y * inv, b.x * inv, b.y * inv),
-                    Kv<FMT>::encode4(c.x * inv, c.y * inv, d.x * inv, d.y * inv));
+  const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(x[i] << 16);
+    f[2 * i + 1] = __uint_as_float(x[i] & 0xffff0000u);
+  }
+  if constexpr (FINITE && FMT == kKvInt8) {
+    // |f * inv| <= 127: added to 1.5 * 2^23 the number is rounded to the nearest integer, ties to even, whose low byte is the
+    // code
+    uint32_t c[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = __float_as_uint(fmaf(f[i], inv, 12582912.f));
+    return make_uint2(__byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410),
+                      __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410));
+  } else {
+    return make_uint2(Kv<FMT>::encode4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
+                      Kv<FMT>::encode4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
+  }
 }
 
 // The tokens [t0, t0 + n) of one (block, head), written by a team of NT threads.
@@ -266,15 +284,23 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, int kv, int h, i
     return reinterpret_cast<const uint4*>(x + static_cast<int64_t>(t0 + i / PPR) * ts + (i % PPR) * 8);
   };
   uint4 keep[kKeep];
-  float m = 0.f;
+  uint32_t bits = 0;
 #pragma unroll
   for (int k = 0; k < kKeep; ++k)
     if (me + k * NT < pieces) keep[k] = __ldg(source(me + k * NT));
 #pragma unroll
   for (int k = 0; k < kKeep; ++k)
-    if (me + k * NT < pieces) m = fmaxf(m, amax8(keep[k]));
-  for (int i = me + kKeep * NT; i < pieces; i += NT) m = fmaxf(m, amax8(__ldg(source(i))));
-  m = warp_max(m);
+    if (me + k * NT < pieces) bits = max(bits, amax_bits(keep[k]));
+  for (int i = me + kKeep * NT; i < pieces; i += NT) bits = max(bits, amax_bits(__ldg(source(i))));
+  const bool finite = bits < kInfBits;
+  if (!finite) {
+    bits = 0;
+#pragma unroll
+    for (int k = 0; k < kKeep; ++k)
+      if (me + k * NT < pieces) bits = max(bits, amax_bits_finite(keep[k]));
+    for (int i = me + kKeep * NT; i < pieces; i += NT) bits = max(bits, amax_bits_finite(__ldg(source(i))));
+  }
+  float m = __uint_as_float(__reduce_max_sync(0xffffffffu, bits) << 16);
   auto team_sync = [&]() {
     if constexpr (NT > 32) asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(NT) : "memory");
     else __syncwarp();
@@ -307,7 +333,7 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, int kv, int h, i
   }
   auto put = [&](int i, const uint4& w) {
     const int s = a.slots[t0 + i / PPR] - static_cast<int>(id) * a.block;
-    *reinterpret_cast<uint2*>(rows + s * ct + (i % PPR) * 8) = encode8<FMT>(w, inv);
+    *reinterpret_cast<uint2*>(rows + s * ct + (i % PPR) * 8) = finite ? encode8<FMT, true>(w, inv) : encode8<FMT, false>(w, inv);
   };
 #pragma unroll
   for (int k = 0; k < kKeep; ++k)
@@ -325,7 +351,7 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, int kv, int h, i
 // of threads per (run, head) and 4 KB of each run in flight, prompts ran at 16% of HBM; with a warp per pair the runs are
 // looked for once per eight pairs.
 template <int FMT, int D, int NT>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, 3) append_kernel(AppendArgs a) {
   constexpr int kTeams = kAppendThreads / NT;
   __shared__ int s_first[kAppendRows];
   __shared__ int s_n;
