@@ -279,26 +279,28 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, int kv, int h, i
   uint8_t* rows = (kv ? a.cache[1] : a.cache[0]) + id * (kv ? a.c_block[1] : a.c_block[0]) + h * (kv ? a.c_head[1] : a.c_head[0]);
   float* sp = (kv ? a.scale[1] : a.scale[0]) + id * (kv ? a.s_block[1] : a.s_block[0]) + h;
   const float old = first > 0 ? *sp : 0.f;
-  const int pieces = n * PPR;
-  auto source = [&](int i) {
-    return reinterpret_cast<const uint4*>(x + static_cast<int64_t>(t0 + i / PPR) * ts + (i % PPR) * 8);
-  };
+  // the thread's pieces: column `me % PPR` of the rows row0, row0 + RS, ... (one 64-bit step each, no products)
+  constexpr int RS = NT / PPR;
+  const int row0 = me / PPR;
+  const bf16* const src = x + static_cast<int64_t>(t0 + row0) * ts + (me % PPR) * 8;
+  const int64_t src_step = RS * ts;
   uint4 keep[kKeep];
   uint32_t bits = 0;
+  {
+    const bf16* q = src;
 #pragma unroll
-  for (int k = 0; k < kKeep; ++k)
-    if (me + k * NT < pieces) keep[k] = __ldg(source(me + k * NT));
+    for (int k = 0; k < kKeep; ++k, q += src_step)
+      if (row0 + k * RS < n) keep[k] = __ldg(reinterpret_cast<const uint4*>(q));
 #pragma unroll
-  for (int k = 0; k < kKeep; ++k)
-    if (me + k * NT < pieces) bits = max(bits, amax_bits(keep[k]));
-  for (int i = me + kKeep * NT; i < pieces; i += NT) bits = max(bits, amax_bits(__ldg(source(i))));
+    for (int k = 0; k < kKeep; ++k)
+      if (row0 + k * RS < n) bits = max(bits, amax_bits(keep[k]));
+    for (int r = row0 + kKeep * RS; r < n; r += RS, q += src_step) bits = max(bits, amax_bits(__ldg(reinterpret_cast<const uint4*>(q))));
+  }
   const bool finite = bits < kInfBits;
   if (!finite) {
     bits = 0;
-#pragma unroll
-    for (int k = 0; k < kKeep; ++k)
-      if (me + k * NT < pieces) bits = max(bits, amax_bits_finite(keep[k]));
-    for (int i = me + kKeep * NT; i < pieces; i += NT) bits = max(bits, amax_bits_finite(__ldg(source(i))));
+    for (int r = row0; r < n; r += RS)
+      bits = max(bits, amax_bits_finite(__ldg(reinterpret_cast<const uint4*>(src + static_cast<int64_t>(r - row0) * ts))));
   }
   float m = __uint_as_float(__reduce_max_sync(0xffffffffu, bits) << 16);
   auto team_sync = [&]() {
@@ -331,14 +333,21 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, int kv, int h, i
       *p = Kv<FMT>::encode4(u.x * ratio, u.y * ratio, v.x * ratio, v.y * ratio);
     }
   }
-  auto put = [&](int i, const uint4& w) {
-    const int s = a.slots[t0 + i / PPR] - static_cast<int>(id) * a.block;
-    *reinterpret_cast<uint2*>(rows + s * ct + (i % PPR) * 8) = finite ? encode8<FMT, true>(w, inv) : encode8<FMT, false>(w, inv);
+  // Ascending slots as many as their span are consecutive; others (a plan never makes them) are looked up one by one.
+  const bool straight = a.slots[t0 + n - 1] - slot0 == n - 1;
+  uint8_t* const dst = rows + static_cast<int64_t>(first + row0) * ct + (me % PPR) * 8;
+  auto put = [&](int r, uint8_t* to, const uint4& w) {
+    if (!straight) to = rows + static_cast<int64_t>(a.slots[t0 + r] - static_cast<int>(id) * a.block) * ct + (me % PPR) * 8;
+    *reinterpret_cast<uint2*>(to) = finite ? encode8<FMT, true>(w, inv) : encode8<FMT, false>(w, inv);
   };
+  {
+    uint8_t* q = dst;
 #pragma unroll
-  for (int k = 0; k < kKeep; ++k)
-    if (me + k * NT < pieces) put(me + k * NT, keep[k]);
-  for (int i = me + kKeep * NT; i < pieces; i += NT) put(i, __ldg(source(i)));
+    for (int k = 0; k < kKeep; ++k, q += RS * ct)
+      if (row0 + k * RS < n) put(row0 + k * RS, q, keep[k]);
+    for (int r = row0 + kKeep * RS; r < n; r += RS, q += RS * ct)
+      put(r, q, __ldg(reinterpret_cast<const uint4*>(src + static_cast<int64_t>(r - row0) * ts)));
+  }
   team_sync();  // `red` and the old scale have been read
   if (me == 0) *sp = scale;
 }
@@ -353,44 +362,38 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, int kv, int h, i
 template <int FMT, int D, int NT>
 __global__ void __launch_bounds__(kAppendThreads, 3) append_kernel(AppendArgs a) {
   constexpr int kTeams = kAppendThreads / NT;
-  __shared__ int s_first[kAppendRows];
-  __shared__ int s_n;
   __shared__ float s_red[kAppendThreads / 32];
   const int lane = threadIdx.x % 32, team = threadIdx.x / NT, me = threadIdx.x % NT;
   griddep_wait();
   griddep_launch();
   const int r0 = blockIdx.x * a.rows, r1 = min(r0 + a.rows, a.T);
-  if (threadIdx.x == 0) s_n = 0;
-  __syncthreads();
   // the cache block of a token; -1: none (padding, or a slot that the cache does not have)
   auto block_of = [&](int t) {
     const int s = a.slots[t];
     if (s < 0) return -1;
-    const int id = s / a.block;
+    const int id = static_cast<int>(static_cast<uint32_t>(s) / static_cast<uint32_t>(a.block));
     return id < a.blocks ? id : -1;
   };
-  for (int t = r0 + threadIdx.x; t < r1; t += kAppendThreads) {
-    const int id = block_of(t);
-    if (id < 0 || (t > 0 && block_of(t - 1) == id)) continue;
-    s_first[atomicAdd(&s_n, 1)] = t;  // the order of the runs does not matter: each is a block of its own
-  }
-  __syncthreads();
-  const int runs = s_n;
-  auto length = [&](int t) {  // tokens of the run that begins at t; whole warps call it
-    const int id = block_of(t);
-    int n = 1;
-    while (true) {
-      const int u = t + n + lane;
-      const unsigned same = __ballot_sync(0xffffffffu, u < a.T && n + lane < a.block && block_of(u) == id);
-      n += __ffs(~same) ? __ffs(~same) - 1 : 32;
-      if (same != 0xffffffffu) return n;
-    }
-  };
-  for (int i = 0; i < runs; ++i) {
-    const int t0 = s_first[i], n = length(t0);
-    for (int k = 0; k < a.turns; ++k) {
-      const int pair = (blockIdx.y * a.turns + k) * kTeams + team;
-      if (pair < 2 * a.Hkv) append_run<FMT, D, NT>(a, pair & 1, pair >> 1, t0, n, team, me, s_red + team * (NT / 32));
+  // Every warp looks for the runs itself: they are few, and nothing has to be waited for.
+  for (int base = r0; base < r1; base += 32) {
+    const int mine = base + lane < r1 ? block_of(base + lane) : -1;
+    const int before = base + lane < r1 && base + lane > 0 ? block_of(base + lane - 1) : -1;
+    unsigned heads = __ballot_sync(0xffffffffu, mine >= 0 && mine != before);
+    while (heads) {
+      const int at = __ffs(heads) - 1;
+      heads &= heads - 1;
+      const int t0 = base + at, id = __shfl_sync(0xffffffffu, mine, at);
+      int n = 1;
+      while (true) {
+        const int u = t0 + n + lane;
+        const unsigned same = __ballot_sync(0xffffffffu, u < a.T && n + lane < a.block && block_of(u) == id);
+        n += same == 0xffffffffu ? 32 : __ffs(~same) - 1;
+        if (same != 0xffffffffu) break;
+      }
+      for (int k = 0; k < a.turns; ++k) {
+        const int pair = (blockIdx.y * a.turns + k) * kTeams + team;
+        if (pair < 2 * a.Hkv) append_run<FMT, D, NT>(a, pair & 1, pair >> 1, t0, n, team, me, s_red + team * (NT / 32));
+      }
     }
   }
 }

@@ -4,15 +4,16 @@
 //   x -= frequency * count;  x -= presence                for the ids generated `count` > 0 times
 //   x += bias;  -inf where the mask's bit is 0
 //
-// A block of threads owns a range of one row's ids. It scans the row's history (a few thousand ids, from L2), counts those
-// of its range in shared memory, and turns the counts, with the bias row, into one number to add and one bit (penalised or
-// not) per id. Then it reads and writes each logit once, 16 bytes at a time. That needs no count tables in memory, no sort
-// and no second launch. Counts are integers, so the order of the atomics does not matter. The bias goes through shared
-// memory because a thread's eight ids are not on a 16-byte boundary of its row: read next to the logits, eight numbers apart
-// from lane to lane, it kept L1 busy for 79% of the time. Bound by HBM for many rows, by latency for one.
+// A block of threads owns a range of one row's ids and keeps their counts in shared memory: it scans the row's history
+// (a few thousand ids, from L2) and counts those of its range, then reads and writes each logit once, 16 bytes at a
+// time (at most two pieces per thread, fetched before the history). That needs no count tables in memory, no sort and no
+// second launch. Counts are integers, so the order of the atomics does not matter. A thread's ids are on a 16-byte boundary of the logits, not of the bias row: it reads the two or
+// three aligned pieces that hold their biases and shifts (one by one, eight numbers apart from lane to lane, the biases kept
+// L1 busy for 79% of the time). Bound by HBM for many rows, by latency for one.
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "launch.cuh"
@@ -22,6 +23,7 @@ namespace qw {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kPieces = 2;  // 16-byte pieces of a thread
 constexpr uint32_t kPrompt = 0x80000000u;  // in the prompt; the other bits count generated occurrences
 
 template <typename T>
@@ -45,7 +47,7 @@ struct Num<__half> {
 template <typename T>
 __global__ void __launch_bounds__(kThreads) logits_kernel(LogitsArgs a, int range) {
   constexpr int VE = 16 / static_cast<int>(sizeof(T));
-  extern __shared__ __align__(16) uint32_t counts[];  // [range + 2 VE], then the bits
+  extern __shared__ __align__(16) uint32_t counts[];  // [range + 2 VE]
   griddep_wait();
   griddep_launch();
   const int row = blockIdx.y;
@@ -62,63 +64,72 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(LogitsArgs a, int rang
   const int body = wide ? min(hi, blockIdx.x ? lo : lead) : hi;  // first id of the 16-byte pieces
   // id `first` is entry 0: the pieces' entries begin on 16-byte boundaries
   const int first = lo - (VE - (body - lo) % VE) % VE;
-  uint32_t* const seen_bits = counts + range + 2 * VE;
 
+  const int pieces = (hi - body) / VE;  // at most kThreads * kPieces
+  uint4 w[kPieces];
+#pragma unroll
+  for (int k = 0; k < kPieces; ++k) {
+    const int p = threadIdx.x + k * kThreads;
+    if (p < pieces) w[k] = *reinterpret_cast<const uint4*>(src + body + p * VE);
+  }
   int bias_row = -1, mask_row = -1;
   if (a.bias) bias_row = a.bias_rows ? a.bias_rows[row] : row;
   if (a.mask) mask_row = a.mask_rows ? a.mask_rows[row] : row;
   const float* bias = bias_row >= 0 && bias_row < a.biases ? a.bias + bias_row * a.bias_stride : nullptr;
   const uint32_t* mask = mask_row >= 0 && mask_row < a.masks ? a.mask + mask_row * a.mask_stride : nullptr;
-  const bool penalised = a.history != nullptr, adds = penalised || bias;
-  float rep = 1.f;
-  if (adds) {
-    float freq = 0.f, pres = 0.f;
-    if (penalised) {
-      rep = a.repetition ? a.repetition[row] : 1.f;
-      freq = a.frequency ? a.frequency[row] : 0.f;
-      pres = a.presence ? a.presence[row] : 0.f;
-      for (int i = threadIdx.x * 4; i < hi - first; i += kThreads * 4) *reinterpret_cast<uint4*>(counts + i) = make_uint4(0, 0, 0, 0);
-      __syncthreads();
-      const int n = min(max(a.history_lens[row], 0), a.history_width);
-      const int prompt = a.prompt_lens ? a.prompt_lens[row] : 0;
-      const int* ids = a.history + row * a.history_stride;
+  const bool penalised = a.history != nullptr;
+  float rep = 1.f, freq = 0.f, pres = 0.f;
+  if (penalised) {
+    rep = a.repetition ? a.repetition[row] : 1.f;
+    freq = a.frequency ? a.frequency[row] : 0.f;
+    pres = a.presence ? a.presence[row] : 0.f;
+    const int n = min(max(a.history_lens[row], 0), a.history_width);
+    const int prompt = a.prompt_lens ? a.prompt_lens[row] : 0;
+    for (int i = threadIdx.x * 4; i < hi - first; i += kThreads * 4) *reinterpret_cast<uint4*>(counts + i) = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    const int* ids = a.history + row * a.history_stride;
 #pragma unroll 4
-      for (int i = threadIdx.x; i < n; i += kThreads) {
-        const int id = ids[i];
-        if (id >= lo && id < hi) {
-          if (i < prompt) atomicOr(&counts[id - first], kPrompt);
-          else atomicAdd(&counts[id - first], 1u);
-        }
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const int id = ids[i];
+      if (id >= lo && id < hi) {
+        if (i < prompt) atomicOr(&counts[id - first], kPrompt);
+        else atomicAdd(&counts[id - first], 1u);
       }
-      __syncthreads();
-    }
-#pragma unroll 4
-    for (int i = threadIdx.x; i < (hi - first + 31) / 32 * 32; i += kThreads) {
-      const bool there = i >= lo - first && i < hi - first;
-      const uint32_t c = penalised && there ? counts[i] : 0;
-      float add = bias && there ? bias[first + i] : 0.f;
-      const uint32_t made = c & ~kPrompt;
-      if (made) add -= static_cast<float>(made) * freq + pres;
-      if (there) counts[i] = __float_as_uint(add);
-      const uint32_t bits = __ballot_sync(0xffffffffu, c != 0);
-      if (threadIdx.x % 32 == 0) seen_bits[i / 32] = bits;
     }
     __syncthreads();
   }
 
-  auto penalty = [&](float x, bool seen) { return seen ? (x > 0.f ? x / rep : x * rep) : x; };
+  auto penalty = [&](float x, uint32_t c) {
+    if (!c) return x;
+    x = x > 0.f ? x / rep : x * rep;
+    const uint32_t made = c & ~kPrompt;
+    return made ? x - static_cast<float>(made) * freq - pres : x;
+  };
   auto one = [&](float x, int id) {
-    const int i = id - first;
-    if (adds) x = penalty(x, (seen_bits[i >> 5] >> (i & 31)) & 1u) + __uint_as_float(counts[i]);
+    if (penalised) x = penalty(x, counts[id - first]);
+    if (bias) x += bias[id];
     return !mask || ((mask[id >> 5] >> (id & 31)) & 1u) ? x : -INFINITY;
   };
-  const int pieces = (hi - body) / VE;
   for (int i = lo + threadIdx.x; i < body; i += kThreads) dst[i] = Num<T>::put(one(Num<T>::get(src[i]), i));
-#pragma unroll 4
-  for (int p = threadIdx.x; p < pieces; p += kThreads) {
+  // numbers from an aligned piece of the bias row's memory to the bias of a thread's first id
+  const int shift = bias ? static_cast<int>((reinterpret_cast<uintptr_t>(bias + body) & 15) / 4) : 0;
+  auto biased = [&](auto by, float* x, const float* b) {
+    constexpr int S = decltype(by)::value;
+    float f[VE + 4];
+#pragma unroll
+    for (int i = 0; i < VE + (S ? 4 : 0); i += 4) {  // each holds at least one of the VE biases
+      const float4 y = __ldg(reinterpret_cast<const float4*>(b - S + i));
+      f[i] = y.x; f[i + 1] = y.y; f[i + 2] = y.z; f[i + 3] = y.w;
+    }
+#pragma unroll
+    for (int e = 0; e < VE; ++e) x[e] += f[e + S];
+  };
+#pragma unroll
+  for (int k = 0; k < kPieces; ++k) {
+    const int p = threadIdx.x + k * kThreads;
+    if (p >= pieces) break;
     const int id = body + p * VE;
-    uint4 w = *reinterpret_cast<const uint4*>(src + id);
-    T* v = reinterpret_cast<T*>(&w);
+    T* v = reinterpret_cast<T*>(&w[k]);
     uint32_t allowed = 0xffffffffu;
     if (mask) {
       const int at = id >> 5, sh = id & 31;
@@ -128,35 +139,42 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(LogitsArgs a, int rang
     float x[VE];
 #pragma unroll
     for (int e = 0; e < VE; ++e) x[e] = Num<T>::get(v[e]);
-    if (adds) {
-      const int i = id - first;
-      const uint32_t seen = seen_bits[i >> 5] >> (i & 31);  // VE divides 32 and i
-      if (seen & ((1u << VE) - 1)) {
-#pragma unroll
-        for (int e = 0; e < VE; ++e) x[e] = penalty(x[e], (seen >> e) & 1u);
-      }
+    if (penalised) {
+      uint32_t c[VE], any = 0;
 #pragma unroll
       for (int e = 0; e < VE; e += 4) {
-        const float4 add = *reinterpret_cast<const float4*>(counts + i + e);
-        x[e] += add.x; x[e + 1] += add.y; x[e + 2] += add.z; x[e + 3] += add.w;
+        const uint4 y = *reinterpret_cast<const uint4*>(counts + id - first + e);
+        c[e] = y.x; c[e + 1] = y.y; c[e + 2] = y.z; c[e + 3] = y.w;
+        any |= y.x | y.y | y.z | y.w;
       }
+      if (any) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) x[e] = penalty(x[e], c[e]);
+      }
+    }
+    if (bias) {
+      if (shift == 0) biased(std::integral_constant<int, 0>{}, x, bias + id);
+      else if (shift == 1) biased(std::integral_constant<int, 1>{}, x, bias + id);
+      else if (shift == 2) biased(std::integral_constant<int, 2>{}, x, bias + id);
+      else biased(std::integral_constant<int, 3>{}, x, bias + id);
     }
 #pragma unroll
     for (int e = 0; e < VE; ++e) v[e] = Num<T>::put((allowed >> e) & 1u ? x[e] : -INFINITY);
-    *reinterpret_cast<uint4*>(dst + id) = w;
+    *reinterpret_cast<uint4*>(dst + id) = w[k];
   }
   for (int i = body + pieces * VE + threadIdx.x; i < hi; i += kThreads) dst[i] = Num<T>::put(one(Num<T>::get(src[i]), i));
 }
 
 template <typename T>
 void launch(const LogitsArgs& a, cudaStream_t stream) {
-  // one row: short ranges, so that all SMs share it; many rows: 8192 ids (32 KB of counts, six blocks on an SM), so that
-  // the history is scanned few times
-  int range = 8192;
-  while (range > 1024 && static_cast<int64_t>(a.rows) * ((a.vocab + range - 1) / range) < 296) range /= 2;
+  // equal ranges of at most two pieces per thread, of one where that leaves SMs without work
   constexpr int VE = 16 / static_cast<int>(sizeof(T));
-  const dim3 grid((a.vocab + range - 1) / range + 1, a.rows);  // the ids before the first boundary can shift the last range
-  const size_t smem = a.history || a.bias ? (range + 2 * VE + range / 32 + 2) * sizeof(uint32_t) : 0;
+  int most = kThreads * kPieces * VE;
+  if (static_cast<int64_t>(a.rows) * ((a.vocab + most - 1) / most) < 148) most /= 2;
+  const int ranges = (a.vocab + most - 1) / most;
+  const int range = ((a.vocab + ranges - 1) / ranges + 32 * VE - 1) / (32 * VE) * (32 * VE);
+  const dim3 grid(ranges, a.rows);  // the ids before the first boundary come on top of the first range
+  const size_t smem = a.history ? (range + 2 * VE + 4) * sizeof(uint32_t) : 0;
   launch_pdl(logits_kernel<T>, grid, dim3(kThreads), smem, stream, "process_logits", a, range);
 }
 
