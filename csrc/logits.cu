@@ -24,6 +24,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kPieces = 2;  // 16-byte pieces of a thread
+constexpr int kEarly = 4;   // ids of the history that a thread fetches before it knows how many there are
 constexpr uint32_t kPrompt = 0x80000000u;  // in the prompt; the other bits count generated occurrences
 
 template <typename T>
@@ -65,6 +66,12 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(LogitsArgs a, int rang
   // id `first` is entry 0: the pieces' entries begin on 16-byte boundaries
   const int first = lo - (VE - (body - lo) % VE) % VE;
 
+  // Everything that depends on nothing else is read first: a block of threads lives for a few memory latencies.
+  const bool penalised = a.history != nullptr;
+  int bias_row = -1, mask_row = -1, used = 0, prompt = 0;
+  float rep = 1.f, freq = 0.f, pres = 0.f;
+  if (a.bias) bias_row = a.bias_rows ? a.bias_rows[row] : row;
+  if (a.mask) mask_row = a.mask_rows ? a.mask_rows[row] : row;
   const int pieces = (hi - body) / VE;  // at most kThreads * kPieces
   uint4 w[kPieces];
 #pragma unroll
@@ -72,30 +79,41 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(LogitsArgs a, int rang
     const int p = threadIdx.x + k * kThreads;
     if (p < pieces) w[k] = *reinterpret_cast<const uint4*>(src + body + p * VE);
   }
-  int bias_row = -1, mask_row = -1;
-  if (a.bias) bias_row = a.bias_rows ? a.bias_rows[row] : row;
-  if (a.mask) mask_row = a.mask_rows ? a.mask_rows[row] : row;
-  const float* bias = bias_row >= 0 && bias_row < a.biases ? a.bias + bias_row * a.bias_stride : nullptr;
-  const uint32_t* mask = mask_row >= 0 && mask_row < a.masks ? a.mask + mask_row * a.mask_stride : nullptr;
-  const bool penalised = a.history != nullptr;
-  float rep = 1.f, freq = 0.f, pres = 0.f;
+  const int* ids = a.history + (penalised ? row * a.history_stride : 0);
+  int early[kEarly];
   if (penalised) {
+    used = min(max(a.history_lens[row], 0), a.history_width);
+    prompt = a.prompt_lens ? a.prompt_lens[row] : 0;
     rep = a.repetition ? a.repetition[row] : 1.f;
     freq = a.frequency ? a.frequency[row] : 0.f;
     pres = a.presence ? a.presence[row] : 0.f;
-    const int n = min(max(a.history_lens[row], 0), a.history_width);
-    const int prompt = a.prompt_lens ? a.prompt_lens[row] : 0;
+#pragma unroll
+    for (int k = 0; k < kEarly; ++k) {
+      const int i = threadIdx.x + k * kThreads;
+      early[k] = i < a.history_width ? ids[i] : -1;
+    }
     for (int i = threadIdx.x * 4; i < hi - first; i += kThreads * 4) *reinterpret_cast<uint4*>(counts + i) = make_uint4(0, 0, 0, 0);
+  }
+  const float* bias = bias_row >= 0 && bias_row < a.biases ? a.bias + bias_row * a.bias_stride : nullptr;
+  const uint32_t* mask = mask_row >= 0 && mask_row < a.masks ? a.mask + mask_row * a.mask_stride : nullptr;
+#pragma unroll
+  for (int k = 0; k < kPieces; ++k) {
+    const int id = body + (threadIdx.x + k * kThreads) * VE;
+    if (id < hi && bias) asm volatile("prefetch.global.L1 [%0];" ::"l"(bias + id));
+    if (id < hi && mask) asm volatile("prefetch.global.L1 [%0];" ::"l"(mask + (id >> 5)));
+  }
+  if (penalised) {
     __syncthreads();
-    const int* ids = a.history + row * a.history_stride;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const int id = ids[i];
-      if (id >= lo && id < hi) {
+    auto count = [&](int i, int id) {
+      if (i < used && id >= lo && id < hi) {
         if (i < prompt) atomicOr(&counts[id - first], kPrompt);
         else atomicAdd(&counts[id - first], 1u);
       }
-    }
+    };
+#pragma unroll
+    for (int k = 0; k < kEarly; ++k) count(threadIdx.x + k * kThreads, early[k]);
+#pragma unroll 4
+    for (int i = threadIdx.x + kEarly * kThreads; i < used; i += kThreads) count(i, ids[i]);
     __syncthreads();
   }
 
