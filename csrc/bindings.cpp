@@ -785,9 +785,18 @@ std::vector<Tensor> plan_blocks(Tensor cached_lens, Tensor new_lens, Tensor stat
   TORCH_CHECK(tokens >= 0 && tokens < (int64_t{1} << 30), "plan_blocks: bad token count ", num(tokens));
   TORCH_CHECK(free_blocks.numel() * block < (int64_t{1} << 31), "plan_blocks: slots must fit 32 bits");
   c10::cuda::CUDAGuard g(dev);
-  const auto opt = cached_lens.options();
-  auto query_start = torch::empty({B + 1}, opt), context = torch::empty({B}, opt), positions = torch::empty({tokens}, opt),
-       slots = torch::empty({tokens}, opt), state_out = torch::empty({B + 1}, opt), missing = torch::empty({1}, opt);
+  // one allocation for the six results: an allocation takes about as long on the host as the kernel on the device
+  const int64_t sizes[6] = {B + 1, B, tokens, tokens, B + 1, 1};
+  int64_t total = 0;
+  for (int64_t n : sizes) total += (n + 3) / 4 * 4;
+  const auto all = torch::empty({total}, cached_lens.options());
+  int64_t at = 0;
+  auto part = [&](int i) {
+    auto t = all.as_strided({sizes[i]}, {1}, at);
+    at += (sizes[i] + 3) / 4 * 4;
+    return t;
+  };
+  auto query_start = part(0), context = part(1), positions = part(2), slots = part(3), state_out = part(4), missing = part(5);
   qw::plan_blocks(cached_lens.data_ptr<int>(), new_lens.data_ptr<int>(), state.data_ptr<int>(), table.data_ptr<int>(),
                   table.stride(0), free_blocks.data_ptr<int>(), static_cast<int>(free_blocks.numel()), static_cast<int>(B),
                   static_cast<int>(table.size(1)), static_cast<int>(block), static_cast<int>(tokens),

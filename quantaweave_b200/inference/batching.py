@@ -12,6 +12,11 @@ and its decoder is batch-1 (``src/fast_decode.py:86-379``). Here the decoder's `
 
 Requests therefore join and leave between steps without waiting for each other, and a step costs the same whether
 one or ``max_batch`` requests are active.
+
+With a block-wise cache (``FastDecoder(kv_cache="fp8")``) the slots share a pool of blocks: a request is admitted when the
+blocks of its prompt and budget fit beside those promised to the others, idle slots hold none, and a retired request's
+return to the pool. Penalties and grammar masks (``GenerationRequest``) are applied to the step's logits on the device in one
+pass (``ops.logits``).
 """
 
 from __future__ import annotations
@@ -37,11 +42,19 @@ class GenerationRequest:
     stop_ids: tuple = ()
     on_token: Optional[Callable[[int], None]] = None
     logit_bias: Optional[torch.Tensor] = None  # added to the logits before sampling (e.g. -inf on invalid ids)
+    repetition_penalty: float = 1.0  # positive logits of ids seen (prompt and generated) divided by it, others multiplied
+    frequency_penalty: float = 0.0   # subtracted per occurrence among the generated ids
+    presence_penalty: float = 0.0    # subtracted once for each generated id
+    allowed: Optional[Callable[[list], torch.Tensor]] = None  # generated ids -> bool [vocab]: what a grammar lets follow
     cancelled: bool = False  # set (e.g. by ``on_token`` on a text stop string) to retire the request after this token
     # results
     tokens: list = field(default_factory=list)
     finish_reason: Optional[str] = None
     done: threading.Event = field(default_factory=threading.Event)
+
+    @property
+    def penalised(self) -> bool:
+        return self.repetition_penalty != 1.0 or self.frequency_penalty != 0.0 or self.presence_penalty != 0.0
 
     def wait(self, timeout: Optional[float] = None) -> list:
         if not self.done.wait(timeout):
@@ -63,6 +76,10 @@ class ContinuousBatcher:
         self._position = [0] * self.slots
         self._next_token = [0] * self.slots
         self._generators: dict[int, torch.Generator] = {}
+        # block-wise cache: blocks promised to each slot's request, and slots whose last request ended in an error and may
+        # still hold blocks
+        self._blocks = [0] * self.slots
+        self._unreleased: set = set()
         self.steps = 0
 
     # ---- queue --------------------------------------------------------------------------------------------
@@ -74,9 +91,18 @@ class ContinuousBatcher:
         if len(request.prompt) + request.max_new > self.decoder.capacity:
             raise ValueError(f"prompt ({len(request.prompt)}) + max_new ({request.max_new}) exceed the decoder "
                              f"context {self.decoder.capacity}")
+        if request.repetition_penalty <= 0:
+            raise ValueError("repetition_penalty must be positive")
+        cache = self.decoder.cache
+        if cache is not None and self._blocks_of(request) > cache.blocks:
+            raise ValueError(f"prompt ({len(request.prompt)}) + max_new ({request.max_new}) need {self._blocks_of(request)} "
+                             f"cache blocks, the pool has {cache.blocks}")
         with self.lock:
             self.waiting.append(request)
         return request
+
+    def _blocks_of(self, request: GenerationRequest) -> int:
+        return self.decoder.cache.blocks_for(len(request.prompt) + request.max_new)
 
     def withdraw(self, request: GenerationRequest) -> bool:
         """Take a request that has not reached a slot yet back out of the queue; False once it is decoding."""
@@ -95,18 +121,29 @@ class ContinuousBatcher:
 
     # ---- scheduling ---------------------------------------------------------------------------------------
     def _admit(self) -> None:
+        if self._unreleased:
+            if self.decoder.cache is not None:
+                self.decoder.cache.release_rows(sorted(self._unreleased - set(self.active)))
+            self._unreleased.clear()
         while True:
             with self.lock:
                 free = [s for s in range(self.slots) if s not in self.active]
                 if not free or not self.waiting:
                     return
+                if self.decoder.cache is not None:
+                    promised = sum(self._blocks[s] for s in self.active)
+                    if promised + self._blocks_of(self.waiting[0]) > self.decoder.cache.blocks:
+                        return  # the next in line waits for blocks, and the others behind it
                 request = self.waiting.popleft()
             slot = free[0]
+            if self.decoder.cache is not None:
+                self._blocks[slot] = self._blocks_of(request)
             prompt = list(request.prompt)
             try:
                 self.decoder._prefill(torch.tensor([prompt[:-1]], dtype=torch.long), first_row=slot)
             except BaseException as exc:
                 # the request left the queue but never reached a slot: finish it here so its waiter returns
+                self._unreleased.add(slot)
                 request.finish_reason = f"error: {exc}"
                 request.done.set()
                 raise
@@ -115,6 +152,30 @@ class ContinuousBatcher:
             self._generators[slot] = torch.Generator().manual_seed(request.seed)
             with self.lock:
                 self.active[slot] = request
+
+    def _processed(self, logits: torch.Tensor, rows: list) -> torch.Tensor:
+        """Penalties and grammar masks of the active rows' requests, in one pass on the logits' device."""
+        requests = [self.active[s] for s in rows]
+        if not any(r.penalised or r.allowed is not None for r in requests):
+            return logits
+        from ..ops.logits import pack_mask, process_logits
+
+        dev, kw = logits.device, {}
+        if any(r.penalised for r in requests):
+            seen = [list(r.prompt) + r.tokens for r in requests]
+            length = max(len(ids) for ids in seen)
+            history = torch.tensor([ids + [0] * (length - len(ids)) for ids in seen], dtype=torch.int32)
+            lens = torch.tensor([[len(ids) for ids in seen], [len(r.prompt) for r in requests]], dtype=torch.int32).to(dev)
+            penalties = torch.tensor([[r.repetition_penalty for r in requests], [r.frequency_penalty for r in requests],
+                                      [r.presence_penalty for r in requests]]).to(dev)
+            kw.update(history=history.to(dev), history_lens=lens[0], prompt_lens=lens[1], repetition=penalties[0],
+                      frequency=penalties[1], presence=penalties[2])
+        masks = [r.allowed(r.tokens) for r in requests if r.allowed is not None]
+        if masks:
+            which = iter(range(len(masks)))
+            kw.update(mask=pack_mask(torch.stack([m.cpu() for m in masks])).to(dev),
+                      mask_rows=torch.tensor([-1 if r.allowed is None else next(which) for r in requests], dtype=torch.int32).to(dev))
+        return process_logits(logits, **kw)
 
     def _sample(self, logits: torch.Tensor, request: GenerationRequest, generator: torch.Generator) -> int:
         if request.logit_bias is not None:
@@ -133,10 +194,16 @@ class ContinuousBatcher:
         if not rows:
             return 0
         dev = self.decoder.device
-        tokens = torch.tensor([self._next_token[s] if s in rows else 0 for s in range(self.slots)], device=dev)
         positions = torch.tensor([self._position[s] if s in rows else 0 for s in range(self.slots)],
                                  dtype=torch.int32, device=dev)
-        logits = self.decoder.run_step(tokens, positions)[rows].float().cpu()
+        if self.decoder.cache is not None:  # the active rows only, in slot order; idle slots have no token
+            tokens = [self._next_token[s] for s in rows] + [0] * (self.slots - len(rows))
+            new = torch.tensor([int(s in rows) for s in range(self.slots)], dtype=torch.int32, device=dev)
+            logits = self.decoder.run_step(torch.tensor(tokens, device=dev), positions, new)[: len(rows)]
+        else:
+            tokens = torch.tensor([self._next_token[s] if s in rows else 0 for s in range(self.slots)], device=dev)
+            logits = self.decoder.run_step(tokens, positions)[rows]
+        logits = self._processed(logits.float(), rows).cpu()
         self.steps += 1
         for i, slot in enumerate(rows):
             request = self.active[slot]
@@ -155,6 +222,8 @@ class ContinuousBatcher:
                 request.finish_reason = reason
                 with self.lock:
                     del self.active[slot]
+                if self.decoder.cache is not None:
+                    self.decoder.cache.release_rows([slot])
                 request.done.set()
         with self.lock:
             return len(self.active)
@@ -197,6 +266,7 @@ class BatchingWorker:
     def _fail_all(self, reason: str) -> None:
         with self.batcher.lock:
             stuck = list(self.batcher.active.values()) + list(self.batcher.waiting)
+            self.batcher._unreleased.update(self.batcher.active)
             self.batcher.active.clear()
             self.batcher.waiting.clear()
         for request in stuck:

@@ -17,6 +17,10 @@ B200 design:
   launched with programmatic dependent launch so the next kernel's weight prefetch overlaps the previous one;
 * prefill runs the training kernels (tcgen05 GEMMs, flash attention, grouped SwiGLU) over the prompt.
 
+``kv_cache="fp8"`` or ``"int8"`` keeps keys and values in blocks of 8 bits instead (``inference.paged_cache``): requests share
+one pool (``cache_blocks``), the step plans its own blocks on the device inside the graph, and prompts are read in pieces of
+``prefill_chunk`` tokens that attend to the cache.
+
 On CPU the same step runs as plain fp32 PyTorch (the oracle the GPU path is tested against).
 
 Expert-parallel models (the reference refuses them, ``src/fast_decode.py:89-90``) decode SPMD: every rank of the
@@ -82,7 +86,9 @@ class _Layer:
 
 class FastDecoder:
     def __init__(self, model, device: torch.device, precision: str = "auto", use_graph: Optional[bool] = None,
-                 compile: Optional[bool] = None, max_batch: int = 1, max_length: Optional[int] = None) -> None:
+                 compile: Optional[bool] = None, max_batch: int = 1, max_length: Optional[int] = None,
+                 kv_cache: str = "dense", cache_block: int = 64, cache_blocks: Optional[int] = None,
+                 prefill_chunk: int = 2048) -> None:
         from ..models.layers import Attention
 
         if not all(hasattr(model, name) for name in ("config", "blocks", "token_embedding", "lm_head")):
@@ -92,6 +98,10 @@ class FastDecoder:
             raise Unsupported("pipeline-stage models hold only some layers")
         if ep is not None and (getattr(ep, "tp_size", 1) > 1 or getattr(ep, "sequence_parallel", False)):
             raise Unsupported("tensor-parallel attention")
+        if kv_cache not in ("dense", "fp8", "int8"):
+            raise ValueError(f"kv_cache is dense, fp8 or int8, got {kv_cache!r}")
+        if prefill_chunk < 1:
+            raise ValueError("prefill_chunk must be positive")
         cfg = model.config
         self.model = model
         self.config = cfg
@@ -112,6 +122,17 @@ class FastDecoder:
         self.heads, self.kv_heads, self.head_dim = cfg.attention_heads, cfg.num_kv_heads, cfg.head_dim
         self.hidden, self.vocab = cfg.hidden_size, cfg.vocab_size
         self.layers: list[_Layer] = []
+        self.cache = None
+        self.prefill_chunk = prefill_chunk
+        if kv_cache != "dense":
+            from .paged_cache import PagedKVCache
+
+            if self.ep is not None:
+                raise Unsupported("the block-wise KV cache with expert-parallel decoding")
+            if self.native and self.head_dim not in (32, 64, 128):
+                raise Unsupported(f"the block-wise KV cache needs head_dim 32, 64 or 128, got {self.head_dim}")
+            self.cache = PagedKVCache(cfg.layers, max_batch, self.capacity, self.kv_heads, self.head_dim, self.device, kv_cache,
+                                      cache_block, cache_blocks)
         dev, dt = self.device, self.dtype
         with torch.no_grad():
             self.tok_emb = model.token_embedding.weight.detach().to(dev, dt)
@@ -135,9 +156,10 @@ class FastDecoder:
                 layer.num_experts = moe.num_experts
                 layer.ffn = moe.ffn_local
                 self._experts(layer, moe)
-                shape = (max_batch, self.kv_heads, self.capacity, self.head_dim)
-                layer.keys = torch.zeros(shape, dtype=dt, device=dev)
-                layer.values = torch.zeros(shape, dtype=dt, device=dev)
+                if self.cache is None:
+                    shape = (max_batch, self.kv_heads, self.capacity, self.head_dim)
+                    layer.keys = torch.zeros(shape, dtype=dt, device=dev)
+                    layer.values = torch.zeros(shape, dtype=dt, device=dev)
                 self.layers.append(layer)
         if cfg.position_embedding == "rope":
             from ..models.layers import rope_tables
@@ -151,6 +173,7 @@ class FastDecoder:
         # static step inputs/outputs (graph-safe)
         self.tokens_in = torch.zeros(max_batch, dtype=torch.long, device=dev)
         self.positions_in = torch.zeros(max_batch, dtype=torch.int32, device=dev)
+        self.new_in = torch.zeros(max_batch, dtype=torch.int32, device=dev)  # block-wise cache: tokens of each request
         self.logits = torch.zeros(max_batch, self.vocab, dtype=torch.float32, device=dev)
         self.noise = torch.zeros(BATCH, self.vocab, dtype=torch.float32, device=dev)
         self.sampled = torch.zeros(BATCH, max_batch, dtype=torch.long, device=dev)
@@ -244,12 +267,20 @@ class FastDecoder:
         from ..models.layers import apply_rope_reference, rope_tables, rms_norm_reference
 
         tokens, positions = self.tokens_in[:batch], self.positions_in[:batch]
+        plan = None
+        if self.cache is not None:
+            plan = self.cache.plan(self.positions_in, self.new_in, batch)
+            positions = plan.positions
         x = self._embed(tokens, positions).float()
         hq, hkv, d = self.heads, self.kv_heads, self.head_dim
         pos = positions.long()
-        for layer in self.layers:
+        for li, layer in enumerate(self.layers):
             n1 = self._apply_norm(x, layer.norm1)
             qkv = F.linear(n1, layer.wqkv.float(), layer.bqkv)
+            if plan is not None:
+                att = self._attend_paged(li, qkv, plan, 1, self.capacity)
+                x = self._after_attention(layer, x + F.linear(att, layer.wo.float(), layer.bo))
+                continue
             q = qkv[:, : hq * d].view(batch, 1, hq, d)
             k = qkv[:, hq * d:(hq + hkv) * d].view(batch, 1, hkv, d)
             v = qkv[:, (hq + hkv) * d:].view(batch, hkv, d)
@@ -264,34 +295,55 @@ class FastDecoder:
             values = layer.values[:batch].float().repeat_interleave(hq // hkv, dim=1)
             visible = (torch.arange(self.capacity, device=x.device)[None, :] <= pos[:, None]).view(batch, 1, 1, -1)
             att = F.scaled_dot_product_attention(q.transpose(1, 2), keys, values, attn_mask=visible)
-            x = x + F.linear(att.reshape(batch, hq * d), layer.wo.float(), layer.bo)
-            n2 = self._apply_norm(x, layer.norm2)
-            scores = F.linear(n2, layer.router) / layer.temperature
-            probs = scores.softmax(-1)
-            chosen = (scores + layer.bias if layer.bias is not None else probs).topk(layer.top_k, dim=-1).indices
-            weights = probs.gather(1, chosen)
-            weights = weights / weights.sum(-1, keepdim=True)
-            f = layer.ffn
-            if self.ep is not None:  # this rank's experts only; the group's partial outputs are summed below
-                local = layer.q_gu.size(0)
-                first = self.ep.rank * local
-                mine = (chosen >= first) & (chosen < first + local)
-                weights = weights * mine
-                chosen = (chosen - first).clamp(0, local - 1)
-            wgu = layer.q_gu[chosen].float()          # [B, k, 2F, H]
-            wd = layer.q_d[chosen].float()            # [B, k, H, F]
-            g = torch.einsum("bkfh,bh->bkf", wgu[:, :, :f], n2)
-            u = torch.einsum("bkfh,bh->bkf", wgu[:, :, f:], n2)
-            out = torch.einsum("bkhf,bkf->bkh", wd, F.silu(g) * u)
-            moe_out = (out * weights[..., None]).sum(1)
-            if self.ep is not None:
-                import torch.distributed as dist
-
-                dist.all_reduce(moe_out, group=self.ep.group)
-            x = x + moe_out
+            x = self._after_attention(layer, x + F.linear(att.reshape(batch, hq * d), layer.wo.float(), layer.bo))
         del rope_tables, rms_norm_reference
         x = self._apply_norm(x, self.final_norm)
         return F.linear(x, self.lm_head.float())
+
+    def _after_attention(self, layer, x: Tensor) -> Tensor:
+        """The MoE half of a layer (CPU oracle): x + experts(norm(x))."""
+        n2 = self._apply_norm(x, layer.norm2)
+        scores = F.linear(n2, layer.router) / layer.temperature
+        probs = scores.softmax(-1)
+        chosen = (scores + layer.bias if layer.bias is not None else probs).topk(layer.top_k, dim=-1).indices
+        weights = probs.gather(1, chosen)
+        weights = weights / weights.sum(-1, keepdim=True)
+        f = layer.ffn
+        if self.ep is not None:  # this rank's experts only; the group's partial outputs are summed below
+            local = layer.q_gu.size(0)
+            first = self.ep.rank * local
+            mine = (chosen >= first) & (chosen < first + local)
+            weights = weights * mine
+            chosen = (chosen - first).clamp(0, local - 1)
+        wgu = layer.q_gu[chosen].float()          # [B, k, 2F, H]
+        wd = layer.q_d[chosen].float()            # [B, k, H, F]
+        g = torch.einsum("bkfh,bh->bkf", wgu[:, :, :f], n2)
+        u = torch.einsum("bkfh,bh->bkf", wgu[:, :, f:], n2)
+        out = torch.einsum("bkhf,bkf->bkh", wd, F.silu(g) * u)
+        moe_out = (out * weights[..., None]).sum(1)
+        if self.ep is not None:
+            import torch.distributed as dist
+
+            dist.all_reduce(moe_out, group=self.ep.group)
+        return x + moe_out
+
+    def _attend_paged(self, index: int, qkv: Tensor, plan, max_query: int, max_context: int) -> Tensor:
+        """One layer's attention through the block-wise cache: rotate the rows of ``qkv``, write their keys and values, attend.
+        Returns ``[rows, heads * head_dim]``."""
+        hq, hkv, d = self.heads, self.kv_heads, self.head_dim
+        rows = qkv.size(0)
+        if not self.learned:
+            if self.native:
+                self._C.rope_apply(qkv, hq + hkv, d, 1, plan.positions, self.cos, self.sin, False)
+            else:
+                from ..models.layers import apply_rope_reference
+
+                pos = plan.positions.long()
+                turned = apply_rope_reference(qkv[:, : (hq + hkv) * d].reshape(1, rows, hq + hkv, d), self.cos[pos], self.sin[pos])
+                qkv = torch.cat([turned.reshape(rows, -1), qkv[:, (hq + hkv) * d:]], dim=1)
+        heads = qkv.view(rows, hq + 2 * hkv, d)
+        self.cache.append(index, heads[:, hq:hq + hkv], heads[:, hq + hkv:], plan)
+        return self.cache.attend(index, heads[:, :hq], plan, max_query, max_context).reshape(rows, hq * d)
 
     @staticmethod
     def _apply_norm(x: Tensor, norm) -> Tensor:
@@ -326,6 +378,10 @@ class FastDecoder:
         bf = torch.bfloat16
         chunks = C.decode_attn_chunks(self.capacity)
         tickets = self._tickets
+        plan = None
+        if self.cache is not None:  # blocks of the new tokens: in the step, so that a replayed graph takes its own
+            plan = self.cache.plan(self.positions_in, self.new_in, batch)
+            positions = plan.positions
         x = None
         pending = None  # (y, slot, top_w, k) of the previous layer's MoE, or its layer index (expert-parallel)
         if self.ep is not None:
@@ -344,12 +400,15 @@ class FastDecoder:
             qkv = torch.empty(batch, (hq + 2 * hkv) * d, device=dev, dtype=bf)
             C.grouped_gemv(n1, layer.wqkv, None, qkv.size(1), H, 0, 0, False, None, None, None, 1, batch,
                            qkv, False, layer.bqkv, None, None)
-            part_o = torch.empty(batch * hq * chunks * d, device=dev, dtype=torch.float32)
-            part_ml = torch.empty(batch * hq * chunks * 2, device=dev, dtype=torch.float32)
-            att = torch.empty(batch, hq * d, device=dev, dtype=bf)
-            # RoPE and the cache append of the new token happen inside the attention launch
-            C.decode_attention_rope(qkv, positions, self.cos, self.sin, not self.learned, layer.keys[:batch],
-                                    layer.values[:batch], hq, 1.0 / math.sqrt(d), part_o, part_ml, tickets, att)
+            if plan is not None:
+                att = self._attend_paged(li, qkv, plan, 1, self.capacity)
+            else:
+                part_o = torch.empty(batch * hq * chunks * d, device=dev, dtype=torch.float32)
+                part_ml = torch.empty(batch * hq * chunks * 2, device=dev, dtype=torch.float32)
+                att = torch.empty(batch, hq * d, device=dev, dtype=bf)
+                # RoPE and the cache append of the new token happen inside the attention launch
+                C.decode_attention_rope(qkv, positions, self.cos, self.sin, not self.learned, layer.keys[:batch],
+                                        layer.values[:batch], hq, 1.0 / math.sqrt(d), part_o, part_ml, tickets, att)
             x_new = torch.empty_like(x)  # out-projection with bias and the residual add in the GEMV epilogue
             C.grouped_gemv(att, layer.wo, None, H, hq * d, 0, 0, False, None, None, None, 1, batch, x_new,
                            False, layer.bo, x, None)
@@ -434,6 +493,9 @@ class FastDecoder:
         with torch.cuda.graph(graph):
             self.logits[:batch].copy_(self._step(batch))
         self.graph = graph
+        if self.cache is not None:
+            self.cache.clear()
+            return
         for layer in self.layers:
             layer.keys.zero_()
             layer.values.zero_()
@@ -444,7 +506,9 @@ class FastDecoder:
 
     @property
     def description(self) -> str:
-        base = "KV cache" if not self.native else "KV cache + native sm_100a kernels"
+        base = "KV cache" if self.cache is None else f"{self.cache.fmt} block-wise KV cache"
+        if self.native:
+            base += " + native sm_100a kernels"
         return base + (" + CUDA graph" if self.graph is not None else "")
 
     # ---- prefill -------------------------------------------------------------------------------------
@@ -454,16 +518,16 @@ class FastDecoder:
         ``first_row .. first_row + B - 1`` (a continuous batcher fills one slot at a time)."""
         batch, n = prompts.shape
         self.length = n
+        if self.cache is not None:
+            self.cache.release_rows(slice(first_row, first_row + batch))  # the rows begin anew
         if n == 0:
+            return
+        if self.cache is not None:
+            self._prefill_paged(prompts.to(self.device), first_row)
             return
         rows = slice(first_row, first_row + batch)
         model = self.model
-        saved = [(moe.capacity_factor, moe.drop_overflow_tokens, moe.kernel) for moe in model.moes()]
-        for moe in model.moes():
-            moe.drop_overflow_tokens = False
-            if self.ep is not None:
-                moe.kernel = "loop"  # expert-parallel prefill: the per-expert exchange path (fp32, any device)
-        try:
+        with self._no_capacity():
             hidden = model.embed(prompts.to(self.device))
             hq, hkv, d = self.heads, self.kv_heads, self.head_dim
             for block, layer in zip(model.blocks, self.layers):
@@ -488,9 +552,53 @@ class FastDecoder:
                     hidden = hidden + att.out_proj(o)
                 moe_out = block.moe(block.moe_norm(hidden))[0]
                 hidden = hidden + moe_out
+
+    @contextlib.contextmanager
+    def _no_capacity(self):
+        """The model's own modules without expert capacity, as the decoder's steps run them."""
+        moes = list(self.model.moes())
+        saved = [(moe.capacity_factor, moe.drop_overflow_tokens, moe.kernel) for moe in moes]
+        for moe in moes:
+            moe.drop_overflow_tokens = False
+            if self.ep is not None:
+                moe.kernel = "loop"  # expert-parallel prefill: the per-expert exchange path (fp32, any device)
+        try:
+            yield
         finally:
-            for moe, (cf, drop, kernel) in zip(model.moes(), saved):
+            for moe, (cf, drop, kernel) in zip(moes, saved):
                 moe.capacity_factor, moe.drop_overflow_tokens, moe.kernel = cf, drop, kernel
+
+    def _prefill_paged(self, prompts: Tensor, first_row: int) -> None:
+        """The prompts in pieces of ``prefill_chunk`` tokens: each piece's keys and values are written, then its rows attend to
+        all that the cache holds of their request."""
+        if self.native:
+            from ..ops import ext
+            from ..ops.linear import linear
+
+            self._C = ext()
+        batch, n = prompts.shape
+        lens = torch.zeros(2, self.max_batch, dtype=torch.int32)
+        with self._no_capacity():
+            for start in range(0, n, self.prefill_chunk):
+                piece = prompts[:, start:start + self.prefill_chunk]
+                m = piece.size(1)
+                lens[0, first_row:first_row + batch], lens[1, first_row:first_row + batch] = start, m
+                cached, new = lens.to(self.device)
+                plan = self.cache.plan(cached, new, batch * m)
+                hidden = self._embed(piece.reshape(-1), plan.positions).view(batch, m, self.hidden)
+                for li, block in enumerate(self.model.blocks):
+                    att = block.attention
+                    normed = block.attention_norm(hidden).reshape(batch * m, self.hidden)
+                    if self.native:
+                        qkv = linear(normed, att.in_proj_weight, att.in_proj_bias).contiguous()
+                        o = self._attend_paged(li, qkv, plan, m, start + m)
+                        hidden = linear(o, att.out_proj.weight, att.out_proj.bias,
+                                        hidden.reshape(-1, self.hidden)).view(batch, m, self.hidden)
+                    else:
+                        qkv = F.linear(normed, att.in_proj_weight, att.in_proj_bias)
+                        o = self._attend_paged(li, qkv, plan, m, start + m).to(hidden.dtype)
+                        hidden = hidden + att.out_proj(o).view(batch, m, self.hidden)
+                    hidden = hidden + block.moe(block.moe_norm(hidden))[0]
 
     def _native_attention(self, q: Tensor, k: Tensor, v: Tensor, batch: int, n: int) -> Tensor:
         """Causal flash attention over the (already rotated) prompt; q/k/v are views into the packed QKV rows."""
@@ -518,11 +626,22 @@ class FastDecoder:
 
     # ---- batched generation ------------------------------------------------------------------------------
     @torch.no_grad()
-    def run_step(self, tokens: Tensor, positions: Tensor) -> Tensor:
-        """One step for ``tokens [B]`` at ``positions [B]``; returns fp32 logits ``[B, V]`` (a reused buffer)."""
+    def run_step(self, tokens: Tensor, positions: Tensor, new: Optional[Tensor] = None) -> Tensor:
+        """One step for ``tokens [B]`` at ``positions [B]``; returns fp32 logits ``[B, V]`` (a reused buffer).
+
+        With the block-wise cache ``new [max_batch]`` (0 or 1) may leave requests out: ``positions`` is then ``[max_batch]``, and
+        ``tokens [max_batch]`` holds the tokens of the others in order, padded at the end; so are the logits."""
         batch = tokens.numel()
         self.tokens_in[:batch].copy_(tokens)
-        self.positions_in[:batch].copy_(positions.to(torch.int32))
+        if self.cache is not None:
+            self.new_in.zero_()
+            if new is None:
+                self.new_in[:batch] = 1
+            else:
+                self.new_in.copy_(new.to(torch.int32))
+        elif new is not None:
+            raise ValueError("only the block-wise KV cache leaves requests out of a step")
+        self.positions_in[:positions.numel()].copy_(positions.to(torch.int32))
         if self.graph is not None and batch == self.max_batch:
             self.graph.replay()
         else:

@@ -57,6 +57,14 @@ class GenerateRequest(BaseModel):
     top_p: float = Field(1.0, gt=0, le=1)
     seed: Optional[int] = None
     stop: list[str] = Field(default_factory=list)
+    # with --batching only
+    repetition_penalty: float = Field(1.0, gt=0)
+    frequency_penalty: float = 0.0
+    presence_penalty: float = 0.0
+
+    @property
+    def penalised(self) -> bool:
+        return (self.repetition_penalty, self.frequency_penalty, self.presence_penalty) != (1.0, 0.0, 0.0)
 
 
 class ChatMessage(BaseModel):
@@ -200,7 +208,7 @@ class Server:
                  api_key: Optional[str] = None, rate_limit: Optional[int] = None, rate_limit_window: float = 60.0,
                  request_timeout: Optional[float] = None, max_queue: Optional[int] = None,
                  moderation_patterns: Optional[Path] = None, sessions: Optional[tuple] = None,
-                 batching: int = 0) -> None:
+                 batching: int = 0, kv_cache: str = "dense", cache_blocks: Optional[int] = None) -> None:
         from ..utils.hardware import choose_precision, detect
 
         self.checkpoint, self.adapter, self.device = checkpoint, adapter, device
@@ -227,7 +235,8 @@ class Server:
             from ..inference.fast_decode import FastDecoder
 
             model = self.complete_session.model
-            self.batch_decoder = FastDecoder(model, device, self.precision, max_batch=batching)
+            self.batch_decoder = FastDecoder(model, device, self.precision, max_batch=batching, kv_cache=kv_cache,
+                                             cache_blocks=cache_blocks)
             self.worker = BatchingWorker(ContinuousBatcher(self.batch_decoder))
 
     def close(self) -> None:
@@ -269,7 +278,8 @@ class Server:
         state = {"generated": [], "text": "", "emitted": 0, "reason": "length"}
         seed = request.seed if request.seed is not None else random.randrange(1 << 31)
         job = GenerationRequest(ids, budget, request.temperature, request.top_k, request.top_p, seed,
-                                stop_ids=(tok.eos_id,), logit_bias=bias)
+                                stop_ids=(tok.eos_id,), logit_bias=bias, repetition_penalty=request.repetition_penalty,
+                                frequency_penalty=request.frequency_penalty, presence_penalty=request.presence_penalty)
 
         def on_token(token: int) -> None:
             if token == tok.eos_id:
@@ -321,7 +331,8 @@ class Server:
                 "uptime_seconds": time.time() - self.started_at, "requests_served": self.requests_served,
                 "auth_required": self.api_key is not None, "rate_limit": self.rate_limiter.limit,
                 "request_timeout": self.request_timeout, "max_queue": self.max_queue,
-                "batching_slots": self.worker.batcher.slots if self.worker is not None else 0}
+                "batching_slots": self.worker.batcher.slots if self.worker is not None else 0,
+                "batching_cache": self.batch_decoder.description if self.worker is not None else None}
 
     async def _acquire(self) -> None:
         """Take the generation lock. A request that finds it free always proceeds (even ``max_queue=0``); one that
@@ -357,8 +368,15 @@ class Server:
         return Settings(mode="complete", tokens=r.tokens, temperature=r.temperature, top_k=r.top_k, top_p=r.top_p,
                         seed=r.seed, stop=r.stop)
 
+    def _check_penalties(self, request: GenerateRequest) -> None:
+        if request.penalised and self.worker is None:
+            from fastapi import HTTPException
+
+            raise HTTPException(422, "repetition, frequency and presence penalties need a server started with --batching")
+
     async def generate(self, request: GenerateRequest) -> dict:
         self._check(request.prompt, "prompt")
+        self._check_penalties(request)
         if self.worker is not None:
             self._admit_batched()
             payload = await asyncio.to_thread(self._batched, request)
@@ -452,6 +470,7 @@ class Server:
         """Server-sent events: ``data: {"text": ...}`` per piece, then ``event: done`` with the full reply. With the
         batching worker the request joins the shared decode; otherwise it holds the session lock while it streams."""
         self._check(request.prompt, "prompt")
+        self._check_penalties(request)
         if self.worker is not None:
             self._admit_batched()
             handle: list = []
@@ -563,6 +582,10 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--batching", type=int, default=0, metavar="N",
                    help="continuous batching of /generate and /generate/stream over N decoder slots (0 = one "
                         "request at a time)")
+    p.add_argument("--kv-cache", choices=("dense", "fp8", "int8"), default="dense",
+                   help="with --batching: fp8 or int8 keep keys and values in blocks of 8 bits that the slots share")
+    p.add_argument("--cache-blocks", type=int, metavar="N",
+                   help="blocks of 64 tokens in that pool (default: enough for every slot's full context)")
     h = p.add_argument_group("hardening")
     h.add_argument("--api-key", help="require this key (Authorization: Bearer or X-API-Key) on every route but /health")
     h.add_argument("--rate-limit", type=int, help="429 past this many requests per --rate-limit-window per caller")
@@ -587,7 +610,8 @@ def main(argv=None) -> None:
     server = Server(checkpoint, adapter, device, args.precision, use_cache=not args.no_cache, api_key=args.api_key,
                     rate_limit=args.rate_limit, rate_limit_window=args.rate_limit_window,
                     request_timeout=args.request_timeout, max_queue=args.max_queue,
-                    moderation_patterns=args.moderation_blocklist, batching=args.batching)
+                    moderation_patterns=args.moderation_blocklist, batching=args.batching, kv_cache=args.kv_cache,
+                    cache_blocks=args.cache_blocks)
     print(f"model: {checkpoint}" + (f" + adapter {adapter}" if adapter else "")
           + f"  device: {device}  decoding: {server.complete_session.cache_note}")
     if server.api_key is None:
