@@ -208,8 +208,10 @@ __global__ void __launch_bounds__(kThreads, Layout<D, ROWS>::kPerSm) cached_attn
 
   // ---- the range of this block of threads, and the request that it begins in
   if (warp == 0) {
-    int64_t total = 0;
-    for (int b = lane; b < p.B; b += 32) total += work_of(p, b, R);
+    // the first 32 requests stay in registers between the two passes
+    const int64_t mine = lane < p.B ? work_of(p, lane, R) : 0;
+    int64_t total = mine;
+    for (int b = lane + 32; b < p.B; b += 32) total += work_of(p, b, R);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     const int64_t workers = min(static_cast<int64_t>(gridDim.x), total);
@@ -219,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D, ROWS>::kPerSm) cached_attn
     if (lane == 0) s_find[0] = total;
     for (int b0 = 0; b0 < p.B && (publish || before <= begin); b0 += 32) {
       const int b = b0 + lane;
-      const int64_t w = b < p.B ? work_of(p, b, R) : 0;
+      const int64_t w = b0 == 0 ? mine : b < p.B ? work_of(p, b, R) : 0;
       int64_t x = w;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -626,41 +628,41 @@ __global__ void __launch_bounds__(128) cached_attn_join_kernel(CachedAttn p, int
   float acc[PER];
 #pragma unroll
   for (int e = 0; e < PER; ++e) acc[e] = 0.f;
-  int lo = 0, hi = p.B;  // the last request whose start is <= tok
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.query_start[mid] <= tok) lo = mid;
-    else hi = mid;
-  }
-  const int b = lo;
+  const int b = request_of(p, tok);
   float l = 0.f;
   const NewRows fresh = p.B > 0 ? new_rows(p, b) : NewRows{0, 0};
   if (tok >= fresh.first && tok < fresh.first + fresh.n) {
-    const int64_t total = p.prefix[p.B];
+    const int64_t total = p.prefix[p.B], at0 = p.prefix[b];
     const Shape s = shape_of(p, b, R);
     if (s.units > 0) {
       const int row_all = (tok - fresh.first) * p.group + hq % p.group;
       const int h = hq / p.group, tile = row_all / R, row = row_all % R;
-      const int64_t u0 = p.prefix[b] + (static_cast<int64_t>(tile) * p.Hkv + h) * s.units;
+      const int64_t u0 = at0 + (static_cast<int64_t>(tile) * p.Hkv + h) * s.units;
       const int workers = static_cast<int>(min(static_cast<int64_t>(workers_max), total));
       const int w0 = worker_of(u0, total, workers), w1 = worker_of(u0 + s.units - 1, total, workers);
       if (w0 == w1) return;  // one range had the whole item
+      auto place = [&](int w) { return (2 * static_cast<int64_t>(w) + (w == w0)) * R + row; };
+      // each lane holds one range's maximum and sum, 32 ranges at a time
       float m = kNone;
-      for (int w = w0 + lane; w <= w1; w += 32)
-        m = fmaxf(m, p.part_ml[((2 * static_cast<int64_t>(w) + (w == w0)) * R + row) * 2]);
+      for (int w = w0 + lane; w <= w1; w += 32) m = fmaxf(m, p.part_ml[place(w) * 2]);
       m = warp_max(m);
-      {
-#pragma unroll 4
-        for (int w = w0; w <= w1; ++w) {
-          const int64_t at = (2 * static_cast<int64_t>(w) + (w == w0)) * R + row;
-          const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
-          const float f = exp2f_approx(ml.x - m);
+      for (int w32 = w0; w32 <= w1; w32 += 32) {
+        float f = 0.f;
+        if (w32 + lane <= w1) {
+          const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + place(w32 + lane) * 2);
+          f = exp2f_approx(ml.x - m);
           l += ml.y * f;
-          const float* src = p.part_o + at * D + lane * PER;
+        }
+        const int n = min(32, w1 - w32 + 1);
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) {
+          const float fi = __shfl_sync(0xffffffffu, f, i);
+          const float* src = p.part_o + place(w32 + i) * D + lane * PER;
 #pragma unroll
-          for (int e = 0; e < PER; ++e) acc[e] += src[e] * f;
+          for (int e = 0; e < PER; ++e) acc[e] += src[e] * fi;
         }
       }
+      l = warp_sum(l);
     }
   }
   const float inv = l != 0.f ? 1.f / l : 0.f;

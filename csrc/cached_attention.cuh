@@ -41,6 +41,21 @@ __device__ __forceinline__ NewRows new_rows(const CachedAttn& p, int b) {
   return {first, min(p.query_start[b + 1], p.T) - first};
 }
 
+// The request that row `tok` of q belongs to (the last one that begins at or before it), for a whole warp: the offsets are
+// read side by side, not one after another as in a binary search.
+__device__ __forceinline__ int request_of(const CachedAttn& p, int tok) {
+  const int lane = threadIdx.x % 32;
+  int n = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 128) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int b = b0 + i * 32 + lane;
+      n += __popc(__ballot_sync(0xffffffffu, b < p.B && p.query_start[b < p.B ? b : 0] <= tok));
+    }
+  }
+  return max(n - 1, 0);
+}
+
 // tcgen05 kernel for prompts (head_dim 64 and 128), `splits` parts of the keys; rows and resident blocks of threads per SM
 constexpr int prompt_rows(int D) { return D == 64 ? 128 : 256; }
 constexpr int prompt_per_sm(int D) { return D == 64 ? 2 : 1; }

@@ -703,12 +703,7 @@ __global__ void __launch_bounds__(128) cached_attn_tc_join_kernel(CachedAttn p, 
   griddep_launch();
   if (i >= static_cast<int64_t>(p.T) * p.Hkv * p.group) return;
   const int tok = static_cast<int>(i / (p.Hkv * p.group)), hq = static_cast<int>(i % (p.Hkv * p.group));
-  int lo = 0, hi = p.B;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.query_start[mid] <= tok) lo = mid;
-    else hi = mid;
-  }
+  const int lo = request_of(p, tok);
   const NewRows fresh = p.B > 0 ? new_rows(p, lo) : NewRows{0, 0};
   if (tok < fresh.first || tok >= fresh.first + fresh.n) return;  // zeroed by the attention kernel
   const int r = (tok - fresh.first) * p.group + hq % p.group;

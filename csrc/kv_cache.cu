@@ -17,31 +17,31 @@ namespace {
 constexpr int kPlanThreads = 256;
 constexpr int kPlanTokens = 1024;  // tokens of a block of threads
 
-// Exclusive sum over the block's threads; `total` gets the sum. Two barriers inside, one after.
-__device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total) {
+// Exclusive sums of two numbers (below 2^31 in all) over the block's threads; `total` gets both sums.
+struct Two {
+  int tokens, blocks;
+};
+__device__ __forceinline__ Two block_scan(Two v, uint64_t* warp_sums, Two& total) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  int x = v;
+  const uint64_t own = (static_cast<uint64_t>(static_cast<uint32_t>(v.tokens)) << 32) | static_cast<uint32_t>(v.blocks);
+  uint64_t x = own;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    const uint64_t y = __shfl_up_sync(0xffffffffu, x, o);
     if (lane >= o) x += y;
   }
   if (lane == 31) warp_sums[warp] = x;
   __syncthreads();
-  if (warp == 0) {
-    int s = lane < kPlanThreads / 32 ? warp_sums[lane] : 0;
+  uint64_t before = 0, all = 0;
 #pragma unroll
-    for (int o = 1; o < kPlanThreads / 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += y;
-    }
-    if (lane < kPlanThreads / 32) warp_sums[lane] = s;
+  for (int w = 0; w < kPlanThreads / 32; ++w) {  // eight reads of shared memory instead of a second scan and its barriers
+    const uint64_t s = warp_sums[w];
+    if (w < warp) before += s;
+    all += s;
   }
-  __syncthreads();
-  total = warp_sums[kPlanThreads / 32 - 1];
-  const int before = warp > 0 ? warp_sums[warp - 1] : 0;
-  __syncthreads();
-  return before + x - v;
+  total = {static_cast<int>(all >> 32), static_cast<int>(all & 0xffffffffu)};
+  const uint64_t at = before + x - own;
+  return {static_cast<int>(at >> 32), static_cast<int>(at & 0xffffffffu)};
 }
 
 struct PlanArgs {
@@ -61,18 +61,18 @@ struct PlanArgs {
   int* missing;
 };
 
-__device__ __forceinline__ int clamp_len(int64_t v) {
-  return static_cast<int>(v < 0 ? 0 : (v > 0x7fffffff ? 0x7fffffff : v));
-}
-
 struct Need {
-  int held, fits, wanted;
+  int cached, fresh, context;
+  int held, fits, wanted;  // blocks
 };
 
 __device__ __forceinline__ Need need_of(const PlanArgs& a, int b) {
-  const int64_t total = static_cast<int64_t>(max(a.cached[b], 0)) + max(a.fresh[b], 0);
   Need n;
-  n.wanted = static_cast<int>((total + a.block - 1) / a.block);
+  n.cached = max(a.cached[b], 0);
+  n.fresh = max(a.fresh[b], 0);
+  const uint32_t total = min(static_cast<uint32_t>(n.cached) + static_cast<uint32_t>(n.fresh), 0x7fffffffu);
+  n.context = static_cast<int>(total);
+  n.wanted = static_cast<int>((total + static_cast<uint32_t>(a.block) - 1) / static_cast<uint32_t>(a.block));
   n.fits = min(n.wanted, a.width);
   n.held = min(max(a.state[1 + b], 0), a.width);
   return n;
@@ -82,103 +82,106 @@ __device__ __forceinline__ Need need_of(const PlanArgs& a, int b) {
 // few hundred requests they cost less than a second launch. Then the work is spread over the blocks: the tokens' slots
 // and positions by ranges, the tables' new entries by requests. A token's slot in a new block comes from the free list
 // itself, not from the table, so that no block reads an entry that another one writes.
-// Bound by the latency of the dependent reads (lengths, then tables, then slots), not by its few bytes.
+// Bound by the latency of the dependent reads (lengths, then tables, then slots), not by its few bytes: what the later parts
+// need of a request is kept in shared memory.
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PlanArgs a) {
   extern __shared__ int plan_smem[];
   int* start = plan_smem;           // [B + 1]
-  int* rank = plan_smem + a.B + 1;  // [B]
-  __shared__ int sums[kPlanThreads / 32];
+  int* rank = start + a.B + 1;      // [B]
+  int* cached = rank + a.B;         // [B]
+  int* held = cached + a.B;         // [B]
+  int* fits = held + a.B;           // [B]
+  __shared__ uint64_t sums[kPlanThreads / 32];
   __shared__ int s_short[kPlanThreads / 32];
   griddep_wait();
   griddep_launch();
   const int per = (a.B + kPlanThreads - 1) / kPlanThreads;
   const int b0 = min(static_cast<int>(threadIdx.x) * per, a.B), b1 = min(b0 + per, a.B);
-  int tokens = 0, blocks = 0, narrow = 0;
+  const int free = min(max(a.state[0], 0), a.capacity);
+  Two mine{0, 0}, all;
+  int narrow = 0;
   for (int b = b0; b < b1; ++b) {
     const Need n = need_of(a, b);
-    tokens += max(a.fresh[b], 0);
-    blocks += max(n.fits - n.held, 0);
+    start[b] = n.fresh;
+    rank[b] = max(n.fits - n.held, 0);
+    cached[b] = n.cached;
+    held[b] = n.held;
+    fits[b] = n.fits;
+    if (blockIdx.x == 0) a.context[b] = n.context;
+    mine.tokens += n.fresh;
+    mine.blocks += rank[b];
     narrow += n.wanted - n.fits;
   }
-  int all_tokens, all_blocks;
-  int t = block_scan(tokens, sums, all_tokens);
-  int r = block_scan(blocks, sums, all_blocks);
+  Two at = block_scan(mine, sums, all);
   for (int b = b0; b < b1; ++b) {
-    const Need n = need_of(a, b);
-    start[b] = t;
-    rank[b] = r;
-    t += max(a.fresh[b], 0);
-    r += max(n.fits - n.held, 0);
+    const int tokens = start[b], blocks = rank[b];
+    start[b] = at.tokens;
+    rank[b] = at.blocks;
+    if (blockIdx.x == 0) {
+      a.query_start[b] = at.tokens;
+      a.state_out[1 + b] = held[b] + min(blocks, max(free - at.blocks, 0));
+    }
+    at.tokens += tokens;
+    at.blocks += blocks;
   }
-  if (threadIdx.x == 0) start[a.B] = all_tokens;
-  const int free = min(max(a.state[0], 0), a.capacity);
-  __syncthreads();
-
+  if (threadIdx.x == 0) start[a.B] = all.tokens;
   if (blockIdx.x == 0) {
-    for (int b = b0; b < b1; ++b) {
-      const Need n = need_of(a, b);
-      a.query_start[b] = start[b];
-      a.context[b] = clamp_len(static_cast<int64_t>(max(a.cached[b], 0)) + max(a.fresh[b], 0));
-      a.state_out[1 + b] = n.held + min(max(n.fits - n.held, 0), max(free - rank[b], 0));
-    }
-    int sum = narrow;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (threadIdx.x % 32 == 0) s_short[threadIdx.x / 32] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      int m = all_blocks - min(all_blocks, free);
-      for (int w = 0; w < kPlanThreads / 32; ++w) m += s_short[w];
-      a.query_start[a.B] = all_tokens;
-      a.state_out[0] = free - min(all_blocks, free);
-      a.missing[0] = m;
-    }
+    for (int o = 16; o > 0; o >>= 1) narrow += __shfl_xor_sync(0xffffffffu, narrow, o);
+    if (threadIdx.x % 32 == 0) s_short[threadIdx.x / 32] = narrow;
   }
-  // new table entries: a warp per request
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  for (int b = blockIdx.x * (kPlanThreads / 32) + warp; b < a.B; b += gridDim.x * (kPlanThreads / 32)) {
-    const Need n = need_of(a, b);
-    for (int e = n.held + lane; e < n.fits; e += 32) {
-      const int k = rank[b] + e - n.held;
-      a.table[b * a.table_stride + e] = k < free ? a.free_blocks[free - 1 - k] : -1;
-    }
+  __syncthreads();
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    int m = all.blocks - min(all.blocks, free);
+    for (int w = 0; w < kPlanThreads / 32; ++w) m += s_short[w];
+    a.query_start[a.B] = all.tokens;
+    a.state_out[0] = free - min(all.blocks, free);
+    a.missing[0] = m;
   }
   // slots and positions: kPlanTokens consecutive tokens per turn, neighbouring threads on neighbouring tokens
   for (int base = blockIdx.x * kPlanTokens; base < a.tokens; base += gridDim.x * kPlanTokens) {
-    for (int i = threadIdx.x; i < kPlanTokens && base + i < a.tokens; i += kPlanThreads) {
-      const int tok = base + i;
+#pragma unroll
+    for (int i = 0; i < kPlanTokens / kPlanThreads; ++i) {
+      const int tok = base + i * kPlanThreads + static_cast<int>(threadIdx.x);
+      if (tok >= a.tokens) break;
       int slot = -1, pos = 0;
-      if (tok < all_tokens) {
+      if (tok < all.tokens) {
         int lo = 0, hi = a.B;  // the last request whose start is <= tok
         while (hi - lo > 1) {
           const int mid = (lo + hi) >> 1;
           if (start[mid] <= tok) lo = mid;
           else hi = mid;
         }
-        const int b = lo;
-        const Need n = need_of(a, b);
-        pos = clamp_len(static_cast<int64_t>(tok - start[b]) + max(a.cached[b], 0));
-        const int e = pos / a.block;
+        const uint32_t p = min(static_cast<uint32_t>(tok - start[lo]) + static_cast<uint32_t>(cached[lo]), 0x7fffffffu);
+        const uint32_t e = p / static_cast<uint32_t>(a.block), in = p - e * a.block;
+        pos = static_cast<int>(p);
         int id = -1;
-        if (e < n.held) {
-          id = a.table[b * a.table_stride + e];
-        } else if (e < n.fits) {
-          const int k = rank[b] + e - n.held;
+        if (static_cast<int>(e) < held[lo]) {
+          id = a.table[lo * a.table_stride + e];
+        } else if (static_cast<int>(e) < fits[lo]) {
+          const int k = rank[lo] + static_cast<int>(e) - held[lo];
           if (k < free) id = a.free_blocks[free - 1 - k];
         }
-        if (id >= 0) slot = id * a.block + pos % a.block;
+        if (id >= 0) slot = id * a.block + static_cast<int>(in);
       }
       a.positions[tok] = pos;
       a.slots[tok] = slot;
     }
   }
+  // new table entries: a warp per request
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  for (int b = blockIdx.x * (kPlanThreads / 32) + warp; b < a.B; b += gridDim.x * (kPlanThreads / 32))
+    for (int e = held[b] + lane; e < fits[b]; e += 32) {
+      const int k = rank[b] + e - held[b];
+      a.table[b * a.table_stride + e] = k < free ? a.free_blocks[free - 1 - k] : -1;
+    }
 }
 
 // One block of threads: a request's entries past its kept tokens go onto the stack, requests in order.
 __global__ void __launch_bounds__(kPlanThreads) release_kernel(const int* keep, int* state, int* table,
                                                                int64_t table_stride, int* free_blocks, int capacity,
                                                                int B, int width, int block) {
-  __shared__ int sums[kPlanThreads / 32];
+  __shared__ uint64_t sums[kPlanThreads / 32];
   griddep_wait();
   griddep_launch();
   const int per = (B + kPlanThreads - 1) / kPlanThreads;
@@ -191,8 +194,8 @@ __global__ void __launch_bounds__(kPlanThreads) release_kernel(const int* keep, 
     const int held = min(max(state[1 + b], 0), width);
     n += held - kept(b, held);
   }
-  int total;
-  int at = block_scan(n, sums, total) + min(max(state[0], 0), capacity);
+  Two total;
+  int at = block_scan(Two{0, n}, sums, total).blocks + min(max(state[0], 0), capacity);
   for (int b = b0; b < b1; ++b) {
     const int held = min(max(state[1 + b], 0), width), k = kept(b, held);
     for (int e = k; e < held; ++e, ++at) {
@@ -202,7 +205,7 @@ __global__ void __launch_bounds__(kPlanThreads) release_kernel(const int* keep, 
     state[1 + b] = k;
   }
   __syncthreads();  // every thread has read state[0]
-  if (threadIdx.x == 0) state[0] = min(min(max(state[0], 0), capacity) + total, capacity);
+  if (threadIdx.x == 0) state[0] = min(min(max(state[0], 0), capacity) + total.blocks, capacity);
 }
 
 // ------------------------------------------------------------------------------------------------ append
@@ -436,7 +439,14 @@ void plan_blocks(const int* cached, const int* fresh, const int* state, int* tab
   PlanArgs a{cached, fresh, state, table, table_stride, free_blocks, capacity, B, width, block, tokens,
              query_start, context, positions, slots, state_out, missing};
   const int grid = std::min(148, std::max((tokens + kPlanTokens - 1) / kPlanTokens, (B + 63) / 64));
-  launch_pdl(plan_kernel, dim3(std::max(grid, 1)), dim3(kPlanThreads), static_cast<size_t>(2 * B + 1) * sizeof(int), stream,
+  static const bool configured = [] {
+    check_cuda(cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    static_cast<int>((5 * plan_max_requests() + 1) * sizeof(int))),
+               "plan_blocks smem");
+    return true;
+  }();
+  (void)configured;
+  launch_pdl(plan_kernel, dim3(std::max(grid, 1)), dim3(kPlanThreads), static_cast<size_t>(5 * B + 1) * sizeof(int), stream,
              "plan_blocks", a);
 }
 
