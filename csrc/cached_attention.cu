@@ -179,7 +179,7 @@ struct Walk {
   }
   // keys that a row of the piece's tile sees: [0, lim)
   __device__ __forceinline__ int lim_of(const CachedAttn& p, int row) const {
-    return min(ctx, p.context[b] - n + (row0 + min(row, rows - 1)) / p.group + 1);
+    return min(ctx, p.context[b] - n + p.by_group.quotient(row0 + min(row, rows - 1)) + 1);
   }
   __device__ __forceinline__ int key_end(const CachedAttn& p) const { return min(lim_of(p, rows - 1), (u0 + units - kLead) * kUnit); }
 };
@@ -290,8 +290,8 @@ __global__ void __launch_bounds__(kThreads, Layout<D, ROWS>::kPerSm) cached_attn
         a_j = ahead.first_key + warp * 16;
         a_end = ahead.key_end(p);
       } while (a_j >= a_end);
-      a_entry = p.table + static_cast<int64_t>(ahead.b) * p.table_stride + a_j / p.block;
-      a_in = a_j % p.block;
+      a_entry = p.table + static_cast<int64_t>(ahead.b) * p.table_stride + p.by_block.quotient(a_j);
+      a_in = p.by_block.remainder(a_j, p.by_block.quotient(a_j));
       a_k = p.k.codes + static_cast<int64_t>(ahead.h) * p.k.head_stride + k_lane;
       a_v = p.v.codes + static_cast<int64_t>(ahead.h) * p.v.head_stride + v_lane;
     }
@@ -345,7 +345,8 @@ __global__ void __launch_bounds__(kThreads, Layout<D, ROWS>::kPerSm) cached_attn
       float m = 0.f;
       if (row < rows) {
         const int r = now.row0 + row;
-        const bf16* src = p.q + static_cast<int64_t>(now.q0 + r / p.group) * p.q_token + (now.h * p.group + r % p.group) * p.q_head;
+        const int rt = p.by_group.quotient(r);
+        const bf16* src = p.q + static_cast<int64_t>(now.q0 + rt) * p.q_token + (now.h * p.group + p.by_group.remainder(r, rt)) * p.q_head;
 #pragma unroll
         for (int c = 0; c < CH; ++c)
 #pragma unroll
@@ -594,7 +595,8 @@ __global__ void __launch_bounds__(kThreads, Layout<D, ROWS>::kPerSm) cached_attn
           if (whole) {
             const float inv = m == kNone ? 0.f : 1.f / l;  // a row that sees no key is zero
             const int r = now.row0 + row;
-            bf16* dst = p.out + static_cast<int64_t>(now.q0 + r / p.group) * p.o_token + (now.h * p.group + r % p.group) * p.o_head + d;
+            const int rt = p.by_group.quotient(r);
+            bf16* dst = p.out + static_cast<int64_t>(now.q0 + rt) * p.o_token + (now.h * p.group + p.by_group.remainder(r, rt)) * p.o_head + d;
             *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
           } else {
             *reinterpret_cast<float4*>(p.part_o + (slot * R + row) * D + d) = acc;
@@ -729,7 +731,8 @@ Way way_of(int T, int B, int Hq, int Hkv, int D, int max_query, int max_context)
   w.tile = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 24 ? 24 : 32;
   int64_t slots;
   if (w.prompt) {
-    w.tiles_max = static_cast<int>(static_cast<int64_t>(T) * group / prompt_rows(D) + B);
+    const int64_t R = prompt_rows(D);  // sum of ceil(rows / R) over B requests is at most:
+    w.tiles_max = static_cast<int>(std::max<int64_t>(1, (static_cast<int64_t>(T) * group + B * (R - 1)) / R));
     // too few row tiles for the SMs: split the keys, two tiles of 128 at least for each part
     const int64_t blocks = static_cast<int64_t>(w.tiles_max) * Hkv;
     w.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(148 * prompt_per_sm(D) / std::max<int64_t>(blocks, 1), max_context / 256)));
@@ -779,6 +782,8 @@ void cached_attention(const bf16* q, int64_t q_token, int64_t q_head, bf16* out,
   p.Hkv = Hkv;
   p.group = Hq / Hkv;
   p.block = block;
+  p.by_group = Divisor(p.group);
+  p.by_block = Divisor(block);
   p.blocks = blocks;
   p.max_table_tokens = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(width) * block, 0x7fffffff));
   p.scale = scale;

@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 3 - Layout<D>::kGroups) c
   const int row0 = row_tile * kRows;
   const int rows = static_cast<int>(min(static_cast<int64_t>(kRows), static_cast<int64_t>(n) * p.group - row0));
   // keys that a row of the tile sees: [0, lim)
-  auto lim_of = [&](int row) { return min(ctx, all_ctx - n + (row0 + min(row, rows - 1)) / p.group + 1); };
+  auto lim_of = [&](int row) { return min(ctx, all_ctx - n + p.by_group.quotient(row0 + min(row, rows - 1)) + 1); };
   const int lim_all = lim_of(0), lim_any = lim_of(rows - 1);
   const int tiles = lim_any > 0 ? (lim_any + KT - 1) / KT : 0;
   const int per = (tiles + args.splits - 1) / args.splits;
@@ -264,12 +264,13 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 3 - Layout<D>::kGroups) c
     };
     auto id_of = [&](int j) {
       const int key = (t0 + j) * KT + lane * 16;
-      return lane < 8 && j < nk && key < lim_any ? __ldg(table + key / p.block) : -1;
+      return lane < 8 && j < nk && key < lim_any ? __ldg(table + p.by_block.quotient(key)) : -1;
     };
     auto groups_of = [&](int j, int id) {
       Groups x{{-1, -1}, {-1.f, 0.f}};
       if (static_cast<unsigned>(id) < static_cast<unsigned>(p.blocks)) {
-        const uint32_t in = static_cast<uint32_t>((t0 + j) * KT + lane * 16) % static_cast<uint32_t>(p.block);
+        const int key = (t0 + j) * KT + lane * 16;
+        const uint32_t in = p.by_block.remainder(key, p.by_block.quotient(key));
         const uint64_t u = static_cast<uint32_t>(id);
         x.at[0] = static_cast<int64_t>(u * p.k.block_stride + in * p.k.token_stride);
         x.at[1] = static_cast<int64_t>(u * p.v.block_stride + in * p.v.token_stride);
@@ -446,7 +447,8 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 3 - Layout<D>::kGroups) c
     const int r = g * kGroupRows + row;         // of the tile
     const int n_g = g == 0 ? n0 : n1;
     const bool real = r < rows;
-    const int tok = q0 + (row0 + r) / p.group, head = h * p.group + (row0 + r) % p.group;
+    const int row_tok = p.by_group.quotient(row0 + r);
+    const int tok = q0 + row_tok, head = h * p.group + p.by_group.remainder(row0 + r, row_tok);
     const uint32_t lane_off = static_cast<uint32_t>((warp % 4) * 32) << 16;
     const uint32_t ts = tmem + lane_off + g * KT + half * 64;
     const uint32_t to = tmem + lane_off + L::kTmemO + g * D + half * (D / 2);
@@ -467,11 +469,11 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 3 - Layout<D>::kGroups) c
       uint4 w[NI];
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        const int rr = g * kGroupRows + w16 * 16 + i * RPI + lane / LPR, rq = row0 + rr;
+        const int rr = g * kGroupRows + w16 * 16 + i * RPI + lane / LPR, rt = p.by_group.quotient(row0 + rr);
         w[i] = make_uint4(0, 0, 0, 0);
         if (rr < rows)
-          w[i] = __ldg(reinterpret_cast<const uint4*>(p.q + static_cast<int64_t>(q0 + rq / p.group) * p.q_token +
-                                                      (h * p.group + rq % p.group) * p.q_head) + c);
+          w[i] = __ldg(reinterpret_cast<const uint4*>(p.q + static_cast<int64_t>(q0 + rt) * p.q_token +
+                                                      (h * p.group + p.by_group.remainder(row0 + rr, rt)) * p.q_head) + c);
       }
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
