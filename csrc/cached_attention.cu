@@ -16,7 +16,8 @@
 //
 // The work is the list of all (request, row tile, kv head) items times their 64-key units. It is cut into equal
 // consecutive ranges, one per resident block of threads, so ragged lengths cost nothing; a range that ends inside an item
-// leaves a partial result (at most two per block), which the join kernel adds up in a fixed order.
+// leaves a partial result (at most two per block), which the join kernel adds up in a fixed order. Where there is little
+// work (cluster_parts), a cluster of blocks takes each (request, kv head) instead and adds its results up itself.
 #include <algorithm>
 #include <type_traits>
 
@@ -78,6 +79,7 @@ struct Shape {
   int units, tiles;
 };
 constexpr int kLead = 3;
+constexpr int kMaxParts = 16;  // blocks of a cluster
 __device__ __forceinline__ Shape shape_of(const CachedAttn& p, int b, int rows_per_tile) {
   const int n = new_rows(p, b).n;
   const int ctx = min(p.context[b], p.max_table_tokens);
@@ -105,6 +107,7 @@ struct Layout {
   static constexpr int kJoin = kWarps * kJoinRows * D * 4;
   static constexpr int kQ = ROWS > 16 ? ROWS / 8 * (D / 16) * 32 * 8 : 0;  // query fragments (fewer: in registers)
   static constexpr int kTotal = kRing + kJoin + kQ;
+  static constexpr int kPart = kJoinRows * (D + 2) * 4;          // a cluster's block: its result of those rows
   // blocks of threads per SM: registers and shared memory allow no more
   static constexpr int kPerSm = D == 128 ? (ROWS > 16 ? 2 : 3) : ROWS > 16 ? 3 : ROWS > 8 ? 4 : 5;
 };
@@ -145,6 +148,43 @@ __device__ __forceinline__ void lds(uint32_t* w, const uint8_t* p) {
   }
 }
 
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// shared memory of the cluster's block `rank`, at the place that this block calls `at`
+__device__ __forceinline__ float4 ld_cluster4(uint32_t at, int rank) {
+  float4 x;
+  asm volatile(
+      "{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\t"
+      "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
+      : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+      : "r"(at), "r"(rank));
+  return x;
+}
+__device__ __forceinline__ float2 ld_cluster2(uint32_t at, int rank) {
+  float2 x;
+  asm volatile(
+      "{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %2, %3;\n\t"
+      "ld.shared::cluster.v2.f32 {%0, %1}, [a];\n\t}"
+      : "=f"(x.x), "=f"(x.y)
+      : "r"(at), "r"(rank));
+  return x;
+}
+
+// Rows that belong to no request are zero.
+template <int D>
+__device__ void zero_free_rows(const CachedAttn& p) {
+  const int first = p.B > 0 ? min(max(p.query_start[0], 0), p.T) : p.T;
+  const int last = p.B > 0 ? min(max(p.query_start[p.B], first), p.T) : p.T;
+  const int64_t per = static_cast<int64_t>(p.Hkv) * p.group * (D / 8);
+  for (int64_t i = threadIdx.x; i < (first + p.T - last) * per; i += kThreads) {
+    const int r = static_cast<int>(i / per), c = static_cast<int>(i % per);
+    const int64_t tok = r < first ? r : last + (r - first);
+    *reinterpret_cast<uint4*>(p.out + tok * p.o_token + c / (D / 8) * p.o_head + (c % (D / 8)) * 8) = make_uint4(0, 0, 0, 0);
+  }
+}
+
 // Walks the pieces (one item's consecutive units) of a range.
 struct Walk {
   int64_t u, at;  // next unit; first unit of request b
@@ -170,6 +210,20 @@ struct Walk {
     first_key = max(u0 - kLead, 0) * kUnit;
     tile = item / p.Hkv;
     h = item - tile * p.Hkv;
+    rows_of<R>(p);
+  }
+  // Part `rank` of `parts` of the keys of the next row tile of (b, h). u counts the row tiles.
+  template <int R>
+  __device__ __forceinline__ void next_tile(const CachedAttn& p, int rank, int parts) {
+    tile = static_cast<int>(u++);
+    rows_of<R>(p);
+    const int all = max(shape.units - kLead, 0), from = static_cast<int>(static_cast<int64_t>(all) * rank / parts);
+    u0 = from + kLead;
+    units = static_cast<int>(static_cast<int64_t>(all) * (rank + 1) / parts) - from;
+    first_key = from * kUnit;
+  }
+  template <int R>
+  __device__ __forceinline__ void rows_of(const CachedAttn& p) {
     const NewRows fresh = new_rows(p, b);
     q0 = fresh.first;
     n = fresh.n;
@@ -184,8 +238,10 @@ struct Walk {
   __device__ __forceinline__ int key_end(const CachedAttn& p) const { return min(lim_of(p, rows - 1), (u0 + units - kLead) * kUnit); }
 };
 
-template <int FMT, int D, int ROWS>
-__global__ void __launch_bounds__(kThreads, Layout<D, ROWS>::kPerSm) cached_attn_kernel(CachedAttn p) {
+// CLUSTERS: a cluster of blocks for each (request, kv head) instead of equal ranges of all work. Its blocks share the keys and
+// add their results over distributed shared memory, without a second kernel.
+template <int FMT, int D, int ROWS, bool CLUSTERS>
+__global__ void __launch_bounds__(kThreads, Layout<D, ROWS>::kPerSm) cached_attn_kernel(CachedAttn p, int parts) {
   using L = Layout<D, ROWS>;
   constexpr int R = ROWS;                         // rows of a tile
   constexpr int N = ROWS / 8;                     // 8-row tiles of queries
@@ -205,57 +261,78 @@ __global__ void __launch_bounds__(kThreads, Layout<D, ROWS>::kPerSm) cached_attn
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int g = lane / 4, t = lane % 4;
   griddep_wait();
-
-  // ---- the range of this block of threads, and the request that it begins in
-  if (warp == 0) {
-    // the first 32 requests stay in registers between the two passes
-    const int64_t mine = lane < p.B ? work_of(p, lane, R) : 0;
-    int64_t total = mine;
-    for (int b = lane + 32; b < p.B; b += 32) total += work_of(p, b, R);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    const int64_t workers = min(static_cast<int64_t>(gridDim.x), total);
-    const int64_t begin = blockIdx.x < workers ? blockIdx.x * total / workers : total;
-    int64_t before = 0;
-    const bool publish = blockIdx.x == 0;  // the join kernel reads the prefix sums
-    if (lane == 0) s_find[0] = total;
-    for (int b0 = 0; b0 < p.B && (publish || before <= begin); b0 += 32) {
-      const int b = b0 + lane;
-      const int64_t w = b0 == 0 ? mine : b < p.B ? work_of(p, b, R) : 0;
-      int64_t x = w;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      const int64_t at = before + x - w;
-      if (w > 0 && begin >= at && begin < at + w) {
-        s_find[1] = b;
-        s_find[2] = at;
-      }
-      if (publish && b < p.B) p.prefix[b] = at;
-      before += __shfl_sync(0xffffffffu, x, 31);
+  int64_t begin = 0, end;
+  Walk ahead;
+  const int rank = CLUSTERS ? static_cast<int>(blockIdx.x) % parts : 0;
+  if constexpr (CLUSTERS) {
+    for (int i = threadIdx.x; i < D; i += kThreads) s_poison[i] = 0x7fffffff;
+    if (blockIdx.x == 0) zero_free_rows<D>(p);
+    const int item = static_cast<int>(blockIdx.x) / parts;
+    ahead.b = item / p.Hkv;
+    ahead.h = item - ahead.b * p.Hkv;
+    ahead.shape = shape_of(p, ahead.b, R);
+    end = ahead.shape.tiles;
+    __syncthreads();
+    if (end == 0) {  // the same in the whole cluster
+      griddep_launch();
+      return;
     }
-    if (publish && lane == 0) p.prefix[p.B] = total;
+  } else {
+    // ---- the range of this block of threads, and the request that it begins in
+    if (warp == 0) {
+      // the first 32 requests stay in registers between the two passes
+      const int64_t mine = lane < p.B ? work_of(p, lane, R) : 0;
+      int64_t total = mine;
+      for (int b = lane + 32; b < p.B; b += 32) total += work_of(p, b, R);
+  #pragma unroll
+      for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+      const int64_t workers = min(static_cast<int64_t>(gridDim.x), total);
+      const int64_t first = blockIdx.x < workers ? blockIdx.x * total / workers : total;
+      int64_t before = 0;
+      const bool publish = blockIdx.x == 0;  // the join kernel reads the prefix sums
+      if (lane == 0) s_find[0] = total;
+      for (int b0 = 0; b0 < p.B && (publish || before <= first); b0 += 32) {
+        const int b = b0 + lane;
+        const int64_t w = b0 == 0 ? mine : b < p.B ? work_of(p, b, R) : 0;
+        int64_t x = w;
+  #pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+          if (lane >= o) x += y;
+        }
+        const int64_t at = before + x - w;
+        if (w > 0 && first >= at && first < at + w) {
+          s_find[1] = b;
+          s_find[2] = at;
+        }
+        if (publish && b < p.B) p.prefix[b] = at;
+        before += __shfl_sync(0xffffffffu, x, 31);
+      }
+      if (publish && lane == 0) p.prefix[p.B] = total;
+    }
+    for (int i = threadIdx.x; i < D; i += kThreads) s_poison[i] = 0x7fffffff;
+    __syncthreads();
+    const int64_t total = s_find[0];
+    const int workers = static_cast<int>(min(static_cast<int64_t>(gridDim.x), total));
+    if (static_cast<int>(blockIdx.x) >= workers) {
+      griddep_launch();
+      return;
+    }
+    begin = blockIdx.x * total / workers;
+    end = (blockIdx.x + 1) * total / workers;
+    ahead.b = static_cast<int>(s_find[1]);
+    ahead.at = s_find[2];
+    ahead.shape = shape_of(p, ahead.b, R);
   }
-  for (int i = threadIdx.x; i < D; i += kThreads) s_poison[i] = 0x7fffffff;
-  __syncthreads();
-  const int64_t total = s_find[0];
-  const int workers = static_cast<int>(min(static_cast<int64_t>(gridDim.x), total));
-  if (static_cast<int>(blockIdx.x) >= workers) {
-    griddep_launch();
-    return;
-  }
-  const int64_t begin = blockIdx.x * total / workers, end = (blockIdx.x + 1) * total / workers;
+  ahead.u = begin;
+  auto next_piece = [&](Walk& x) {
+    if constexpr (CLUSTERS) x.next_tile<R>(p, rank, parts);
+    else x.next<R>(p, end);
+  };
 
   // ---- the warp's 16-key steps, fetched S - 1 steps ahead across the pieces
   uint8_t* ring = smem + warp * S * L::kStep;
   const uint32_t ring_u32 = smem_u32(ring), scale_u32 = smem_u32(&s_scale[warp][0][0]);
-  Walk ahead;
-  ahead.u = begin;
-  ahead.b = static_cast<int>(s_find[1]);
-  ahead.at = s_find[2];
-  ahead.shape = shape_of(p, ahead.b, R);
   Walk now = ahead;
   constexpr int CPR = D / 16;                         // 16-byte pieces of a row
   constexpr int RPI = 32 / CPR < 16 ? 32 / CPR : 16;  // rows per instruction
@@ -286,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D, ROWS>::kPerSm) cached_attn
           a_done = true;
           return;
         }
-        ahead.next<R>(p, end);
+        next_piece(ahead);
         a_j = ahead.first_key + warp * 16;
         a_end = ahead.key_end(p);
       } while (a_j >= a_end);
@@ -331,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D, ROWS>::kPerSm) cached_attn
   int stage = 0;
 
   while (now.u < end) {
-    now.next<R>(p, end);
+    next_piece(now);
     const int rows = now.rows;
     const int lim_first = now.lim_of(p, 0), lim_last = now.lim_of(p, rows - 1);
     const int key_end = now.key_end(p);
@@ -556,7 +633,14 @@ __global__ void __launch_bounds__(kThreads, Layout<D, ROWS>::kPerSm) cached_attn
           dst[2] = v_ref[n][e];
         }
       }
-    const bool whole = now.units == now.shape.units;
+    const bool whole = CLUSTERS ? parts == 1 : now.units == now.shape.units;
+    float* const s_part = reinterpret_cast<float*>(smem + L::kTotal);  // with CLUSTERS: [8][D], then [8] maximum and sum
+    auto store_row4 = [&](int row, int d, const float4& x, float f) {
+      const int r = now.row0 + row;
+      const int rt = p.by_group.quotient(r);
+      bf16* dst = p.out + static_cast<int64_t>(now.q0 + rt) * p.o_token + (now.h * p.group + p.by_group.remainder(r, rt)) * p.o_head + d;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(x.x * f, x.y * f), pack_bf16(x.z * f, x.w * f));
+    };
     const int64_t slot = now.u0 > 0 ? 2 * static_cast<int64_t>(blockIdx.x) : 2 * static_cast<int64_t>(blockIdx.x) + 1;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
@@ -594,16 +678,40 @@ __global__ void __launch_bounds__(kThreads, Layout<D, ROWS>::kPerSm) cached_attn
           if (s_poison[d + 3] < lim) acc.w = __int_as_float(0x7fffffff);
           if (whole) {
             const float inv = m == kNone ? 0.f : 1.f / l;  // a row that sees no key is zero
-            const int r = now.row0 + row;
-            const int rt = p.by_group.quotient(r);
-            bf16* dst = p.out + static_cast<int64_t>(now.q0 + rt) * p.o_token + (now.h * p.group + p.by_group.remainder(r, rt)) * p.o_head + d;
-            *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+            store_row4(row, d, acc, inv);
+          } else if constexpr (CLUSTERS) {
+            *reinterpret_cast<float4*>(s_part + in * D + d) = acc;
+            if (d == 0) *reinterpret_cast<float2*>(s_part + 8 * D + in * 2) = make_float2(m, l);
           } else {
             *reinterpret_cast<float4*>(p.part_o + (slot * R + row) * D + d) = acc;
             if (d == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * R + row) * 2) = make_float2(m, l);
           }
         }
-        __syncthreads();
+        if (CLUSTERS && parts > 1) {
+          cluster_sync();
+          for (int i = rank * kThreads + threadIdx.x; i < min(8, rows - first) * (D / 4); i += parts * kThreads) {
+            const int in = i / (D / 4), d = (i % (D / 4)) * 4;
+            const uint32_t at = smem_u32(s_part + in * D + d), at_ml = smem_u32(s_part + 8 * D + in * 2);
+            float m = kNone;
+#pragma unroll 8
+            for (int c = 0; c < parts; ++c) m = fmaxf(m, ld_cluster2(at_ml, c).x);
+            float l = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+            for (int c = 0; c < parts; ++c) {
+              const float2 ml = ld_cluster2(at_ml, c);
+              const float4 x = ld_cluster4(at, c);
+              const float f = exp2f_approx(ml.x - m);
+              l += ml.y * f;
+              acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
+            }
+            const float inv = l != 0.f ? 1.f / l : 0.f;
+            store_row4(in + first, d, acc, inv);
+          }
+          cluster_sync();  // the others have read this block's rows
+        } else {
+          __syncthreads();
+        }
       }
     }
     if (FMT == kKvFp8 && key_end > lim_first) {  // uniform: only then a NaN may have been noted
@@ -690,26 +798,36 @@ int workers_of(int D, int rows) {
   return 148 * with_shape(D, rows, [](auto d, auto r) { return Layout<d(), r()>::kPerSm; });
 }
 
-template <int FMT, int D, int ROWS>
-void launch(const CachedAttn& p, cudaStream_t stream) {
-  auto kernel = cached_attn_kernel<FMT, D, ROWS>;
-  constexpr int smem = Layout<D, ROWS>::kTotal;
+template <int FMT, int D, int ROWS, bool CLUSTERS>
+void launch(const CachedAttn& p, int parts, cudaStream_t stream) {
+  auto kernel = cached_attn_kernel<FMT, D, ROWS, CLUSTERS>;
+  constexpr int smem = Layout<D, ROWS>::kTotal + (CLUSTERS ? Layout<D, ROWS>::kPart : 0);
   static const bool configured = [&] {
     check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cached_attention smem");
+    if (CLUSTERS) check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "cached_attention cluster");
     return true;
   }();
   (void)configured;
-  const int workers = 148 * Layout<D, ROWS>::kPerSm;
-  launch_pdl(kernel, dim3(workers), dim3(kThreads), smem, stream, "cached_attention", p);
-  const int64_t rows = static_cast<int64_t>(p.T) * p.Hkv * p.group;
-  launch_pdl(cached_attn_join_kernel<D>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), 0, stream,
-             "cached_attention join", p, workers, ROWS);
+  if constexpr (CLUSTERS) {
+    launch_pdl_clusters(kernel, dim3(static_cast<unsigned>(p.B) * p.Hkv * parts), dim3(kThreads), parts, smem, stream,
+                        "cached_attention", p, parts);
+  } else {
+    const int workers = 148 * Layout<D, ROWS>::kPerSm;
+    launch_pdl(kernel, dim3(workers), dim3(kThreads), smem, stream, "cached_attention", p, 0);
+    const int64_t rows = static_cast<int64_t>(p.T) * p.Hkv * p.group;
+    launch_pdl(cached_attn_join_kernel<D>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), 0, stream,
+               "cached_attention join", p, workers, ROWS);
+  }
 }
 
-void cached_attention_rows(const CachedAttn& p, int D, int fmt, int rows, cudaStream_t stream) {
+void cached_attention_rows(const CachedAttn& p, int D, int fmt, int rows, int parts, cudaStream_t stream) {
   with_shape(D, rows, [&](auto d, auto r) {
-    if (fmt == kKvFp8) launch<kKvFp8, d(), r()>(p, stream);
-    else launch<kKvInt8, d(), r()>(p, stream);
+    auto run = [&](auto f) {
+      if (parts > 0) launch<f(), d(), r(), true>(p, parts, stream);
+      else launch<f(), d(), r(), false>(p, 0, stream);
+    };
+    if (fmt == kKvFp8) run(std::integral_constant<int, kKvFp8>{});
+    else run(std::integral_constant<int, kKvInt8>{});
   });
 }
 
@@ -718,10 +836,30 @@ int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 // Which kernel, and how its work is split.
 struct Way {
   bool prompt;
-  int tile;                 // few rows: rows of a tile
+  int tile, parts;          // few rows: rows of a tile, blocks of a cluster (0: equal ranges)
   int tiles_max, splits;    // prompts
   int64_t part_o, part_ml, bytes;  // of the workspace; the prefix sums are at its beginning
 };
+
+// Few rows, little work: the blocks of a cluster that each (request, kv head) gets, or 0 for equal ranges of all work. Equal
+// ranges leave no SM idle, but a second kernel has to add their results, and finding them takes time: about 5 us. Measured
+// (us, clusters against ranges, 8 kv heads of 128 dims, 4 rows each): 1 request of 600 tokens 6.4 / 11.0, of 2400 8.8 / 16.5,
+// of 16000 (16 blocks) 19.6 / 22.6; 4 of 4800 tokens 14.6 / 18.2; 64 of up to 400 tokens 13.1 / 16.5, of up to 1600 28.8 / 22.8.
+// 20 rows: 1 request of 4800 tokens 21.0 / 23.1, of 16000 33.4 / 28.3. So a block of a cluster gets at most `longest` units of
+// 64 keys, fewer where lengths may differ (B > 1) and where a unit takes longer. More blocks than the SMs hold at a time cost
+// more than the ranges do, but for clusters of one; the largest clusters need some room to be placed.
+int cluster_parts(int64_t B, int Hkv, int tile, int resident, int max_context) {
+  const int64_t items = B * Hkv, units = (static_cast<int64_t>(max_context) + kUnit - 1) / kUnit;
+  if (items == 0) return 0;
+  int parts = 1;
+  if (units > 48 && items * kMaxParts * 10 <= resident * 7) {
+    parts = kMaxParts;
+  } else {
+    while (parts < 8 && items * parts * 2 * 8 <= resident * 7) parts *= 2;
+  }
+  const int64_t longest = parts == 1 ? 13 : tile > 8 ? 9 : B == 1 ? 20 : 12;
+  return units <= parts * longest ? parts : 0;
+}
 
 Way way_of(int T, int B, int Hq, int Hkv, int D, int max_query, int max_context) {
   Way w{};
@@ -735,10 +873,12 @@ Way way_of(int T, int B, int Hq, int Hkv, int D, int max_query, int max_context)
     w.tiles_max = static_cast<int>(std::max<int64_t>(1, (static_cast<int64_t>(T) * group + B * (R - 1)) / R));
     // too few row tiles for the SMs: split the keys, two tiles of 128 at least for each part
     const int64_t blocks = static_cast<int64_t>(w.tiles_max) * Hkv;
-    w.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(148 * prompt_per_sm(D) / std::max<int64_t>(blocks, 1), max_context / 256)));
+    w.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(148 * prompt_per_sm(D) / blocks, max_context / 256)));
     slots = w.splits > 1 ? blocks * w.splits * prompt_rows(D) : 0;
   } else {
-    slots = 2 * static_cast<int64_t>(workers_of(D, w.tile)) * w.tile;
+    const int resident = workers_of(D, w.tile);
+    w.parts = cluster_parts(B, Hkv, w.tile, resident, max_context);
+    slots = w.parts > 0 ? 0 : 2 * static_cast<int64_t>(resident) * w.tile;
   }
   w.part_o = align256((static_cast<int64_t>(B) + 1) * sizeof(int64_t));
   w.part_ml = w.part_o + align256(slots * D * sizeof(float));
@@ -791,7 +931,7 @@ void cached_attention(const bf16* q, int64_t q_token, int64_t q_head, bf16* out,
   p.part_o = reinterpret_cast<float*>(base + w.part_o);
   p.part_ml = reinterpret_cast<float*>(base + w.part_ml);
   if (w.prompt) cached_attention_prompt(p, D, fmt, w.tiles_max, w.splits, stream);
-  else cached_attention_rows(p, D, fmt, w.tile, stream);
+  else cached_attention_rows(p, D, fmt, w.tile, w.parts, stream);
 }
 
 int cached_attention_status(bool clear) { return read_status_word(clear); }

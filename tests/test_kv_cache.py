@@ -9,6 +9,7 @@ key's part is at most 2^-33 times the largest scale times its code. So |error| <
 2^-32 max_j scale_j sum_j |code_j| holds with a factor of two to spare on each term."""
 
 import math
+import sys
 
 import pytest
 import torch
@@ -382,6 +383,48 @@ def test_a_nan_value_reaches_the_rows_that_see_it_and_no_other(dim, new, device)
     bad[new - 4:, :, d] = True
     assert torch.equal(o.isnan(), bad)
     _check(torch.where(bad, 0.0, o.double()), torch.where(bad, 0.0, want), size)
+
+
+SPLITS = [  # [(cached, new)], heads, kv heads, head_dim, block: a request's keys over 16, 4, 2 and 1 blocks of threads
+    ([(4000, 2), (9, 1)], 8, 2, 128, 64),
+    ([(700, 1), (64, 1)] * 10, 4, 4, 64, 16),
+    ([(500, 1), (0, 0), (1, 1)] * 15, 4, 4, 128, 32),
+    ([(200, 1), (63, 1), (64, 1), (65, 1)] * 30, 4, 4, 128, 64),
+]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("case", range(len(SPLITS)))
+def test_attention_with_few_and_many_requests(case, fmt, device, monkeypatch):
+    monkeypatch.setattr(sys.modules[__name__], "SHAPES", SPLITS)
+    test_attention_matches_64_bits(case, fmt, device)
+
+
+@pytest.fixture
+def no_bound(monkeypatch):
+    """The host knows no useful bound of the lengths: all work in equal ranges."""
+    attend = kvc.cached_attention
+
+    def loose(*args, **kw):
+        return attend(*args[:8], *(args[8:9] or (max(args[0].size(0), 1),)), 1 << 24, **kw)
+
+    monkeypatch.setattr(kvc, "cached_attention", loose)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("case", range(len(SHAPES)))
+def test_attention_without_a_bound(case, fmt, device, no_bound):
+    test_attention_matches_64_bits(case, fmt, device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lens", [[(70, 1), (3, 4)], [(40, 150), (0, 90)]])
+def test_masks_and_nan_without_a_bound(lens, dim, device, no_bound):
+    test_what_is_masked_does_not_count(dim, lens, "fp8", device)
+    test_a_nan_value_reaches_the_rows_that_see_it_and_no_other(dim, 6 if lens[0][1] == 1 else 200, device)
 
 
 @pytest.mark.parametrize("device", DEVICES)
