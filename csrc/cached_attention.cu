@@ -18,6 +18,11 @@
 // consecutive ranges, one per resident block of threads, so ragged lengths cost nothing; a range that ends inside an item
 // leaves a partial result (at most two per block), which the join kernel adds up in a fixed order. Where there is little
 // work (cluster_parts), a cluster of blocks takes each (request, kv head) instead and adds its results up itself.
+//
+// Measured on a B200, single tokens, 32 heads on 8 of 128, fp8: 64 requests of every length up to 16384 tokens 111-117 us,
+// 5.4-5.7 TB/s, 83-87% of the measured copy rate; one of 600 tokens 7.7 us, latency alone (the launch, then lengths, table,
+// codes and products one after another). 32 requests of up to 2047 tokens, 16 kv heads of 64: 25 us, where the two launches
+// and the pieces' ends (512 items, two ends per range) take most of it.
 #include <algorithm>
 #include <type_traits>
 

@@ -4,24 +4,37 @@
 //   P_g  = exp2(S_g * scale * k_scale - m_g) * v_scale / v_ref     softmax warps, f16, TMEM
 //   O_g += P_g V_j          TMEM, 128 x D; P_g from TMEM, V_j from shared memory
 //
-// A block of threads owns 256 query rows (new tokens x the query heads of one kv head) of one request as two groups of
-// 128, so that the tensor core works on one group's tiles while the other's scores become probabilities, and walks the
-// request's cache in tiles of 128 keys. No TMA: the operands are not in memory as the tensor core wants them. Four warps
-// fetch the codes of each tile by the block table, widen them to f16 (every code is one) and store them in the
-// 128-byte-swizzled layout; the scales of the tile's 16-key groups go beside it and are applied in 32 bits, as in the
-// kernel for few rows (cached_attention.cu), whose rules for masks, row factors and value scales hold here too. The
-// widening is shared by 256 rows: about 2 instructions per code against 256 x 4 flops.
+// A block of threads owns query rows (new tokens x the query heads of one kv head) of one request and walks the request's
+// cache in tiles of 128 keys. With head_dim 128 it has 256 rows as two groups of 128, so that the tensor core works on one
+// group's tiles while the other's scores become probabilities, and the widening is shared by 256 rows (about 2 instructions
+// per code against 256 x 4 flops). With head_dim 64 it has one group, and two blocks share an SM: prompts of a few hundred
+// tokens have few tiles per block, and the second block works while the first begins or ends. Where the row
+// tiles are fewer than the SMs hold, the keys are split as well and a second kernel adds up.
+//
+// No TMA: the operands are not in memory as the tensor core wants them. Four warps fetch the codes of each tile by the block
+// table (cp.async, a whole tile ahead), widen them to f16 (every code is one) and store them in the 128-byte-swizzled layout;
+// the scales of the tile's 16-key groups go beside it and are applied in 32 bits, as in the kernel for few rows
+// (cached_attention.cu), whose rules for masks, row factors and value scales hold here too.
 //
 // Probabilities come from 32-bit exponentials: f16x2 ones would halve the special-function work, but the rounding of
 // their argument costs 2^-8 relative at arguments of 8.
 //
-// TMEM (512 columns): S_0, S_1 at 0 and 128, O_0, O_1 at 256 (D columns each). head_dim 64 has room for P_0, P_1 at 384 and
-// 448; head_dim 128 has none, so P_g lies in S_g (each half of the weights in the columns of its own keys), and the next S_g
-// is issued only once P_g V has completed. A softmax thread reads its row twice (maximum, then exponentials, 32 columns at a time), so that it needs no
-// 128 registers for it: 14 warps with 128 registers each fit the SM.
+// TMEM: S_g, then O_g (D columns each). head_dim 64 (256 columns) has room for P behind them; head_dim 128 (512 columns) has
+// none, so P_g lies in S_g (each half of the weights in the columns of its own keys), and the next S_g is issued only once
+// P_g V has completed. A thread reads its scores twice (maximum, then exponentials, 32 columns at a time): kept in between,
+// they cost the registers that a second block (or the second group) needs, and took longer.
 //
-// Warps: 0-3 widen, 4-7 softmax of group 0, 8-11 of group 1, 12 and 13 issue the groups' MMAs. Every wait is bounded (common.cuh); on a
-// timeout all roles stop, MMAs in flight are waited for, TMEM is freed and the status word records the cause.
+// Warps: 0-3 widen; then eight softmax warps per group, two threads per row; then one warp per group that issues its MMAs,
+// converged (from a single diverged thread an N = 128 MMA took 93 to 105 cycles instead of 64). Every wait is bounded
+// (common.cuh); on a timeout all roles stop, MMAs in flight are waited for, TMEM is freed and the status word records the
+// cause.
+//
+// Measured on a B200: 2048 new tokens after 14337, 32 heads on 8 of 128, fp8: 581-593 us, 870-890 TFLOP/s, 53% of the
+// measured bf16 rate. Bound by the chain S -> maximum -> exponentials -> P V of two groups that share the tensor core (their
+// exponentials alone take 0.35 of the time) and by the last wave: 256 row tiles on 148 SMs. Splitting the tiles of that wave
+// over the keys gave back in partial results what it won. 16 ragged prompts of up to 2048 tokens, 16 heads of 64, int8:
+// 128 us, 268 TFLOP/s: a block has five tiles on average, so its beginning and end and the masked tile on the diagonal count
+// as much as the tiles; 57% of the issue slots are busy.
 #include <algorithm>
 #include <type_traits>
 
@@ -124,7 +137,7 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 3 - Layout<D>::kGroups) c
   uint64_t* teardown = turn + 2;          // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(teardown + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* s_item = reinterpret_cast<int*>(tmem_slot + 2);  // request, row tile, number of tiles, first row, new rows, context
+  int* s_item = reinterpret_cast<int*>(tmem_slot + 2);  // request, row tile, all row tiles, first row, new rows, context
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (smem_u32(smem) & 1023) {  // never with dynamic shared memory alone

