@@ -1,6 +1,7 @@
 // Arguments of the attention over the block-wise 8-bit KV cache, shared by its kernels.
 #pragma once
 
+#include "divisor.cuh"
 #include "launchers.h"
 
 namespace qw {
@@ -12,22 +13,6 @@ struct CachedPages {
   uint32_t block_stride, head_stride, token_stride;
   const float* scale;
   uint32_t scale_stride;
-};
-
-// x / d for 0 <= x < 2^31 by a product: q = (x + floor(x m / 2^32)) >> s with s = ceil(log2 d), m = floor(2^32 (2^s - d) / d)
-// + 1 (Granlund and Montgomery, 1994). The compiler's own division takes ten times the instructions, and these kernels divide
-// by the head group for every row and by the block size for every tile.
-struct Divisor {
-  uint32_t d, m, s;
-  Divisor() = default;
-  explicit Divisor(uint32_t of) : d(of), s(0) {
-    while ((uint64_t{1} << s) < d) ++s;
-    m = static_cast<uint32_t>((uint64_t{1} << 32) * ((uint64_t{1} << s) - d) / d + 1);
-  }
-  __device__ __forceinline__ int quotient(int x) const {
-    return static_cast<int>((__umulhi(m, static_cast<uint32_t>(x)) + static_cast<uint32_t>(x)) >> s);
-  }
-  __device__ __forceinline__ int remainder(int x, int q) const { return x - q * static_cast<int>(d); }
 };
 
 struct CachedAttn {

@@ -7,6 +7,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "divisor.cuh"
 #include "kv_format.cuh"
 #include "launch.cuh"
 #include "launchers.h"
@@ -220,6 +221,7 @@ struct AppendArgs {
   float* scale[2];  // [blocks, Hkv]
   int64_t s_block[2];
   int T, Hkv, block, blocks;
+  Divisor by_block;
   int rows;   // tokens of a block of threads
   int turns;  // (head, keys or values) pairs of a team
 };
@@ -271,13 +273,12 @@ __device__ __forceinline__ uint2 encode8(const uint4& w, float inv) {
   }
 }
 
-// The tokens [t0, t0 + n) of one (block, head), written by a team of NT threads.
+// The tokens [t0, t0 + n) of one (block, head), written by a team of NT threads: into the block from token `first` on where
+// the slots ascend one by one (`straight`).
 template <int FMT, int D, int NT>
-__device__ __forceinline__ void append_run(const AppendArgs& a, int kv, int h, int t0, int n, int team, int me, float* red) {
+__device__ __forceinline__ void append_run(const AppendArgs& a, int kv, int h, int t0, int n, int64_t id, int first,
+                                           bool straight, int team, int me, float* red) {
   constexpr int PPR = D / 8;  // 16-byte pieces of a token's row
-  const int slot0 = a.slots[t0];
-  const int64_t id = slot0 / a.block;
-  const int first = slot0 - static_cast<int>(id) * a.block;
   const bf16* x = (kv ? a.x[1] : a.x[0]) + h * (kv ? a.head_stride[1] : a.head_stride[0]);
   const int64_t ts = kv ? a.token_stride[1] : a.token_stride[0];
   const int64_t ct = kv ? a.c_token[1] : a.c_token[0];
@@ -291,14 +292,23 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, int kv, int h, i
   const int64_t src_step = RS * ts;
   uint4 keep[kKeep];
   uint32_t bits = 0;
+  const bool all = n >= kKeep * RS;  // every thread keeps kKeep pieces: no branch for each
   {
     const bf16* q = src;
+    if (all) {
 #pragma unroll
-    for (int k = 0; k < kKeep; ++k, q += src_step)
-      if (row0 + k * RS < n) keep[k] = __ldg(reinterpret_cast<const uint4*>(q));
+      for (int k = 0; k < kKeep; ++k, q += src_step) keep[k] = __ldg(reinterpret_cast<const uint4*>(q));
 #pragma unroll
-    for (int k = 0; k < kKeep; ++k)
-      if (row0 + k * RS < n) bits = max(bits, amax_bits(keep[k]));
+      for (int k = 0; k < kKeep; ++k) bits = max(bits, amax_bits(keep[k]));
+    } else {
+#pragma unroll
+      for (int k = 0; k < kKeep; ++k, q += src_step) {
+        keep[k] = make_uint4(0, 0, 0, 0);
+        if (row0 + k * RS < n) keep[k] = __ldg(reinterpret_cast<const uint4*>(q));
+      }
+#pragma unroll
+      for (int k = 0; k < kKeep; ++k) bits = max(bits, amax_bits(keep[k]));
+    }
     for (int r = row0 + kKeep * RS; r < n; r += RS, q += src_step) bits = max(bits, amax_bits(__ldg(reinterpret_cast<const uint4*>(q))));
   }
   const bool finite = bits < kInfBits;
@@ -338,8 +348,6 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, int kv, int h, i
       *p = Kv<FMT>::encode4(u.x * ratio, u.y * ratio, v.x * ratio, v.y * ratio);
     }
   }
-  // Ascending slots as many as their span are consecutive; others (a plan never makes them) are looked up one by one.
-  const bool straight = a.slots[t0 + n - 1] - slot0 == n - 1;
   uint8_t* const dst = rows + static_cast<int64_t>(first + row0) * ct + (me % PPR) * 8;
   auto put = [&](int r, uint8_t* to, const uint4& w) {
     if (!straight) to = rows + static_cast<int64_t>(a.slots[t0 + r] - static_cast<int>(id) * a.block) * ct + (me % PPR) * 8;
@@ -347,9 +355,14 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, int kv, int h, i
   };
   {
     uint8_t* q = dst;
+    if (all && straight && finite) {
 #pragma unroll
-    for (int k = 0; k < kKeep; ++k, q += RS * ct)
-      if (row0 + k * RS < n) put(row0 + k * RS, q, keep[k]);
+      for (int k = 0; k < kKeep; ++k, q += RS * ct) *reinterpret_cast<uint2*>(q) = encode8<FMT, true>(keep[k], inv);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kKeep; ++k, q += RS * ct)
+        if (row0 + k * RS < n) put(row0 + k * RS, q, keep[k]);
+    }
     for (int r = row0 + kKeep * RS; r < n; r += RS, q += RS * ct)
       put(r, q, __ldg(reinterpret_cast<const uint4*>(src + static_cast<int64_t>(r - row0) * ts)));
   }
@@ -364,8 +377,8 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, int kv, int h, i
 // Bound by HBM for prompts (2 bytes read, 1 written per number), by the latency of dependent reads for decode. With a block
 // of threads per (run, head) and 4 KB of each run in flight, prompts ran at 16% of HBM; with a warp per pair the runs are
 // looked for once per eight pairs.
-// Measured on a B200: 24 prompts of 14900 tokens in all, bf16 to int8, 16 heads of 64 each for keys and values: 26.7 us,
-// 3.4 TB/s, 53% of the measured copy rate (the rest is the arithmetic per number: magnitude, product, rounding, clamp and
+// Measured on a B200: 24 prompts of 14900 tokens in all, bf16 to int8, 16 heads of 64 each for keys and values: 24.2 us,
+// 3.8 TB/s, 58% of the measured copy rate (the rest is the arithmetic per number: magnitude, product, rounding, clamp and
 // packing); 32 single tokens 4.4 us, one launch's latency.
 template <int FMT, int D, int NT>
 __global__ void __launch_bounds__(kAppendThreads, 3) append_kernel(AppendArgs a) {
@@ -375,32 +388,43 @@ __global__ void __launch_bounds__(kAppendThreads, 3) append_kernel(AppendArgs a)
   griddep_wait();
   griddep_launch();
   const int r0 = blockIdx.x * a.rows, r1 = min(r0 + a.rows, a.T);
-  // the cache block of a token; -1: none (padding, or a slot that the cache does not have)
-  auto block_of = [&](int t) {
-    const int s = a.slots[t];
-    if (s < 0) return -1;
-    const int id = static_cast<int>(static_cast<uint32_t>(s) / static_cast<uint32_t>(a.block));
-    return id < a.blocks ? id : -1;
+  // a token's slot; -1: none (padding, or a slot that the cache does not have)
+  auto slot_of = [&](int t) {
+    const int s = t >= 0 && t < a.T ? a.slots[t] : -1;
+    return s >= 0 && a.by_block.quotient(s) < a.blocks ? s : -1;
   };
-  // Every warp looks for the runs itself: they are few, and nothing has to be waited for.
+  auto block_of = [&](int s) { return s < 0 ? -1 : a.by_block.quotient(s); };
+  // Every warp looks for the runs itself: they are few, and nothing has to be waited for. The slots of 64 tokens are read at
+  // once, so that what most runs need to be found is there after one latency.
   for (int base = r0; base < r1; base += 32) {
-    const int mine = base + lane < r1 ? block_of(base + lane) : -1;
-    const int before = base + lane < r1 && base + lane > 0 ? block_of(base + lane - 1) : -1;
-    unsigned heads = __ballot_sync(0xffffffffu, mine >= 0 && mine != before);
+    const int slots[2] = {slot_of(base + lane), slot_of(base + 32 + lane)};
+    const int before = block_of(slot_of(base + lane - 1));
+    const int ids[2] = {block_of(slots[0]), block_of(slots[1])};
+    unsigned heads = __ballot_sync(0xffffffffu, base + lane < r1 && ids[0] >= 0 && ids[0] != before);
     while (heads) {
       const int at = __ffs(heads) - 1;
       heads &= heads - 1;
-      const int t0 = base + at, id = __shfl_sync(0xffffffffu, mine, at);
-      int n = 1;
-      while (true) {
-        const int u = t0 + n + lane;
-        const unsigned same = __ballot_sync(0xffffffffu, u < a.T && n + lane < a.block && block_of(u) == id);
-        n += same == 0xffffffffu ? 32 : __ffs(~same) - 1;
-        if (same != 0xffffffffu) break;
+      const int t0 = base + at, id = __shfl_sync(0xffffffffu, ids[0], at), slot0 = __shfl_sync(0xffffffffu, slots[0], at);
+      const unsigned others[2] = {~(__ballot_sync(0xffffffffu, ids[0] == id) >> at), ~__ballot_sync(0xffffffffu, ids[1] == id)};
+      int n = __ffs(others[0]) - 1;  // a shift leaves zeros at the top; none for at = 0
+      if (others[0] == 0) n = 32;
+      if (at + n == 32) n += others[1] ? __ffs(others[1]) - 1 : 32;
+      if (at + n == 64) {
+        while (n < a.block) {
+          const unsigned other = __ballot_sync(0xffffffffu, block_of(slot_of(t0 + n + lane)) != id);
+          n += other ? __ffs(other) - 1 : 32;
+          if (other) break;
+        }
       }
+      n = min(n, a.block);
+      // Ascending slots as many as their span are consecutive; others (a plan never makes them) are looked up one by one.
+      const int last = at + n - 1, in = __shfl_sync(0xffffffffu, last < 32 ? slots[0] : slots[1], last & 31);
+      const bool straight = (last < 64 ? in : a.slots[t0 + n - 1]) - slot0 == n - 1;
+      const int first = a.by_block.remainder(slot0, id);
       for (int k = 0; k < a.turns; ++k) {
         const int pair = (blockIdx.y * a.turns + k) * kTeams + team;
-        if (pair < 2 * a.Hkv) append_run<FMT, D, NT>(a, pair & 1, pair >> 1, t0, n, team, me, s_red + team * (NT / 32));
+        if (pair < 2 * a.Hkv)
+          append_run<FMT, D, NT>(a, pair & 1, pair >> 1, t0, n, id, first, straight, team, me, s_red + team * (NT / 32));
       }
     }
   }
@@ -414,7 +438,7 @@ void append_launch(AppendArgs a, cudaStream_t stream) {
   // prompt's runs have one owner each, and all pairs of a few hundred blocks per SM in one
   a.rows = std::max(1, std::min({a.block, kAppendRows, static_cast<int>(static_cast<int64_t>(a.T) * groups / (148 * 4))}));
   const int64_t tiles = (a.T + a.rows - 1) / a.rows;
-  a.turns = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(groups, tiles * groups / (148 * 16))));
+  a.turns = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(groups, tiles * groups / (148 * 4))));
   const dim3 grid(static_cast<unsigned>(tiles), (groups + a.turns - 1) / a.turns);
   launch_pdl(append_kernel<FMT, D, NT>, grid, dim3(kAppendThreads), 0, stream, "append_kv", a);
 }
@@ -466,6 +490,7 @@ void append_kv(const KvSource& k, const KvSource& v, const int* slots, const KvP
                int D, int block, int blocks, int fmt, cudaStream_t stream) {
   if (T == 0) return;
   AppendArgs a{};
+  a.by_block = Divisor(block);
   const KvSource* src[2] = {&k, &v};
   const KvPages* dst[2] = {&kc, &vc};
   for (int i = 0; i < 2; ++i) {
