@@ -6,15 +6,16 @@
 //
 // A block of threads owns a range of one row's ids and keeps their counts in shared memory: it scans the row's history
 // (a few thousand ids, from L2) and counts those of its range, then reads and writes each logit once, 16 bytes at a
-// time (at most two pieces per thread, fetched before the history). That needs no count tables in memory, no sort and no
+// time (at most four pieces per thread, fetched before the history). That needs no count tables in memory, no sort and no
 // second launch. Counts are integers, so the order of the atomics does not matter. A thread's ids are on a 16-byte boundary
 // of the logits, not of the bias row: it reads the two or three aligned pieces that hold their biases and shifts (one by one,
 // eight numbers apart from lane to lane, the biases kept L1 busy for 79% of the time). Bound by HBM for many rows, by latency
 // for one.
 //
-// Measured on a B200: 256 rows of 50257 bf16 logits with histories of up to 4096 ids, biases and masks for some rows: 27 us,
-// 2.1 TB/s, 32% of the measured copy rate: the parts of a block follow one another (clear the counts, count, then the
-// logits), and each block scans its row's history anew. One row of 32000 fp32 logits: 6.0 us, latency.
+// Measured on a B200: 256 rows of 50257 bf16 logits with histories of up to 4096 ids, biases and masks for some rows: 23 us,
+// 2.5 TB/s, 38% of the measured copy rate: the parts of a block follow one another (clear the counts, count, then the
+// logits), and each block scans its row's history anew. One row of 32000 fp32 logits: 5.9 us a call, of which 3.0 on the
+// device.
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -28,8 +29,7 @@ namespace qw {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPieces = 2;  // 16-byte pieces of a thread
-constexpr int kEarly = 4;   // ids of the history that a thread fetches before it knows how many there are
+constexpr int kPieces = 4;  // 16-byte pieces of a thread
 constexpr uint32_t kPrompt = 0x80000000u;  // in the prompt; the other bits count generated occurrences
 
 template <typename T>
@@ -85,18 +85,16 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(LogitsArgs a, int rang
     if (p < pieces) w[k] = *reinterpret_cast<const uint4*>(src + body + p * VE);
   }
   const int* ids = a.history + (penalised ? row * a.history_stride : 0);
-  int early[kEarly];
+  // by fours where the row begins on a 16-byte boundary; the first four of a thread before it knows how many there are
+  const int fours = penalised && (reinterpret_cast<uintptr_t>(ids) & 15) == 0 ? a.history_width / 4 : 0;
+  int4 early = make_int4(-1, -1, -1, -1);
   if (penalised) {
     used = min(max(a.history_lens[row], 0), a.history_width);
     prompt = a.prompt_lens ? a.prompt_lens[row] : 0;
     rep = a.repetition ? a.repetition[row] : 1.f;
     freq = a.frequency ? a.frequency[row] : 0.f;
     pres = a.presence ? a.presence[row] : 0.f;
-#pragma unroll
-    for (int k = 0; k < kEarly; ++k) {
-      const int i = threadIdx.x + k * kThreads;
-      early[k] = i < a.history_width ? ids[i] : -1;
-    }
+    if (static_cast<int>(threadIdx.x) < fours) early = __ldg(reinterpret_cast<const int4*>(ids) + threadIdx.x);
     for (int i = threadIdx.x * 4; i < hi - first; i += kThreads * 4) *reinterpret_cast<uint4*>(counts + i) = make_uint4(0, 0, 0, 0);
   }
   const float* bias = bias_row >= 0 && bias_row < a.biases ? a.bias + bias_row * a.bias_stride : nullptr;
@@ -109,16 +107,24 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(LogitsArgs a, int rang
   }
   if (penalised) {
     __syncthreads();
+    const uint32_t span = hi - lo;
     auto count = [&](int i, int id) {
-      if (i < used && id >= lo && id < hi) {
+      if (static_cast<uint32_t>(id - lo) < span && i < used) {
         if (i < prompt) atomicOr(&counts[id - first], kPrompt);
         else atomicAdd(&counts[id - first], 1u);
       }
     };
-#pragma unroll
-    for (int k = 0; k < kEarly; ++k) count(threadIdx.x + k * kThreads, early[k]);
-#pragma unroll 4
-    for (int i = threadIdx.x + kEarly * kThreads; i < used; i += kThreads) count(i, ids[i]);
+    auto count4 = [&](int i, const int4& x) {
+      count(i, x.x);
+      count(i + 1, x.y);
+      count(i + 2, x.z);
+      count(i + 3, x.w);
+    };
+    count4(threadIdx.x * 4, early);
+    const int full = min(fours, (used + 3) / 4);
+#pragma unroll 2
+    for (int i = threadIdx.x + kThreads; i < full; i += kThreads) count4(4 * i, __ldg(reinterpret_cast<const int4*>(ids) + i));
+    for (int i = 4 * fours + threadIdx.x; i < used; i += kThreads) count(i, ids[i]);
     __syncthreads();
   }
 
@@ -194,10 +200,11 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(LogitsArgs a, int rang
 
 template <typename T>
 void launch(const LogitsArgs& a, cudaStream_t stream) {
-  // equal ranges of at most two pieces per thread, of one where that leaves SMs without work
+  // Equal ranges of at most four pieces per thread: each range scans the row's history anew (256 rows of 50257: 23.1 us,
+  // 23.5 with two). Of two or one where that leaves fewer than two blocks for an SM (16 rows: 5.2 us, 5.6 with four).
   constexpr int VE = 16 / static_cast<int>(sizeof(T));
   int most = kThreads * kPieces * VE;
-  if (static_cast<int64_t>(a.rows) * ((a.vocab + most - 1) / most) < 148) most /= 2;
+  while (most > kThreads * VE && static_cast<int64_t>(a.rows) * ((a.vocab + most - 1) / most) < 148 * 2) most /= 2;
   const int ranges = (a.vocab + most - 1) / most;
   const int range = ((a.vocab + ranges - 1) / ranges + 32 * VE - 1) / (32 * VE) * (32 * VE);
   const dim3 grid(ranges, a.rows);  // the ids before the first boundary come on top of the first range
