@@ -852,7 +852,8 @@ struct Way {
 // of 16000 (16 blocks) 19.6 / 22.6; 4 of 4800 tokens 14.6 / 18.2; 64 of up to 400 tokens 13.1 / 16.5, of up to 1600 28.8 / 22.8.
 // 20 rows: 1 request of 4800 tokens 21.0 / 23.1, of 16000 33.4 / 28.3. So a block of a cluster gets at most `longest` units of
 // 64 keys, fewer where lengths may differ (B > 1) and where a unit takes longer. More blocks than the SMs hold at a time cost
-// more than the ranges do, but for clusters of one; the largest clusters need some room to be placed.
+// more than the ranges do, but for clusters of one; the largest clusters need some room to be placed. A block without a unit
+// only costs barriers (27 requests of up to 5 tokens: 4.7 us, 6.8 with eight blocks).
 int cluster_parts(int64_t B, int Hkv, int tile, int resident, int max_context) {
   const int64_t items = B * Hkv, units = (static_cast<int64_t>(max_context) + kUnit - 1) / kUnit;
   if (items == 0) return 0;
@@ -860,7 +861,7 @@ int cluster_parts(int64_t B, int Hkv, int tile, int resident, int max_context) {
   if (units > 48 && items * kMaxParts * 10 <= resident * 7) {
     parts = kMaxParts;
   } else {
-    while (parts < 8 && items * parts * 2 * 8 <= resident * 7) parts *= 2;
+    while (parts < 8 && parts < units && items * parts * 2 * 8 <= resident * 7) parts *= 2;
   }
   const int64_t longest = parts == 1 ? 13 : tile > 8 ? 9 : B == 1 ? 20 : 12;
   return units <= parts * longest ? parts : 0;
@@ -882,7 +883,7 @@ Way way_of(int T, int B, int Hq, int Hkv, int D, int max_query, int max_context)
     slots = w.splits > 1 ? blocks * w.splits * prompt_rows(D) : 0;
   } else {
     const int resident = workers_of(D, w.tile);
-    w.parts = cluster_parts(B, Hkv, w.tile, resident, max_context);
+    w.parts = rows <= w.tile ? cluster_parts(B, Hkv, w.tile, resident, max_context) : 0;  // a request is one row tile
     slots = w.parts > 0 ? 0 : 2 * static_cast<int64_t>(resident) * w.tile;
   }
   w.part_o = align256((static_cast<int64_t>(B) + 1) * sizeof(int64_t));
