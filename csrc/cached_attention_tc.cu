@@ -30,8 +30,8 @@
 // cause.
 //
 // Measured on a B200: 2048 new tokens after 14337, 32 heads on 8 of 128, fp8: 581-593 us, 870-890 TFLOP/s, 53% of the
-// measured bf16 rate. Bound by the chain S -> maximum -> exponentials -> P V of two groups that share the tensor core (their
-// exponentials alone take 0.35 of the time) and by the last wave: 256 row tiles on 148 SMs. Splitting the tiles of that wave
+// measured bf16 rate. Bound by the chain S -> maximum -> exponentials -> P V of two groups that share the tensor core (its pipe
+// is busy for 47% of the active cycles, the special-function units for 51%) and by the last wave: 256 row tiles on 148 SMs. Splitting the tiles of that wave
 // over the keys gave back in partial results what it won. 16 ragged prompts of up to 2048 tokens, 16 heads of 64, int8:
 // 128 us, 268 TFLOP/s: a block has five tiles on average, so its beginning and end and the masked tile on the diagonal count
 // as much as the tiles; 57% of the issue slots are busy.
