@@ -73,7 +73,8 @@ __device__ __forceinline__ Need need_of(const PlanArgs& a, int b) {
   n.fresh = max(a.fresh[b], 0);
   const uint32_t total = min(static_cast<uint32_t>(n.cached) + static_cast<uint32_t>(n.fresh), 0x7fffffffu);
   n.context = static_cast<int>(total);
-  n.wanted = static_cast<int>((total + static_cast<uint32_t>(a.block) - 1) / static_cast<uint32_t>(a.block));
+  // without new tokens: none, whatever length a caller leaves beside a row that it does not use
+  n.wanted = n.fresh > 0 ? static_cast<int>((total + static_cast<uint32_t>(a.block) - 1) / static_cast<uint32_t>(a.block)) : 0;
   n.fits = min(n.wanted, a.width);
   n.held = min(max(a.state[1 + b], 0), a.width);
   return n;

@@ -46,15 +46,15 @@ def plan_blocks(cached_lens: Tensor, new_lens: Tensor, state: Tensor, block_tabl
 
     ``state`` is int32 ``[1 + requests]``: how many of ``free_blocks`` are free (its first entries), then the blocks that
     each request holds already. A request that needs more gets the last free ones, requests in order; their ids go into
-    ``block_table`` (in place, from the held entries on). ``state`` itself is left alone: the new one is in the result.
-    ``tokens`` is the number of rows of the step; rows past the requests' tokens are padding. Where blocks run out the
-    entries are -1 and ``missing`` counts them."""
+    ``block_table`` (in place, from the held entries on). A request without new tokens gets none, whatever its cached
+    length. ``state`` itself is left alone: the new one is in the result. ``tokens`` is the number of rows of the step;
+    rows past the requests' tokens are padding. Where blocks run out the entries are -1 and ``missing`` counts them."""
     if cached_lens.is_cuda:
         return BlockPlan(*ext().plan_blocks(cached_lens, new_lens, state, block_table, free_blocks, block, tokens))
     cached, new = cached_lens.long().clamp(min=0), new_lens.long().clamp(min=0)
     width = block_table.size(1)
     start = torch.cat([new.new_zeros(1), new.cumsum(0)])
-    wanted = (cached + new + block - 1) // block
+    wanted = torch.where(new > 0, (cached + new + block - 1) // block, 0)
     fits = wanted.clamp(max=width)
     held = state[1:].long().clamp(min=0, max=width)
     left = min(max(int(state[0]), 0), free_blocks.numel())
