@@ -76,8 +76,7 @@ class ContinuousBatcher:
         self._position = [0] * self.slots
         self._next_token = [0] * self.slots
         self._generators: dict[int, torch.Generator] = {}
-        # block-wise cache: blocks promised to each slot's request, and slots whose last request ended in an error and may
-        # still hold blocks
+        # block-wise cache: blocks promised to each slot's request, and slots that may still hold blocks of no active request
         self._blocks = [0] * self.slots
         self._unreleased: set = set()
         self.steps = 0
@@ -121,6 +120,8 @@ class ContinuousBatcher:
 
     # ---- scheduling ---------------------------------------------------------------------------------------
     def _admit(self) -> None:
+        if not self.active and self.waiting:  # the decoder may have been used for something else meanwhile
+            self._unreleased.update(range(self.slots))
         if self._unreleased:
             if self.decoder.cache is not None:
                 self.decoder.cache.release_rows(sorted(self._unreleased - set(self.active)))
@@ -199,7 +200,8 @@ class ContinuousBatcher:
         if self.decoder.cache is not None:  # the active rows only, in slot order; idle slots have no token
             tokens = [self._next_token[s] for s in rows] + [0] * (self.slots - len(rows))
             new = torch.tensor([int(s in rows) for s in range(self.slots)], dtype=torch.int32, device=dev)
-            logits = self.decoder.run_step(torch.tensor(tokens, device=dev), positions, new)[: len(rows)]
+            # the blocks promised to the active requests suffice
+            logits = self.decoder._run_step(torch.tensor(tokens, device=dev), positions, new)[: len(rows)]
         else:
             tokens = torch.tensor([self._next_token[s] if s in rows else 0 for s in range(self.slots)], device=dev)
             logits = self.decoder.run_step(tokens, positions)[rows]

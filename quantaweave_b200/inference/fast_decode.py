@@ -42,6 +42,8 @@ import torch
 import torch.nn.functional as F
 from torch import Tensor
 
+from .paged_cache import PagedKVCache, PoolExhausted
+
 BATCH = 8
 
 
@@ -125,8 +127,6 @@ class FastDecoder:
         self.cache = None
         self.prefill_chunk = prefill_chunk
         if kv_cache != "dense":
-            from .paged_cache import PagedKVCache
-
             if self.ep is not None:
                 raise Unsupported("the block-wise KV cache with expert-parallel decoding")
             if self.native and self.head_dim not in (32, 64, 128):
@@ -517,9 +517,11 @@ class FastDecoder:
         """Read ``prompts [B, n]`` in one pass (no expert capacity) and leave their keys/values in cache rows
         ``first_row .. first_row + B - 1`` (a continuous batcher fills one slot at a time)."""
         batch, n = prompts.shape
-        self.length = n
         if self.cache is not None:
+            rows = range(first_row, first_row + batch)
+            self.cache.require(dict.fromkeys(rows, n), rows)
             self.cache.release_rows(slice(first_row, first_row + batch))  # the rows begin anew
+        self.length = n
         if n == 0:
             return
         if self.cache is not None:
@@ -630,7 +632,18 @@ class FastDecoder:
         """One step for ``tokens [B]`` at ``positions [B]``; returns fp32 logits ``[B, V]`` (a reused buffer).
 
         With the block-wise cache ``new [max_batch]`` (0 or 1) may leave requests out: ``positions`` is then ``[max_batch]``, and
-        ``tokens [max_batch]`` holds the tokens of the others in order, padded at the end; so are the logits."""
+        ``tokens [max_batch]`` holds the tokens of the others in order, padded at the end; so are the logits. Where its pool is
+        smaller than all full contexts, the positions and the blocks held are read back before the step, which is refused
+        (``PoolExhausted``) when it would leave a token without a block."""
+        cache = self.cache
+        if cache is not None and cache.blocks < cache.requests * cache.width:
+            at = positions.tolist()
+            there = range(tokens.numel()) if new is None else [row for row, n in enumerate(new.tolist()) if n]
+            cache.require({row: at[row] + 1 for row in there})
+        return self._run_step(tokens, positions, new)
+
+    def _run_step(self, tokens: Tensor, positions: Tensor, new: Optional[Tensor] = None) -> Tensor:
+        """``run_step`` for a caller that knows that the blocks suffice."""
         batch = tokens.numel()
         self.tokens_in[:batch].copy_(tokens)
         if self.cache is not None:
@@ -658,16 +671,25 @@ class FastDecoder:
         batch, plen = prompts.shape
         if plen + max_new > self.capacity:
             raise ValueError(f"prompt + new tokens ({plen + max_new}) exceed the context {self.capacity}")
+        self._begin_alone(batch, max(plen - 1 + max_new, 0))  # the last new token is not read
         prompts = prompts.to(self.device)
         self._prefill(prompts[:, :-1])
         out = torch.empty(batch, max_new, dtype=torch.long, device=self.device)
         token = prompts[:, -1]
         for i in range(max_new):
             positions = torch.full((batch,), plen - 1 + i, dtype=torch.int32, device=self.device)
-            logits = self.run_step(token, positions)
+            logits = self._run_step(token, positions)
             token = logits.argmax(-1)
             out[:, i] = token
         return out
+
+    def _begin_alone(self, batch: int, tokens: int) -> None:
+        """The block-wise cache for the first ``batch`` rows and nothing else: refused where the pool has no room for that many
+        tokens of each, else all rows' blocks are given back."""
+        if self.cache is None:
+            return
+        self.cache.require(dict.fromkeys(range(batch), tokens), range(self.max_batch))
+        self.cache.release_rows(slice(None))
 
     # ---- batch-1 interface (reference parity) ----------------------------------------------------------
     def reset(self) -> None:
@@ -678,7 +700,7 @@ class FastDecoder:
     def _run(self, token: int) -> None:
         t = torch.tensor([token], device=self.device)
         p = torch.tensor([self.length], dtype=torch.int32, device=self.device)
-        self.run_step(t, p)
+        self._run_step(t, p)
         self.length += 1
         self.tokens.append(token)
 
@@ -690,6 +712,7 @@ class FastDecoder:
             from ..ops import ext
 
             self._C = ext()
+        self._begin_alone(1, len(window))
         self.reset()
         self._prefill(torch.tensor([window[:-1]], device=self.device))
         self.tokens = list(window[:-1])
@@ -702,6 +725,9 @@ class FastDecoder:
             self.reset()
             self._prefill(torch.tensor([keep], device=self.device))
             self.tokens = list(keep)
+        if self.cache is not None and self.cache.blocks_for(self.length + 1) > self.cache.blocks:
+            raise PoolExhausted(f"a context of {self.length + 1} tokens needs {self.cache.blocks_for(self.length + 1)} cache "
+                                f"blocks, the pool has {self.cache.blocks}")
         self._run(token)
         return self.logits[0]
 

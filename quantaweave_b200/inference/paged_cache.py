@@ -15,9 +15,13 @@ from torch import Tensor
 from ..ops import kv_cache as ops
 
 
+class PoolExhausted(RuntimeError):
+    """The pool has fewer blocks than the requests need."""
+
+
 class PagedKVCache:
     """``blocks`` defaults to what ``requests`` full contexts need; with fewer, who admits requests keeps count
-    (``blocks_for``)."""
+    (``blocks_for``) or asks before a step (``require``): a token without a block is not stored."""
 
     def __init__(self, layers: int, requests: int, capacity: int, kv_heads: int, head_dim: int, device,
                  fmt: str = "fp8", block: int = 64, blocks: Optional[int] = None) -> None:
@@ -49,6 +53,20 @@ class PagedKVCache:
 
     def blocks_for(self, tokens: int) -> int:
         return -(-tokens // self.block)
+
+    def require(self, tokens: dict, fresh=()) -> None:
+        """Raise ``PoolExhausted`` unless the pool has the blocks for ``tokens[row]`` tokens of each row, beside what all rows
+        hold (those in ``fresh`` as if they held none). Where the pool is smaller than all full contexts this reads the
+        device."""
+        most = max(tokens.values(), default=0)
+        if self.blocks_for(most) > self.width:
+            raise PoolExhausted(f"{most} tokens need {self.blocks_for(most)} cache blocks, a request has at most {self.width}")
+        if self.blocks >= self.requests * self.width:
+            return
+        held = [0 if row in fresh else n for row, n in enumerate(self.state[1:].tolist())]
+        need = sum(max(held[row], self.blocks_for(tokens.get(row, 0))) for row in range(self.requests))
+        if need > self.blocks:
+            raise PoolExhausted(f"the requests need {need} cache blocks, the pool has {self.blocks}")
 
     def plan(self, cached_lens: Tensor, new_lens: Tensor, tokens: int) -> ops.BlockPlan:
         """Blocks for the step's new tokens (``ops.plan_blocks``), taken from the pool."""
