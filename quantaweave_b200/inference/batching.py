@@ -31,6 +31,9 @@ import torch
 from .fast_decode import FastDecoder, filter_logits
 
 
+PENALTY_LIMIT = 1e6
+
+
 @dataclass
 class GenerationRequest:
     prompt: list
@@ -90,8 +93,14 @@ class ContinuousBatcher:
         if len(request.prompt) + request.max_new > self.decoder.capacity:
             raise ValueError(f"prompt ({len(request.prompt)}) + max_new ({request.max_new}) exceed the decoder "
                              f"context {self.decoder.capacity}")
-        if request.repetition_penalty <= 0:
+        # NaN fails these too; within them no logit leaves the range of 32-bit numbers
+        if not 0 < request.repetition_penalty:
             raise ValueError("repetition_penalty must be positive")
+        if not 1 / PENALTY_LIMIT <= request.repetition_penalty <= PENALTY_LIMIT:
+            raise ValueError(f"repetition_penalty must lie between {1 / PENALTY_LIMIT:g} and {PENALTY_LIMIT:g}")
+        for name in ("frequency_penalty", "presence_penalty"):
+            if not abs(getattr(request, name)) <= PENALTY_LIMIT:
+                raise ValueError(f"{name} must be a number of at most {PENALTY_LIMIT:g} in magnitude")
         cache = self.decoder.cache
         if cache is not None and self._blocks_of(request) > cache.blocks:
             raise ValueError(f"prompt ({len(request.prompt)}) + max_new ({request.max_new}) need {self._blocks_of(request)} "

@@ -58,9 +58,9 @@ class GenerateRequest(BaseModel):
     seed: Optional[int] = None
     stop: list[str] = Field(default_factory=list)
     # with --batching only
-    repetition_penalty: float = Field(1.0, gt=0)
-    frequency_penalty: float = 0.0
-    presence_penalty: float = 0.0
+    repetition_penalty: float = Field(1.0, ge=0.01, le=100, allow_inf_nan=False)
+    frequency_penalty: float = Field(0.0, ge=-100, le=100, allow_inf_nan=False)
+    presence_penalty: float = Field(0.0, ge=-100, le=100, allow_inf_nan=False)
 
     @property
     def penalised(self) -> bool:
