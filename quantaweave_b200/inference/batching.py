@@ -163,7 +163,23 @@ class ContinuousBatcher:
             with self.lock:
                 self.active[slot] = request
 
-    def _processed(self, logits: torch.Tensor, rows: list) -> torch.Tensor:
+    def _masks(self, rows: list, failed: dict) -> dict:
+        """``{slot: bool [vocab]}`` of the active rows with a grammar; an error goes to ``failed[slot]``."""
+        masks = {}
+        for slot in rows:
+            request = self.active[slot]
+            if request.allowed is None:
+                continue
+            try:
+                mask = torch.as_tensor(request.allowed(request.tokens)).cpu().bool()
+                if mask.shape != (self.decoder.vocab,):
+                    raise ValueError(f"the grammar's mask must be [{self.decoder.vocab}], got {list(mask.shape)}")
+                masks[slot] = mask
+            except Exception as exc:  # noqa: BLE001 - a request's own callback: it alone ends
+                failed[slot] = exc
+        return masks
+
+    def _processed(self, logits: torch.Tensor, rows: list, failed: dict) -> torch.Tensor:
         """Penalties and grammar masks of the active rows' requests, in one pass on the logits' device."""
         requests = [self.active[s] for s in rows]
         if not any(r.penalised or r.allowed is not None for r in requests):
@@ -180,18 +196,21 @@ class ContinuousBatcher:
                                       [r.presence_penalty for r in requests]]).to(dev)
             kw.update(history=history.to(dev), history_lens=lens[0], prompt_lens=lens[1], repetition=penalties[0],
                       frequency=penalties[1], presence=penalties[2])
-        masks = [r.allowed(r.tokens) for r in requests if r.allowed is not None]
+        masks = self._masks(rows, failed)
         if masks:
-            which = iter(range(len(masks)))
-            kw.update(mask=pack_mask(torch.stack([m.cpu() for m in masks])).to(dev),
-                      mask_rows=torch.tensor([-1 if r.allowed is None else next(which) for r in requests], dtype=torch.int32).to(dev))
+            which = {slot: i for i, slot in enumerate(masks)}
+            kw.update(mask=pack_mask(torch.stack(list(masks.values()))).to(dev),
+                      mask_rows=torch.tensor([which.get(s, -1) for s in rows], dtype=torch.int32).to(dev))
         return process_logits(logits, **kw)
 
     def _sample(self, logits: torch.Tensor, request: GenerationRequest, generator: torch.Generator) -> int:
         if request.logit_bias is not None:
             logits = logits + request.logit_bias
         if request.temperature <= 0:
-            return int(logits.argmax())
+            token = int(logits.argmax())
+            if logits[token] == float("-inf"):
+                raise ValueError("no token is allowed")
+            return token
         filtered = filter_logits(logits[None] / request.temperature, request.top_k, request.top_p)[0]
         return int(torch.multinomial(filtered.softmax(-1), 1, generator=generator))
 
@@ -214,11 +233,19 @@ class ContinuousBatcher:
         else:
             tokens = torch.tensor([self._next_token[s] if s in rows else 0 for s in range(self.slots)], device=dev)
             logits = self.decoder.run_step(tokens, positions)[rows]
-        logits = self._processed(logits.float(), rows).cpu()
+        failed: dict = {}  # a request whose grammar or sampling fails ends alone
+        logits = self._processed(logits.float(), rows, failed).cpu()
         self.steps += 1
         for i, slot in enumerate(rows):
             request = self.active[slot]
-            token = self._sample(logits[i], request, self._generators[slot])
+            if slot not in failed:
+                try:
+                    token = self._sample(logits[i], request, self._generators[slot])
+                except Exception as exc:  # noqa: BLE001
+                    failed[slot] = exc
+            if slot in failed:
+                self._retire(slot, f"error: {failed[slot]}")
+                continue
             request.tokens.append(token)
             if request.on_token is not None:
                 request.on_token(token)
@@ -230,14 +257,18 @@ class ContinuousBatcher:
             elif len(request.tokens) >= request.max_new or self._position[slot] + 1 >= self.decoder.capacity:
                 reason = "length"
             if reason is not None:
-                request.finish_reason = reason
-                with self.lock:
-                    del self.active[slot]
-                if self.decoder.cache is not None:
-                    self.decoder.cache.release_rows([slot])
-                request.done.set()
+                self._retire(slot, reason)
         with self.lock:
             return len(self.active)
+
+    def _retire(self, slot: int, reason: str) -> None:
+        request = self.active[slot]
+        request.finish_reason = reason
+        with self.lock:
+            del self.active[slot]
+        if self.decoder.cache is not None:
+            self.decoder.cache.release_rows([slot])
+        request.done.set()
 
     def run_until_idle(self) -> None:
         while self.pending():

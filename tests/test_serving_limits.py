@@ -46,3 +46,45 @@ def test_penalties_at_their_limits_can_be_sampled(edge):
     request = batcher.submit(GenerationRequest([1, 2, 3], 20, temperature=0.7, **edge))
     batcher.run_until_idle()
     assert len(request.tokens) == 20
+
+
+def _raises(made):
+    raise RuntimeError("no such state")
+
+
+VOCAB = 512  # of the tiny preset
+
+
+@pytest.mark.parametrize("cache", ["dense", "int8"])
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+@pytest.mark.parametrize("bad", [dict(allowed=_raises), dict(allowed=lambda made: torch.zeros(VOCAB, dtype=torch.bool)),
+                                 dict(allowed=lambda made: torch.ones(VOCAB - 1, dtype=torch.bool)),
+                                 dict(allowed=lambda made: None if len(made) == 2 else torch.ones(VOCAB, dtype=torch.bool)),
+                                 dict(logit_bias=torch.full((VOCAB,), -math.inf)), dict(logit_bias=torch.zeros(3))])
+def test_a_request_that_cannot_be_sampled_ends_alone(bad, temperature, cache):
+    alone = _batcher(cache)
+    want = [alone.submit(GenerationRequest([5, 6], 9, temperature=1.0, seed=3)), alone.submit(GenerationRequest([7], 11))]
+    alone.run_until_idle()
+    worker = BatchingWorker(_batcher(cache))
+    try:
+        beside = [worker.submit(GenerationRequest([5, 6], 9, temperature=1.0, seed=3)), None]
+        broken = worker.submit(GenerationRequest([1, 2, 3], 9, temperature=temperature, **bad))
+        beside[1] = worker.submit(GenerationRequest([7], 11))
+        for w, b in zip(want, beside):
+            assert b.wait(30) == w.tokens and b.finish_reason == "length"
+        broken.wait(30)
+        assert broken.finish_reason.startswith("error: ") and len(broken.tokens) in (0, 2)
+        assert worker.error is None and worker.batcher.pending() == 0
+        cache_state = worker.batcher.decoder.cache
+        assert cache_state is None or cache_state.state.tolist() == [cache_state.blocks, 0, 0, 0]
+    finally:
+        worker.close()
+
+
+@pytest.mark.parametrize("given", [list, torch.Tensor.int, lambda m: m.numpy()])
+def test_a_grammar_may_give_its_mask_in_other_forms(given):
+    even = torch.arange(VOCAB) % 2 == 0
+    batcher = _batcher()
+    request = batcher.submit(GenerationRequest([1, 2, 3], 8, allowed=lambda made: given(even)))
+    batcher.run_until_idle()
+    assert len(request.tokens) == 8 and all(t % 2 == 0 for t in request.tokens)
