@@ -201,6 +201,14 @@ def reply_payload(reply) -> dict:
             "unknown_characters": reply.unknown_characters, "truncated_context": reply.truncated_context}
 
 
+def check_cache_options(batching: int, kv_cache: str, cache_blocks: Optional[int]) -> None:
+    """Only the batching decoder has the block-wise cache: its options without it would be ignored."""
+    if kv_cache != "dense" and batching <= 0:
+        raise ValueError(f"--kv-cache {kv_cache} needs --batching")
+    if cache_blocks is not None and kv_cache == "dense":
+        raise ValueError("--cache-blocks needs --kv-cache fp8 or int8")
+
+
 class Server:
     """The loaded model, with access to its stateful decoder serialised across requests."""
 
@@ -211,6 +219,7 @@ class Server:
                  batching: int = 0, kv_cache: str = "dense", cache_blocks: Optional[int] = None) -> None:
         from ..utils.hardware import choose_precision, detect
 
+        check_cache_options(batching, kv_cache, cache_blocks)
         self.checkpoint, self.adapter, self.device = checkpoint, adapter, device
         self.precision = choose_precision(detect(device.type), precision)
         if sessions is None:
@@ -603,7 +612,12 @@ def build_parser() -> argparse.ArgumentParser:
 def main(argv=None) -> None:
     from ..training.trainer import select_device
 
-    args = build_parser().parse_args(argv)
+    parser = build_parser()
+    args = parser.parse_args(argv)
+    try:
+        check_cache_options(args.batching, args.kv_cache, args.cache_blocks)
+    except ValueError as exc:
+        parser.error(str(exc))
     configure_logging(args.log_format)
     checkpoint, adapter = resolve_model(args.checkpoint, args.adapter, args.run, args.latest, args.runs_dir)
     device = select_device(args.device)

@@ -9,7 +9,7 @@ from pydantic import ValidationError
 from quantaweave_b200 import QuantaWeaveMoEForCausalLM, preset
 from quantaweave_b200.inference.batching import BatchingWorker, ContinuousBatcher, GenerationRequest
 from quantaweave_b200.inference.fast_decode import FastDecoder
-from quantaweave_b200.tools.serve import GenerateRequest
+from quantaweave_b200.tools.serve import GenerateRequest, Server, main
 
 
 def _batcher(cache="int8", rows=3):
@@ -88,3 +88,13 @@ def test_a_grammar_may_give_its_mask_in_other_forms(given):
     request = batcher.submit(GenerationRequest([1, 2, 3], 8, allowed=lambda made: given(even)))
     batcher.run_until_idle()
     assert len(request.tokens) == 8 and all(t % 2 == 0 for t in request.tokens)
+
+
+@pytest.mark.parametrize("options", [dict(kv_cache="fp8"), dict(cache_blocks=8), dict(batching=2, cache_blocks=8)])
+def test_cache_options_that_would_be_ignored_are_refused(options, tmp_path, capsys):
+    with pytest.raises(ValueError, match="batching|kv-cache"):
+        Server(tmp_path / "none", None, torch.device("cpu"), "fp32", **options)
+    flags = [f"--{name.replace('_', '-')}={value}" for name, value in options.items()]
+    with pytest.raises(SystemExit):
+        main(["--checkpoint", str(tmp_path / "none"), "--device", "cpu", *flags])
+    assert "needs" in capsys.readouterr().err
