@@ -501,6 +501,11 @@ class FastDecoder:
             layer.values.zero_()
 
     @property
+    def request_capacity(self) -> int:
+        """Tokens that one request can have: the context, or less where the pool of cache blocks is smaller."""
+        return self.capacity if self.cache is None else min(self.capacity, self.cache.blocks * self.cache.block)
+
+    @property
     def uses_graph(self) -> bool:
         return self.graph is not None
 

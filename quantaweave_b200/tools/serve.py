@@ -273,10 +273,11 @@ class Server:
         tok = session.tokenizer
         prompt = request.prompt
         ids = tok.encode(prompt) or [tok.eos_id]
-        budget = max(1, min(request.tokens, dec.capacity - 1))
-        truncated = len(ids) + budget > dec.capacity
+        context = dec.request_capacity
+        budget = max(1, min(request.tokens, context - 1))
+        truncated = len(ids) + budget > context
         if truncated:
-            ids = ids[-(dec.capacity - budget):]
+            ids = ids[-(context - budget):]
         stops = [x for x in request.stop if x]
         holdback = max((len(x) for x in stops), default=1) - 1
         bias = torch.zeros(dec.vocab)

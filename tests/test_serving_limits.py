@@ -1,10 +1,12 @@
 """What one request asks for must not end the others (CPU forms)."""
 
+import asyncio
 import math
 
 import pytest
 import torch
 from pydantic import ValidationError
+from test_tools_cpu import _train
 
 from quantaweave_b200 import QuantaWeaveMoEForCausalLM, preset
 from quantaweave_b200.inference.batching import BatchingWorker, ContinuousBatcher, GenerationRequest
@@ -98,3 +100,15 @@ def test_cache_options_that_would_be_ignored_are_refused(options, tmp_path, caps
     with pytest.raises(SystemExit):
         main(["--checkpoint", str(tmp_path / "none"), "--device", "cpu", *flags])
     assert "needs" in capsys.readouterr().err
+
+
+def test_a_server_whose_pool_is_smaller_than_a_context_shortens_the_request(tmp_path):
+    _train(tmp_path, steps=1, sequence_length=160)
+    server = Server(tmp_path / "out", None, torch.device("cpu"), "fp32", batching=2, kv_cache="fp8", cache_blocks=1)
+    try:
+        long = asyncio.run(server.generate(GenerateRequest(prompt="the cat " * 10, tokens=40, temperature=0.0, stop=[])))
+        assert long["truncated_context"] and 1 <= long["tokens"] <= 40
+        many = asyncio.run(server.generate(GenerateRequest(prompt="the", tokens=150, temperature=0.0, stop=[])))
+        assert 1 <= many["tokens"] <= 63 and server.worker.error is None
+    finally:
+        server.close()
