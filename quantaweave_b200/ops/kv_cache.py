@@ -140,8 +140,9 @@ def append_kv(k: Tensor, v: Tensor, slot_map: Tensor, k_cache: Tensor, v_cache: 
             size = torch.where(rows.isfinite(), rows.abs(), 0.0).amax(dim=(0, 2))
             e = _exponent(size, cache.dtype)
             if first:
+                # a held scale stays unless the new tokens need a larger one (none is held: 0, or no number)
                 m, o = torch.frexp(scale[b])
-                e = torch.maximum(e, torch.where(m == 0.5, o - 1, o))
+                e = torch.where((scale[b] > 0) & scale[b].isfinite(), torch.maximum(e, torch.where(m == 0.5, o - 1, o)), e)
                 ratio = scale[b] * _power(-e)
                 cache[b, :, :first] = _encode(cache[b, :, :first].float() * ratio[:, None, None], cache.dtype)
             codes = _encode(rows * _power(-e)[None, :, None], cache.dtype)
