@@ -592,7 +592,13 @@ class FastDecoder:
                 lens[0, first_row:first_row + batch], lens[1, first_row:first_row + batch] = start, m
                 cached, new = lens.to(self.device)
                 plan = self.cache.plan(cached, new, batch * m)
-                hidden = self._embed(piece.reshape(-1), plan.positions).view(batch, m, self.hidden)
+                if self.native:
+                    hidden = self._embed(piece.reshape(-1), plan.positions)
+                else:  # the model's own tables: its modules compute in their type, whatever the decoder's
+                    hidden = self.model.token_embedding(piece.reshape(-1))
+                    if self.learned:
+                        hidden = hidden + self.model.position_embedding(plan.positions.long())
+                hidden = hidden.view(batch, m, self.hidden)
                 for li, block in enumerate(self.model.blocks):
                     att = block.attention
                     normed = block.attention_norm(hidden).reshape(batch * m, self.hidden)

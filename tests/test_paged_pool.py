@@ -130,3 +130,18 @@ def test_steps_and_prompts_without_room_are_refused(device):
         dec._prefill(ids[:1, :33], first_row=0)                           # the other row holds two of the three
     with pytest.raises(PoolExhausted, match="at most 8"):
         _decoder(model, device, 1)._prefill(torch.zeros(1, 129, dtype=torch.long))
+
+
+@pytest.mark.parametrize("precision", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("layout", [dict(), dict(norm_type="layernorm", position_embedding="learned", attention_bias=True)])
+def test_cpu_decoding_in_every_precision(layout, precision):
+    cfg = preset("tiny-cpu", max_sequence_length=65, **layout)
+    torch.manual_seed(0)
+    model = QuantaWeaveMoEForCausalLM(cfg).eval()
+    ids = torch.randint(0, 512, (2, 20), generator=torch.Generator().manual_seed(3))
+    logits = []
+    for cache in ("dense", "int8"):
+        dec = FastDecoder(model, torch.device("cpu"), precision, max_batch=2, kv_cache=cache)
+        dec._prefill(ids[:, :-1])
+        logits.append(dec.run_step(ids[:, -1], torch.full((2,), 19)).clone())
+    assert (logits[0] - logits[1]).abs().max() < 0.05 * logits[0].abs().max() + 0.05  # the 8-bit cache's own tolerance
