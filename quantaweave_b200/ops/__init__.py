@@ -45,5 +45,13 @@ def ext():
     return native_required()
 
 
+def refuse_gradients(what: str, *tensors) -> None:
+    """For an operator without a backward pass: an input that asks for a gradient is an error, not a silent zero."""
+    import torch
+
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
+
+
 def debug_bounds() -> bool:
     return os.environ.get("QW_DEBUG_BOUNDS", "0") == "1"

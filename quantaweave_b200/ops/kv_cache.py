@@ -12,6 +12,8 @@ One step of a server, all on the device and without a host synchronisation (so t
     o = cached_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, plan.context_lens, plan.query_start,
                          max_query, max_context)                                            # every layer
 
+None of it has a backward pass: inputs that ask for gradients are refused.
+
 CUDA tensors go to the sm_100a kernels (``csrc/kv_cache.cu``, ``csrc/cached_attention*.cu``); CPU tensors to the plain
 PyTorch forms below. ``inference.paged_cache.PagedKVCache`` holds the storage.
 """
@@ -24,7 +26,7 @@ from typing import NamedTuple, Optional
 import torch
 from torch import Tensor
 
-from . import ext
+from . import ext, refuse_gradients
 
 FORMATS = {"fp8": torch.float8_e4m3fn, "int8": torch.int8}
 _LARGEST = {torch.float8_e4m3fn: 448.0, torch.int8: 127.0}
@@ -121,6 +123,7 @@ def append_kv(k: Tensor, v: Tensor, slot_map: Tensor, k_cache: Tensor, v_cache: 
     that starts at a block's first slot starts the block anew; otherwise the block's scale stays or grows, and the codes
     it holds move to the larger scale. Infinities are stored as the largest code and set no scale; NaN stays NaN in fp8 and
     becomes 0 in int8. Slots of -1 (and outside the cache) are skipped."""
+    refuse_gradients("append_kv", k, v)
     if k_cache.is_cuda:
         ext().append_kv(k, v, slot_map, k_cache, v_cache, k_scale, v_scale)
         return
@@ -162,6 +165,7 @@ def cached_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, k_scale: Tenso
     heads are a multiple of the kv heads (consecutive heads share one). Rows that see no key, and rows of no request, are
     zero. Keys without a block (-1) are not seen. ``max_query`` and ``max_context`` are upper bounds that the host knows;
     they choose the kernel and the split, never the result's meaning. ``scale`` defaults to ``1 / sqrt(head_dim)``."""
+    refuse_gradients("cached_attention", q, k_scale, v_scale)
     d = k_cache.size(-1)
     scale = 1.0 / math.sqrt(d) if scale is None else scale
     if k_cache.is_cuda:

@@ -8,7 +8,7 @@ from typing import Optional
 import torch
 from torch import Tensor
 
-from . import ext
+from . import ext, refuse_gradients
 
 
 def pack_mask(allowed: Tensor) -> Tensor:
@@ -35,7 +35,9 @@ def process_logits(logits: Tensor, *, history: Optional[Tensor] = None, history_
     * ``mask [masks, ceil(vocab / 32)]`` (see ``pack_mask``): ids whose bit is 0 in row ``mask_rows[r]`` become -inf.
 
     Without ``bias_rows`` (``mask_rows``) row ``r`` has bias (mask) row ``r``. Ids outside the vocabulary are ignored. Sums
-    are in 32 bits, rounded once. ``out`` may be ``logits`` itself."""
+    are in 32 bits, rounded once. ``out`` may be ``logits`` itself. There is no backward pass: inputs that ask for gradients
+    are refused."""
+    refuse_gradients("process_logits", logits, repetition, frequency, presence, bias)
     if logits.is_cuda:
         return ext().process_logits(logits, history, history_lens, prompt_lens, repetition, frequency, presence, bias,
                                     bias_rows, mask, mask_rows, out)

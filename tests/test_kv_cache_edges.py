@@ -8,6 +8,7 @@ import torch
 
 from conftest import cuda_ready
 from quantaweave_b200.ops import kv_cache as kvc
+from quantaweave_b200.ops.logits import process_logits
 
 GPU = [pytest.mark.gpu, pytest.mark.skipif(not cuda_ready(), reason="needs a B200")]
 DEVICES = ["cpu", pytest.param("cuda", marks=GPU)]
@@ -27,3 +28,23 @@ def test_a_held_scale_that_is_none_sets_no_scale(held, fmt, device):
     for codes, scales in ((kc, ks), (vc, vs)):
         assert scales.tolist() == [[scale]]
         assert torch.equal(codes[0, 0, 5].cpu().double() * scale, x[0, 0].double())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_inputs_that_ask_for_gradients_are_refused(device):
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    kc = torch.zeros(2, 2, 16, 32, dtype=torch.int8, device=device)
+    s = torch.ones(2, 2, device=device)
+    x = torch.zeros(1, 2, 32, dtype=torch.bfloat16, device=device, requires_grad=True)
+    logits = torch.zeros(1, 40, device=device)
+    ones, bias = (torch.ones(shape, device=device, requires_grad=True) for shape in ((1,), (1, 40)))
+    calls = (lambda: kvc.cached_attention(x, kc, kc, s, s, i32([[0]]), i32([1]), i32([0, 1])),
+             lambda: kvc.append_kv(x, x.detach(), i32([3]), kc, kc.clone(), s, s.clone()),
+             lambda: kvc.append_kv(x.detach(), x, i32([3]), kc, kc.clone(), s, s.clone()),
+             lambda: process_logits(logits.clone().requires_grad_()), lambda: process_logits(logits, bias=bias),
+             lambda: process_logits(logits, history=i32([[1]]), history_lens=i32([1]), repetition=ones))
+    for call in calls:
+        with pytest.raises(RuntimeError, match="no backward"):
+            call()
+        with torch.no_grad():
+            call()
