@@ -738,7 +738,7 @@ qw::KvPages kv_pages(const Tensor& cache, const Tensor& scale, const char* what)
   TORCH_CHECK(D == 32 || D == 64 || D == 128, what, ": head_dim must be 32, 64 or 128, got ", num(D));
   TORCH_CHECK(cache.size(2) % 16 == 0 && cache.size(2) > 0, what, ": a block holds a multiple of 16 tokens");
   TORCH_CHECK(cache.size(0) * cache.size(2) < (int64_t{1} << 31), what, ": slots must fit 32 bits");
-  TORCH_CHECK(cache.size(1) < 32768, what, ": too many heads");
+  TORCH_CHECK(cache.size(1) > 0 && cache.size(1) < 32768, what, ": 1 to 32767 heads");
   TORCH_CHECK(cache.stride(3) == 1 && cache.stride(2) >= D, what, ": a token's numbers must be consecutive");
   bool ok = reinterpret_cast<uintptr_t>(cache.data_ptr()) % 16 == 0;
   for (int i = 0; i < 3; ++i) ok = ok && (cache.size(i) <= 1 || cache.stride(i) % 16 == 0);
@@ -846,7 +846,7 @@ Tensor cached_attention(Tensor q, Tensor kc, Tensor vc, Tensor ks, Tensor vs, Te
   q = aligned_rows(q, "q");
   const int64_t T = q.size(0), Hq = q.size(1), Hkv = kc.size(1), D = kc.size(3), B = context.numel();
   TORCH_CHECK(q.device() == kc.device() && q.size(2) == D, "cached_attention: q must be [tokens, heads, ", num(D), "] on the cache's device");
-  TORCH_CHECK(Hkv > 0 && Hq % Hkv == 0 && Hq < 65536, "cached_attention: the query heads (", num(Hq), ") must be a multiple of the kv heads (", num(Hkv), ")");
+  TORCH_CHECK(Hq % Hkv == 0 && Hq < 65536, "cached_attention: the query heads (", num(Hq), ") must be a multiple of the kv heads (", num(Hkv), ")");
   TORCH_CHECK(T < (int64_t{1} << 30) && T * Hq < (int64_t{1} << 33), "cached_attention: too many tokens");
   TORCH_CHECK(max_query >= 1 && max_context >= 1 && max_query < (int64_t{1} << 31) && max_context < (int64_t{1} << 31),
               "cached_attention: max_query and max_context must be positive");
@@ -859,7 +859,7 @@ Tensor cached_attention(Tensor q, Tensor kc, Tensor vc, Tensor ks, Tensor vs, Te
                   (D <= 1 || out.stride(2) == 1) && reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0 &&
                   (out.size(0) <= 1 || out.stride(0) % 8 == 0) && (out.size(1) <= 1 || out.stride(1) % 8 == 0),
               "cached_attention: out must be bfloat16 like q, its rows consecutive and aligned to 16 bytes");
-  if (T == 0) return out;
+  if (out.numel() == 0) return out;  // no tokens or no heads
   auto ws = torch::empty({qw::cached_attention_workspace(T, B, Hq, Hkv, D, max_query, max_context)},
                          q.options().dtype(torch::kUInt8));
   qw::cached_attention(bptr(q), q.stride(0), q.stride(1), bptr_mut(out), out.stride(0), out.stride(1), pk, pv,

@@ -48,3 +48,26 @@ def test_inputs_that_ask_for_gradients_are_refused(device):
             call()
         with torch.no_grad():
             call()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("tokens", [0, 3])
+def test_no_query_heads_give_an_empty_output(tokens, device):
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    kc = torch.zeros(2, 2, 16, 64, dtype=torch.int8, device=device)
+    s = torch.ones(2, 2, device=device)
+    q = torch.zeros(tokens, 0, 64, dtype=torch.bfloat16, device=device)
+    assert kvc.cached_attention(q, kc, kc, s, s, i32([[0]]), i32([5]), i32([0, tokens])).shape == (tokens, 0, 64)
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif(not cuda_ready(), reason="needs a B200")
+def test_a_cache_without_heads_is_refused():
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    kc = torch.zeros(2, 0, 16, 64, dtype=torch.int8, device="cuda")
+    s = torch.ones(2, 0, device="cuda")
+    x = torch.zeros(3, 0, 64, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(RuntimeError, match="head"):
+        kvc.append_kv(x, x, i32([0, 1, 2]), kc, kc.clone(), s, s.clone())
+    with pytest.raises(RuntimeError, match="head"):
+        kvc.cached_attention(x, kc, kc, s, s, i32([[0]]), i32([5]), i32([0, 3]))
