@@ -40,7 +40,7 @@ struct NewRows {
 };
 __device__ __forceinline__ NewRows new_rows(const CachedAttn& p, int b) {
   const int first = min(max(p.query_start[b], 0), p.T);
-  return {first, min(p.query_start[b + 1], p.T) - first};
+  return {first, min(max(p.query_start[b + 1], 0), p.T) - first};
 }
 
 // The request that row `tok` of q belongs to (the last one that begins at or before it), for a whole warp: the offsets are

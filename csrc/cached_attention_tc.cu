@@ -158,6 +158,13 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 3 - Layout<D>::kGroups) c
     for (int b = lane + 32; b < p.B; b += 32) total += tiles_of(new_rows(p, b));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    // Requests whose rows overlap (offsets that do not ascend) could have more tiles than the grid and the partial results have
+    // room for: those past the bound are left out, and the status word says so.
+    const int most = static_cast<int>(gridDim.x) / p.Hkv;
+    if (total < 0 || total > most) {
+      if (lane == 0) set_status(kBoundsError);
+      total = total < 0 ? 0 : most;
+    }
     const int want = total - 1 - static_cast<int>(blockIdx.x) / p.Hkv;
     const bool publish = args.splits > 1 && blockIdx.x == 0 && blockIdx.y == 0;  // for the join kernel
     if (lane == 0) {
@@ -177,7 +184,7 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 3 - Layout<D>::kGroups) c
         if (lane >= o) x += y;
       }
       const int at = before + x - w;
-      if (want >= at && want < at + w) {
+      if (want >= max(at, 0) && want < at + w) {
         s_item[0] = b;
         s_item[1] = want - at;
         s_item[3] = rows_b.first;
@@ -219,8 +226,9 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 3 - Layout<D>::kGroups) c
 
   // rows that belong to no request are zero
   if (blockIdx.x < static_cast<unsigned>(p.Hkv) && blockIdx.y == 0) {
-    const int first = p.B > 0 ? min(max(p.query_start[0], 0), p.T) : p.T, last = p.B > 0 ? min(p.query_start[p.B], p.T) : p.T;
-    const int rows = first + max(p.T - max(last, first), 0);
+    const int first = p.B > 0 ? min(max(p.query_start[0], 0), p.T) : p.T;
+    const int last = p.B > 0 ? min(max(p.query_start[p.B], first), p.T) : p.T;
+    const int rows = first + p.T - last;
     for (int64_t i = threadIdx.x; i < static_cast<int64_t>(rows) * p.group * (D / 8); i += kThreads) {
       const int r = static_cast<int>(i / (p.group * (D / 8))), c = static_cast<int>(i % (p.group * (D / 8)));
       const int64_t tok = r < first ? r : last + (r - first);
@@ -710,7 +718,7 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 3 - Layout<D>::kGroups) c
 
 // One warp per (token, query head): adds the splits' results in their order.
 template <int D>
-__global__ void __launch_bounds__(128) cached_attn_tc_join_kernel(CachedAttn p, int splits) {
+__global__ void __launch_bounds__(128) cached_attn_tc_join_kernel(CachedAttn p, int tiles_max, int splits) {
   constexpr int kRows = Layout<D>::kRows;
   const int lane = threadIdx.x % 32;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 32;
@@ -722,7 +730,9 @@ __global__ void __launch_bounds__(128) cached_attn_tc_join_kernel(CachedAttn p, 
   const NewRows fresh = p.B > 0 ? new_rows(p, lo) : NewRows{0, 0};
   if (tok < fresh.first || tok >= fresh.first + fresh.n) return;  // zeroed by the attention kernel
   const int r = (tok - fresh.first) * p.group + hq % p.group;
-  const int64_t slot0 = ((p.prefix[lo] + r / kRows) * p.Hkv + hq / p.group) * splits;
+  const int64_t tile = p.prefix[lo] + r / kRows;
+  if (tile < 0 || tile >= tiles_max) return;  // overlapping requests: left out (see the other kernel)
+  const int64_t slot0 = (tile * p.Hkv + hq / p.group) * splits;
   float m = kNone;
   for (int s = lane; s < splits; s += 32) m = fmaxf(m, p.part_ml[((slot0 + s) * kRows + r % kRows) * 2]);
   m = warp_max(m);
@@ -759,7 +769,7 @@ void launch(const CachedAttn& p, int tiles_max, int splits, cudaStream_t stream)
   if (splits > 1) {
     const int64_t rows = static_cast<int64_t>(p.T) * p.Hkv * p.group;
     launch_pdl(cached_attn_tc_join_kernel<D>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), 0, stream,
-               "cached_attention tc join", p, splits);
+               "cached_attention tc join", p, tiles_max, splits);
   }
 }
 

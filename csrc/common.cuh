@@ -31,7 +31,7 @@ enum StatusCode : int {
   kTimeoutAccum = 3,      // epilogue waited too long for an accumulator
   kTimeoutAccumFree = 4,  // MMA waited too long for the epilogue to release TMEM
   kTimeoutPeer = 5,       // a peer flag never arrived
-  kBoundsError = 6,       // QW_DEBUG_BOUNDS check failed
+  kBoundsError = 6,       // an index outside its buffer: QW_DEBUG_BOUNDS checks, row offsets of cached_attention
 };
 
 // One status word per translation unit (internal linkage); the host reads each file's copy.

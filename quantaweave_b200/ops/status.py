@@ -15,7 +15,7 @@ STATUS_MESSAGES = {
     3: "an epilogue waited too long for its accumulator",
     4: "an MMA issuer waited too long for the epilogue to release TMEM",
     5: "a peer rank's flag never arrived (a dead, stalled or diverged rank)",
-    6: "a debug bounds check failed (QW_DEBUG_BOUNDS build)",
+    6: "an index outside its buffer was refused (QW_DEBUG_BOUNDS build, or row offsets of cached_attention that overlap)",
 }
 PEER_TIMEOUT = 5
 

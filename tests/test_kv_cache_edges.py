@@ -71,3 +71,27 @@ def test_a_cache_without_heads_is_refused():
         kvc.append_kv(x, x, i32([0, 1, 2]), kc, kc.clone(), s, s.clone())
     with pytest.raises(RuntimeError, match="head"):
         kvc.cached_attention(x, kc, kc, s, s, i32([[0]]), i32([5]), i32([0, 3]))
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif(not cuda_ready(), reason="needs a B200")
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("starts,over", [([0, 1000] * 4, True), ([0, 1000, 990, 1000, 1, 1000], True), ([0, 500, 700, 300], False),
+                                         ([7, 1000, -9], False), ([0, 1000, 1400], False)])
+def test_row_offsets_that_do_not_ascend_stay_inside_the_buffers(starts, over, dim):
+    """Overlapping requests have more row tiles than the rows of q allow: the prompt kernel leaves the surplus out and sets the
+    status word, the rest of the output is that of some request; the next call is as ever."""
+    from quantaweave_b200.ops import ext
+
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    requests, tokens = len(starts) - 1, 1000
+    kc = torch.ones(64, 1, 16, dim, dtype=torch.int8, device="cuda")
+    s = torch.ones(64, 1, device="cuda")
+    table = torch.arange(64, device="cuda", dtype=torch.int32).expand(requests, 64).contiguous()
+    q = torch.randn(tokens, 1, dim, generator=torch.Generator("cuda").manual_seed(0), device="cuda").bfloat16()
+    out = torch.zeros_like(q)
+    kvc.cached_attention(q, kc, kc, s, s, table, i32([1000] * requests), i32(starts), tokens, 1024, out=out)
+    assert (ext().read_status(True) != 0) == over
+    assert ((out == 1) | (out == 0)).all()  # every value is 1
+    o = kvc.cached_attention(q, kc, kc, s, s, table[:1], i32([1000]), i32([0, tokens]), tokens, 1024)
+    assert (o == 1).all() and ext().read_status(True) == 0
