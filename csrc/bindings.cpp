@@ -854,6 +854,8 @@ Tensor cached_attention(Tensor q, Tensor kc, Tensor vc, Tensor ks, Tensor vs, Te
   check_ints(context, B, kc.device(), "context_lens");
   check_ints(query_start, B + 1, kc.device(), "query_start");
   check_table(table, B, kc.device());
+  // positions are 32-bit numbers, and the kernels step past the last one by less than 2^16
+  TORCH_CHECK(table.size(1) <= ((int64_t{1} << 31) - (int64_t{1} << 16)) / kc.size(2), "cached_attention: a row of block_table must stand for fewer than 2^31 - 2^16 tokens");
   Tensor out = out_ && out_->defined() ? *out_ : torch::empty({T, Hq, D}, q.options());
   TORCH_CHECK(out.device() == kc.device() && out.scalar_type() == torch::kBFloat16 && out.sizes() == q.sizes() &&
                   (D <= 1 || out.stride(2) == 1) && reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0 &&

@@ -95,3 +95,20 @@ def test_row_offsets_that_do_not_ascend_stay_inside_the_buffers(starts, over, di
     assert ((out == 1) | (out == 0)).all()  # every value is 1
     o = kvc.cached_attention(q, kc, kc, s, s, table[:1], i32([1000]), i32([0, tokens]), tokens, 1024)
     assert (o == 1).all() and ext().read_status(True) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif(not cuda_ready(), reason="needs a B200")
+def test_a_table_of_more_tokens_than_32_bits_is_refused():
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    block = 1 << 20
+    kc = torch.zeros(1, 1, block, 32, dtype=torch.int8, device="cuda")
+    s = torch.ones(1, 1, device="cuda")
+    q = torch.zeros(1, 1, 32, dtype=torch.bfloat16, device="cuda")
+    for width, fits in ((2047, True), (2048, False), (4096, False)):
+        table = torch.zeros(1, width, dtype=torch.int32, device="cuda")
+        if fits:
+            kvc.cached_attention(q, kc, kc, s, s, table, i32([3]), i32([0, 1]), 1, 3)
+        else:
+            with pytest.raises(RuntimeError, match="tokens"):
+                kvc.cached_attention(q, kc, kc, s, s, table, i32([3]), i32([0, 1]), 1, 3)
