@@ -807,12 +807,11 @@ template <int FMT, int D, int ROWS, bool CLUSTERS>
 void launch(const CachedAttn& p, int parts, cudaStream_t stream) {
   auto kernel = cached_attn_kernel<FMT, D, ROWS, CLUSTERS>;
   constexpr int smem = Layout<D, ROWS>::kTotal + (CLUSTERS ? Layout<D, ROWS>::kPart : 0);
-  static const bool configured = [&] {
+  static std::atomic<uint64_t> configured{0};
+  once_per_device(configured, current_device(), [&] {
     check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cached_attention smem");
     if (CLUSTERS) check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "cached_attention cluster");
-    return true;
-  }();
-  (void)configured;
+  });
   if constexpr (CLUSTERS) {
     launch_pdl_clusters(kernel, dim3(static_cast<unsigned>(p.B) * p.Hkv * parts), dim3(kThreads), parts, smem, stream,
                         "cached_attention", p, parts);

@@ -758,12 +758,11 @@ __global__ void __launch_bounds__(128) cached_attn_tc_join_kernel(CachedAttn p, 
 template <int FMT, int D>
 void launch(const CachedAttn& p, int tiles_max, int splits, cudaStream_t stream) {
   auto kernel = cached_attn_tc_kernel<FMT, D>;
-  static const bool configured = [&] {
+  static std::atomic<uint64_t> configured{0};
+  once_per_device(configured, current_device(), [&] {
     check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kTotal),
                "cached_attention tc smem");
-    return true;
-  }();
-  (void)configured;
+  });
   launch_pdl(kernel, dim3(static_cast<unsigned>(tiles_max) * p.Hkv, splits), dim3(Layout<D>::kThreads), Layout<D>::kTotal, stream,
              "cached_attention tc", TcArgs{p, splits});
   if (splits > 1) {

@@ -469,13 +469,12 @@ void plan_blocks(const int* cached, const int* fresh, const int* state, int* tab
   PlanArgs a{cached, fresh, state, table, table_stride, free_blocks, capacity, B, width, block, tokens,
              query_start, context, positions, slots, state_out, missing};
   const int grid = std::min(148, std::max((tokens + kPlanTokens - 1) / kPlanTokens, (B + 63) / 64));
-  static const bool configured = [] {
+  static std::atomic<uint64_t> configured{0};
+  once_per_device(configured, current_device(), [] {
     check_cuda(cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     static_cast<int>((5 * plan_max_requests() + 1) * sizeof(int))),
                "plan_blocks smem");
-    return true;
-  }();
-  (void)configured;
+  });
   launch_pdl(plan_kernel, dim3(std::max(grid, 1)), dim3(kPlanThreads), static_cast<size_t>(5 * B + 1) * sizeof(int), stream,
              "plan_blocks", a);
 }

@@ -7,8 +7,16 @@
 #include <utility>
 
 #include "launchers.h"
+#include "once.h"
 
 namespace qw {
+
+// The device that launches and settings go to.
+inline int current_device() {
+  int device = 0;
+  check_cuda(cudaGetDevice(&device), "current device");
+  return device;
+}
 
 // In clusters of `cluster` consecutive blocks.
 template <typename... KArgs, typename... Args>
