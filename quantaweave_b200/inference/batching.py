@@ -208,7 +208,7 @@ class ContinuousBatcher:
             logits = logits + request.logit_bias
         if request.temperature <= 0:
             token = int(logits.argmax())
-            if logits[token] == float("-inf"):
+            if (request.allowed is not None or request.logit_bias is not None) and logits[token].item() == float("-inf"):
                 raise ValueError("no token is allowed")
             return token
         filtered = filter_logits(logits[None] / request.temperature, request.top_k, request.top_p)[0]
