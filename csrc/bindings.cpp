@@ -717,6 +717,13 @@ void rope_append(Tensor qkv, Tensor pos, int64_t Hq, int64_t Hkv, Tensor cos_t, 
 // own (linked statically) next to torch's.
 std::string num(int64_t n) { return std::to_string(n); }
 
+// For an operator without a backward pass (the Python wrapper's check would cost half a microsecond).
+void refuse_gradients(const char* what, std::initializer_list<const Tensor*> inputs) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor* t : inputs)
+    TORCH_CHECK(!t->defined() || !t->requires_grad(), what, " has no backward pass: call it under torch.no_grad() or on detached tensors");
+}
+
 // Rows [T, heads, D] whose 16-byte pieces are aligned, or an aligned copy of them (a size-1 dimension's stride is free).
 Tensor aligned_rows(const Tensor& x, const char* what) {
   TORCH_CHECK(x.is_cuda() && x.dim() == 3, what, " must be a CUDA tensor [tokens, heads, head_dim]");
@@ -821,6 +828,7 @@ void release_blocks(Tensor keep_lens, Tensor state, Tensor table, Tensor free_bl
 }
 
 void append_kv(Tensor k, Tensor v, Tensor slots, Tensor kc, Tensor vc, Tensor ks, Tensor vs) {
+  refuse_gradients("append_kv", {&k, &v});
   check_caches(kc, vc);
   const int fmt = kv_format(kc);
   const auto pk = kv_pages(kc, ks, "k_cache"), pv = kv_pages(vc, vs, "v_cache");
@@ -839,6 +847,7 @@ void append_kv(Tensor k, Tensor v, Tensor slots, Tensor kc, Tensor vc, Tensor ks
 
 Tensor cached_attention(Tensor q, Tensor kc, Tensor vc, Tensor ks, Tensor vs, Tensor table, Tensor context,
                         Tensor query_start, int64_t max_query, int64_t max_context, double scale, OptT out_) {
+  refuse_gradients("cached_attention", {&q, &ks, &vs});
   check_caches(kc, vc);
   const int fmt = kv_format(kc);
   const auto pk = kv_pages(kc, ks, "k_cache"), pv = kv_pages(vc, vs, "v_cache");
@@ -890,6 +899,9 @@ Tensor process_logits(Tensor logits, OptT history, OptT history_lens, OptT promp
                       OptT presence, OptT bias, OptT bias_rows, OptT mask, OptT mask_rows, OptT out_) {
   TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.size(1) <= 1 || logits.stride(1) == 1),
               "process_logits: logits must be a CUDA tensor [rows, vocab] with unit inner stride");
+  const Tensor none;
+  auto given = [&](const OptT& t) { return t ? &*t : &none; };
+  refuse_gradients("process_logits", {&logits, given(repetition), given(frequency), given(presence), given(bias)});
   const auto dev = logits.device();
   const int64_t rows = logits.size(0), vocab = logits.size(1);
   TORCH_CHECK(rows <= 65535 && vocab < (int64_t{1} << 30), "process_logits: at most 65535 rows");

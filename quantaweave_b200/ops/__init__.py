@@ -46,7 +46,8 @@ def ext():
 
 
 def refuse_gradients(what: str, *tensors) -> None:
-    """For an operator without a backward pass: an input that asks for a gradient is an error, not a silent zero."""
+    """For an operator without a backward pass: an input that asks for a gradient is an error, not a silent zero. (CPU forms;
+    the bindings check for themselves.)"""
     import torch
 
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):

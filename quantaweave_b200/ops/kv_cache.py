@@ -123,10 +123,10 @@ def append_kv(k: Tensor, v: Tensor, slot_map: Tensor, k_cache: Tensor, v_cache: 
     that starts at a block's first slot starts the block anew; otherwise the block's scale stays or grows, and the codes
     it holds move to the larger scale. Infinities are stored as the largest code and set no scale; NaN stays NaN in fp8 and
     becomes 0 in int8. Slots of -1 (and outside the cache) are skipped."""
-    refuse_gradients("append_kv", k, v)
     if k_cache.is_cuda:
         ext().append_kv(k, v, slot_map, k_cache, v_cache, k_scale, v_scale)
         return
+    refuse_gradients("append_kv", k, v)
     block = k_cache.size(2)
     slots = slot_map.tolist()
     t = 0
@@ -165,7 +165,6 @@ def cached_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, k_scale: Tenso
     heads are a multiple of the kv heads (consecutive heads share one). Rows that see no key, and rows of no request, are
     zero. Keys without a block (-1) are not seen. ``max_query`` and ``max_context`` are upper bounds that the host knows;
     they choose the kernel and the split, never the result's meaning. ``scale`` defaults to ``1 / sqrt(head_dim)``."""
-    refuse_gradients("cached_attention", q, k_scale, v_scale)
     d = k_cache.size(-1)
     scale = 1.0 / math.sqrt(d) if scale is None else scale
     if k_cache.is_cuda:
@@ -173,6 +172,7 @@ def cached_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, k_scale: Tenso
                                       max(q.size(0), 1) if max_query is None else max_query,
                                       block_table.size(1) * k_cache.size(2) if max_context is None else max_context,
                                       scale, out)
+    refuse_gradients("cached_attention", q, k_scale, v_scale)
     heads, group = q.size(1), q.size(1) // k_cache.size(1)
     if out is None:
         out = torch.empty_like(q)

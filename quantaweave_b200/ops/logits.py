@@ -37,10 +37,10 @@ def process_logits(logits: Tensor, *, history: Optional[Tensor] = None, history_
     Without ``bias_rows`` (``mask_rows``) row ``r`` has bias (mask) row ``r``. Ids outside the vocabulary are ignored. Sums
     are in 32 bits, rounded once. ``out`` may be ``logits`` itself. There is no backward pass: inputs that ask for gradients
     are refused."""
-    refuse_gradients("process_logits", logits, repetition, frequency, presence, bias)
     if logits.is_cuda:
         return ext().process_logits(logits, history, history_lens, prompt_lens, repetition, frequency, presence, bias,
                                     bias_rows, mask, mask_rows, out)
+    refuse_gradients("process_logits", logits, repetition, frequency, presence, bias)
     if history is None and not (repetition is None and frequency is None and presence is None):
         raise RuntimeError("process_logits: penalties need the history")
     if history is not None and history_lens is None:

@@ -112,3 +112,29 @@ def test_a_table_of_more_tokens_than_32_bits_is_refused():
         else:
             with pytest.raises(RuntimeError, match="tokens"):
                 kvc.cached_attention(q, kc, kc, s, s, table, i32([3]), i32([0, 1]), 1, 3)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+@pytest.mark.parametrize("new", [1, 6, 200])
+@pytest.mark.parametrize("dim", [32, 64, 128])
+def test_query_numbers_far_below_their_rows_largest_count(dim, new, fmt, device):
+    """A query row whose largest number meets keys of zero, and two numbers 2^-20 of it, unlike in their last bit, that meet large
+    keys of opposite sign: the score is that last bit. The tolerance is that of the other attention tests."""
+    from test_kv_cache import _attend_oracle, _check, _requests
+
+    g = torch.Generator().manual_seed(dim + new)
+    table, context, starts, blocks = _requests([(40, new)], 16, g)
+    codes = torch.zeros(blocks, 2, 16, dim)
+    codes[..., 1] = 120 * (torch.rand(blocks, 2, 16, generator=g) < 0.3)
+    codes[..., 2] = -codes[..., 1]
+    kc = codes.to(kvc.FORMATS[fmt])
+    vc = torch.randint(-100, 101, codes.shape, generator=g).float().to(kvc.FORMATS[fmt])
+    ks, vs = torch.full((blocks, 2), 2.0 ** 19 * math.sqrt(dim / 64)), torch.full((blocks, 2), 2.0 ** -6)
+    q = torch.zeros(new, 4, dim)
+    q[..., 0], q[..., 1], q[..., 2] = 64.0, 64 * 2.0 ** -20 * 255 / 128, 64 * 2.0 ** -20 * 254 / 128
+    q = q.bfloat16()
+    want, size = _attend_oracle(q, kc, vc, ks, vs, table, context, starts, dim ** -0.5)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    o = kvc.cached_attention(*(t.to(device) for t in (q, kc, vc, ks, vs, table)), i32(context), i32(starts), new, context[0])
+    _check(o, want, size)
