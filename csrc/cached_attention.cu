@@ -418,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D, ROWS>::kPerSm) cached_attn
     const int lim_first = now.lim_of(p, 0), lim_last = now.lim_of(p, rows - 1);
     const int key_end = now.key_end(p);
 
-    // ---- query rows as f16 fragments: each row divided by a power of two that brings its largest number to [1, 2)
+    // ---- query rows as f16 fragments, each divided by a power of two (kQueryTop)
     uint32_t q[kQInSmem ? 1 : N][D / 16][2];
     float unit[N][2];  // of the rows 2t, 2t + 1: what a product of codes and fragments is worth, but for the key's scale
     auto load_q = [&](int n, uint32_t (*frag)[2]) {  // row g of tile n; returns the row's unit
@@ -449,15 +449,15 @@ __global__ void __launch_bounds__(kThreads, Layout<D, ROWS>::kPerSm) cached_attn
         for (int i = 0; i < D / 4; ++i) x[i] = 0.f;
       }
       m = quad_max(m);
-      const int e = min(max(static_cast<int>(__float_as_uint(m) >> 23) - 127, -100), 126);
+      const int e = min(max(static_cast<int>(__float_as_uint(m) >> 23) - 127, -100), 127);
       const bool fine = m > 0.f && m <= 3.4028234e38f;  // zero or infinite rows as they are
-      const float inv = fine ? exp2i(-e) : 1.f;
+      const float inv = fine ? exp2i(kQueryTop - e) : 1.f;
 #pragma unroll
       for (int s = 0; s < D / 16; ++s) {
         frag[s][0] = pack_f16(x[4 * s] * inv, x[4 * s + 1] * inv);
         frag[s][1] = pack_f16(x[4 * s + 2] * inv, x[4 * s + 3] * inv);
       }
-      return (fine ? exp2i(e) : 1.f) * p.scale * kLog2e;
+      return (fine ? exp2i(e - kQueryTop) : 1.f) * p.scale * kLog2e;
     };
     if constexpr (!kQInSmem) {
 #pragma unroll

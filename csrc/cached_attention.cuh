@@ -34,6 +34,12 @@ struct CachedAttn {
   int64_t* prefix;  // [B + 1]
 };
 
+// A query row enters f16 divided by a power of two that brings its largest number to [2^14, 2^15): bf16 numbers down to 2^-31 of
+// it are then exact in f16 (8 bits, multiples of 2^-24), and smaller ones are off by at most 2^-39 of it, far below the
+// rounding of the 32-bit sums. (Brought to [1, 2), numbers below 2^-17 of the largest lost bits, which counted where
+// large keys met them.) A sum of 128 products with codes stays below 2^15 * 448 * 128 < 2^31.
+constexpr int kQueryTop = 14;
+
 // The rows of q that belong to request b; offsets outside [0, T] are cut, so that no row outside q is touched.
 struct NewRows {
   int first, n;

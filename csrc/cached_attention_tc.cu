@@ -484,7 +484,7 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 3 - Layout<D>::kGroups) c
       return __all_sync(0xffffffffu, mbar_wait(my_met, phase & 1, kTimeoutAccum)) != 0;
     };
     {
-      // Query rows in f16, each divided by a power of two that brings its largest number to [1, 2). D / 8 lanes read a row.
+      // Query rows in f16, each divided by a power of two (kQueryTop). D / 8 lanes read a row.
       constexpr int LPR = D / 8, RPI = 32 / LPR, NI = 16 / RPI;  // a warp has 16 rows
       const int c = lane % LPR, w16 = (warp - 4) % 8;
       uint4 w[NI];
@@ -506,14 +506,14 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 3 - Layout<D>::kGroups) c
                         fmaxf(fmaxf(fabsf(f2.x), fabsf(f2.y)), fmaxf(fabsf(f3.x), fabsf(f3.y))));
 #pragma unroll
         for (int o = LPR / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const int e = min(max(static_cast<int>(__float_as_uint(m) >> 23) - 127, -100), 126);
+        const int e = min(max(static_cast<int>(__float_as_uint(m) >> 23) - 127, -100), 127);
         const bool fine = m > 0.f && m <= 3.4028234e38f;  // zero or infinite rows as they are
-        const float inv = fine ? exp2i(-e) : 1.f;
+        const float inv = fine ? exp2i(kQueryTop - e) : 1.f;
         *reinterpret_cast<uint4*>(smem + g * L::kQBytes + (c / 8) * (kGroupRows * 128) + in * 128 + ((c % 8) ^ (in & 7)) * 16) =
             make_uint4(pack_f16(f0.x * inv, f0.y * inv), pack_f16(f1.x * inv, f1.y * inv), pack_f16(f2.x * inv, f2.y * inv),
                        pack_f16(f3.x * inv, f3.y * inv));
         if (c < 2)  // for the two threads of the row
-          s_join[(g * 2 + c) * kGroupRows + in] = (fine ? exp2i(e) : 1.f) * p.scale * kLog2e;
+          s_join[(g * 2 + c) * kGroupRows + in] = (fine ? exp2i(e - kQueryTop) : 1.f) * p.scale * kLog2e;
       }
       fence_async_smem();
       __syncwarp();

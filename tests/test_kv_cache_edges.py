@@ -138,3 +138,26 @@ def test_query_numbers_far_below_their_rows_largest_count(dim, new, fmt, device)
     i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
     o = kvc.cached_attention(*(t.to(device) for t in (q, kc, vc, ks, vs, table)), i32(context), i32(starts), new, context[0])
     _check(o, want, size)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("new", [1, 200])
+def test_query_rows_at_the_ends_of_bf16(new, device):
+    """Rows whose largest number is the largest of bf16, and rows of the smallest normal one, with a scale that makes their scores
+    ordinary."""
+    from test_kv_cache import _attend_oracle, _check, _requests
+
+    g = torch.Generator().manual_seed(new)
+    table, context, starts, blocks = _requests([(40, new)], 16, g)
+    kc = torch.randint(-127, 128, (blocks, 2, 16, 64), generator=g).to(torch.int8)
+    vc = torch.randint(-127, 128, (blocks, 2, 16, 64), generator=g).to(torch.int8)
+    vs = torch.full((blocks, 2), 2.0 ** -6)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    for top, unit in ((torch.finfo(torch.bfloat16).max, 2.0 ** -120), (2.0 ** -100, 2.0 ** 108)):
+        q = (torch.rand(new, 4, 64, generator=g) * 2 - 1) * top
+        q[..., 3] = top
+        q = q.bfloat16()
+        ks = torch.full((blocks, 2), unit * 2.0 ** -17)
+        args = (q, kc, vc, ks, vs, table)
+        want, size = _attend_oracle(*args, context, starts, 0.125)
+        _check(kvc.cached_attention(*(t.to(device) for t in args), i32(context), i32(starts), new, context[0], 0.125), want, size)
