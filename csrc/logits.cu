@@ -128,13 +128,11 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(LogitsArgs a, int rang
     __syncthreads();
   }
 
-  // A product with the reciprocal (one rounding more, 2^-24, before the result's own): a division is 20 instructions, and most
-  // warps have a penalised id among their numbers. A reciprocal that overflows would lose finite quotients.
-  const float inv = 1.f / rep;
+  // A division, although most warps have a penalised id among their numbers: a product with the reciprocal would round once
+  // more.
   auto penalty = [&](float x, uint32_t c) {
     if (!c) return x;
-    if (isinf(inv) && x > 0.f) x /= rep;
-    else x *= x > 0.f ? inv : rep;
+    x = x > 0.f ? x / rep : x * rep;
     const uint32_t made = c & ~kPrompt;
     return made ? x - static_cast<float>(made) * freq - pres : x;
   };
