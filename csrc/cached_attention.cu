@@ -12,15 +12,18 @@
 // holds the column of, 16 bytes of each of the four values that it holds the contraction rows of). They are widened to
 // f16, which holds every code exactly, next to the MMA; the block's scales are applied in 32 bits, the key's to the
 // scores and the value's to the probabilities (relative to the largest value scale so far, in steps of two, so that the
-// f16 probabilities keep their 11 bits).
+// f16 probabilities keep their 11 bits). That they are f16 is a choice: the second product then runs at the tensor cores' f16
+// rate beside exact codes, and 11 bits are eight times finer than the bf16 result (error against 64 bits 0.0016 of the
+// result's norm, as with 32-bit probabilities; the two differ by 0.0005 to 0.0009, in last bits of bf16). Sums of the
+// probabilities are of the unrounded ones.
 //
 // The work is the list of all (request, row tile, kv head) items times their 64-key units. It is cut into equal
 // consecutive ranges, one per resident block of threads, so ragged lengths cost nothing; a range that ends inside an item
 // leaves a partial result (at most two per block), which the join kernel adds up in a fixed order. Where there is little
 // work (cluster_parts), a cluster of blocks takes each (request, kv head) instead and adds its results up itself.
 //
-// Measured on a B200, single tokens, 32 heads on 8 of 128, fp8: 64 requests of every length up to 16384 tokens 111-117 us,
-// 5.4-5.7 TB/s, 83-87% of the measured copy rate; one of 600 tokens 7.7 us, latency alone (the launch, then lengths, table,
+// Measured on a B200, single tokens, 32 heads on 8 of 128, fp8: 64 requests of every length up to 16384 tokens 111-118 us,
+// 5.3-5.7 TB/s, 82-87% of the measured copy rate; one of 600 tokens 7.5-7.9 us, latency alone (the launch, then lengths, table,
 // codes and products one after another). 32 requests of up to 2047 tokens, 16 kv heads of 64: 25 us, where the two launches
 // and the pieces' ends (512 items, two ends per range) take most of it.
 #include <algorithm>

@@ -379,8 +379,9 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, int kv, int h, i
 // of threads per (run, head) and 4 KB of each run in flight, prompts ran at 16% of HBM; with a warp per pair the runs are
 // looked for once per eight pairs.
 // Measured on a B200: 24 prompts of 14900 tokens in all, bf16 to int8, 16 heads of 64 each for keys and values: 24.2 us,
-// 3.8 TB/s, 58% of the measured copy rate (the rest is the arithmetic per number: magnitude, product, rounding, clamp and
-// packing); 32 single tokens 4.4 us, one launch's latency.
+// 3.8 TB/s, 58% of the measured copy rate. No unit is full: the issue slots are busy for 49%, a third of the warps is resident
+// (80 registers a thread), so too few bytes are on their way; and the pairs do not divide evenly (there, half of the blocks
+// take three turns and half one). 32 single tokens 4.4 us, one launch's latency.
 template <int FMT, int D, int NT>
 __global__ void __launch_bounds__(kAppendThreads, 3) append_kernel(AppendArgs a) {
   constexpr int kTeams = kAppendThreads / NT;

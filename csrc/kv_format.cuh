@@ -17,7 +17,9 @@ namespace qw {
 
 enum KvFormat : int { kKvFp8 = 0, kKvInt8 = 1 };
 
-constexpr int kMinExponent = -64;  // amax <= 448 * 2^-64 is stored as (almost) zero
+// Scales stop shrinking here: a code's step is then 2^-64 (int8) or at least 2^-73 (e4m3, whose subnormals are multiples of
+// 2^-9), and magnitudes up to half of that become zero.
+constexpr int kMinExponent = -64;
 
 template <int FMT>
 struct Kv;

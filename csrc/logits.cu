@@ -12,9 +12,9 @@
 // eight numbers apart from lane to lane, the biases kept L1 busy for 79% of the time). Bound by HBM for many rows, by latency
 // for one.
 //
-// Measured on a B200: 256 rows of 50257 bf16 logits with histories of up to 4096 ids, biases and masks for some rows: 23 us,
-// 2.5 TB/s, 38% of the measured copy rate: the parts of a block follow one another (clear the counts, count, then the
-// logits), and each block scans its row's history anew. One row of 32000 fp32 logits: 5.9 us a call, of which 3.0 on the
+// Measured on a B200: 256 rows of 50257 bf16 logits with histories of up to 4096 ids, biases and masks for some rows: 23.4 us,
+// 2.4 TB/s, 37% of the measured copy rate: the parts of a block follow one another (clear the counts, count, then the
+// logits), and each block scans its row's history anew. One row of 32000 fp32 logits: 6 us a call, of which 3.1 on the
 // device.
 #include <cuda_fp16.h>
 
@@ -198,8 +198,9 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(LogitsArgs a, int rang
 
 template <typename T>
 void launch(const LogitsArgs& a, cudaStream_t stream) {
-  // Equal ranges of at most four pieces per thread: each range scans the row's history anew (256 rows of 50257: 23.1 us,
-  // 23.5 with two). Of two or one where that leaves fewer than two blocks for an SM (16 rows: 5.2 us, 5.6 with four).
+  // Equal ranges of at most four pieces per thread: each range scans the row's history anew (256 rows of 32000 fp32 logits:
+  // 13.9 us, 17.1 with two; 256 of 50257 bf16: 23.4 and 22.1). Of two or one where that leaves fewer than two blocks for an SM
+  // (16 rows of 50257 bf16: 6.0 us, 8.4 with four; one row 5.2 and 9.2).
   constexpr int VE = 16 / static_cast<int>(sizeof(T));
   int most = kThreads * kPieces * VE;
   while (most > kThreads * VE && static_cast<int64_t>(a.rows) * ((a.vocab + most - 1) / most) < 148 * 2) most /= 2;
